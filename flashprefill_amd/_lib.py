@@ -23,6 +23,9 @@ FP_E_LAUNCH = -3
 FP_DTYPE_BF16 = 0
 FP_DTYPE_F16 = 1
 FP_DTYPE_F32 = 2
+FP_CACHE_16BIT = 0
+FP_CACHE_E4M3 = 1
+FP_CACHE_E5M2 = 2
 FP_STATUS_SEQ_TOO_LONG = 1
 FP_STATUS_BAD_CU_SEQLENS = 2
 ABI_VERSION = 6
@@ -31,7 +34,8 @@ EXPORTS = (
     "fp_workspace_layout", "fp_workspace_bytes", "fp_flashprefill", "fp_plan", "fp_pool_k",
     "fp_search", "fp_select", "fp_sparse_attn_fwd", "fp_read_status", "fp_last_error",
     "fp_abi_version", "fp_flashprefill_noalloc", "fp_kv_cache_write", "fp_rope_qk",
-    "fp_paged_attention", "fp_paged_workspace_bytes",
+    "fp_paged_attention", "fp_paged_workspace_bytes", "fp_kv_cache_write_fp8",
+    "fp_kv_cache_gather", "fp_paged_attention_fp8", "fp_paged_fp8_workspace_bytes",
 )
 NOALLOC_SCRATCH_BYTES = 96 * 1024 * 1024
 
@@ -124,6 +128,38 @@ class FpPagedArgs(ctypes.Structure):
     ]
 
 
+class FpKvScales(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p), ("stride_block", ctypes.c_int64),
+        ("stride_head", ctypes.c_int64), ("per_slot", ctypes.c_int32),
+    ]
+
+
+class FpKvCacheFp8Args(ctypes.Structure):
+    _fields_ = [
+        ("base", FpKvCacheArgs), ("k_scale", FpKvScales), ("v_scale", FpKvScales),
+        ("format", ctypes.c_int32),
+    ]
+
+
+class FpKvGatherArgs(ctypes.Structure):
+    _fields_ = [
+        ("base", FpKvCacheArgs), ("k_scale", FpKvScales), ("v_scale", FpKvScales),
+        ("format", ctypes.c_int32), ("batch", ctypes.c_int32), ("table_width", ctypes.c_int32),
+        ("cu_is64", ctypes.c_int32), ("table_is64", ctypes.c_int32),
+        ("starts_is64", ctypes.c_int32),
+        ("cu_seqlens", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+    ]
+
+
+class FpPagedFp8Args(ctypes.Structure):
+    _fields_ = [
+        ("base", FpPagedArgs), ("k_scale", FpKvScales), ("v_scale", FpKvScales),
+        ("format", ctypes.c_int32),
+    ]
+
+
 _LIB = None
 
 
@@ -151,13 +187,19 @@ def load(path: Path = LIB_PATH) -> ctypes.CDLL:
     lib.fp_paged_attention.argtypes = [ctypes.POINTER(FpPagedArgs), vp, vp]
     lib.fp_paged_workspace_bytes.argtypes = [ctypes.POINTER(FpPagedArgs)]
     lib.fp_paged_workspace_bytes.restype = ctypes.c_size_t
+    lib.fp_kv_cache_write_fp8.argtypes = [ctypes.POINTER(FpKvCacheFp8Args), vp]
+    lib.fp_kv_cache_gather.argtypes = [ctypes.POINTER(FpKvGatherArgs), vp]
+    lib.fp_paged_attention_fp8.argtypes = [ctypes.POINTER(FpPagedFp8Args), vp, vp]
+    lib.fp_paged_fp8_workspace_bytes.argtypes = [ctypes.POINTER(FpPagedFp8Args)]
+    lib.fp_paged_fp8_workspace_bytes.restype = ctypes.c_size_t
     lib.fp_search.argtypes = [P, vp, vp, vp, vp]
     lib.fp_select.argtypes = [P, vp, vp, vp, vp]
     lib.fp_read_status.argtypes = [P, vp, vp, ctypes.POINTER(ctypes.c_uint32)]
     lib.fp_last_error.restype = ctypes.c_char_p
     lib.fp_abi_version.restype = ctypes.c_int
     for name in EXPORTS:
-        if name not in ("fp_workspace_bytes", "fp_paged_workspace_bytes", "fp_last_error", "fp_abi_version"):
+        if not name.endswith("_workspace_bytes") and name not in (
+                "fp_last_error", "fp_abi_version"):
             getattr(lib, name).restype = ctypes.c_int
     if lib.fp_abi_version() != ABI_VERSION:
         raise RuntimeError(f"{path.name} ABI {lib.fp_abi_version()} != expected {ABI_VERSION}")

@@ -596,6 +596,157 @@ PagedSplit paged_split(const fp_paged_args* a) {
   return r;
 }
 
+fp::KvCacheArgs cache_args(const fp_kv_cache_args* a) {
+  fp::KvCacheArgs k;
+  k.key = a->key;
+  k.value = a->value;
+  k.k_stride_tok = a->k_stride_tok;
+  k.k_stride_head = a->k_stride_head;
+  k.v_stride_tok = a->v_stride_tok;
+  k.v_stride_head = a->v_stride_head;
+  k.key_cache = a->key_cache;
+  k.value_cache = a->value_cache;
+  k.kc_stride_block = a->kc_stride_block;
+  k.kc_stride_slot = a->kc_stride_slot;
+  k.kc_stride_head = a->kc_stride_head;
+  k.vc_stride_block = a->vc_stride_block;
+  k.vc_stride_slot = a->vc_stride_slot;
+  k.vc_stride_head = a->vc_stride_head;
+  k.slot_mapping = a->slot_mapping;
+  k.num_tokens = a->num_tokens;
+  k.num_slots = a->num_blocks * a->block_size;
+  k.block_size = a->block_size;
+  k.num_kv_heads = a->num_kv_heads;
+  k.elem_bytes = 2;
+  k.row_bytes = a->head_dim * 2;
+  return k;
+}
+
+// Argument block of the paged kernels; partials behind each other in the workspace.
+fp::PagedArgs paged_args(const fp_paged_args* a, const PagedSplit& sp, void* ws) {
+  fp::PagedArgs r{};
+  r.q = a->q;
+  r.o = a->o;
+  r.kc = a->key_cache;
+  r.vc = a->value_cache;
+  r.qst = a->q_stride_tok;
+  r.qhs = a->q_stride_head;
+  r.ost = a->o_stride_tok;
+  r.ohs = a->o_stride_head;
+  r.kcb = a->kc_stride_block;
+  r.kcs = a->kc_stride_slot;
+  r.kch = a->kc_stride_head;
+  r.vcb = a->vc_stride_block;
+  r.vcs = a->vc_stride_slot;
+  r.vch = a->vc_stride_head;
+  r.cu = a->cu_seqlens;
+  r.used = a->seqused;
+  r.table = a->block_table;
+  r.cu64 = a->cu_is64;
+  r.used64 = a->used_is64;
+  r.table64 = a->table_is64;
+  r.table_stride = a->table_stride;
+  r.T = a->num_tokens;
+  r.nblocks = a->num_blocks;
+  r.B = a->batch;
+  r.width = a->table_width;
+  r.bs = a->block_size;
+  r.bs_shift = -1;
+  for (int sh = 0; sh < 31; ++sh)
+    if ((1 << sh) == a->block_size) r.bs_shift = sh;
+  r.Hq = a->num_q_heads;
+  r.Hkv = a->num_kv_heads;
+  r.G = a->num_q_heads / a->num_kv_heads;
+  r.scale_log2 = a->softmax_scale * static_cast<float>(1.4426950408889634);
+  r.nc = sp.nc;
+  r.part = static_cast<float*>(ws);
+  r.ml = sp.nc > 1 ? static_cast<float*>(ws) + a->num_tokens * a->num_q_heads * sp.nc * a->head_dim
+                   : nullptr;
+  return r;
+}
+
+fp::CacheScales scales(const fp_kv_scales& s) {
+  return fp::CacheScales{s.data, s.per_slot ? s.stride_block : 0, s.data ? s.stride_head : 0,
+                         s.data && s.per_slot ? 1 : 0};
+}
+
+int scales_valid(const fp_kv_scales& s, const char* what) {
+  if (s.per_slot && !s.data) return fail(FP_E_INVALID_ARG, "%s: scales per slot are NULL", what);
+  if (reinterpret_cast<uintptr_t>(s.data) % 4)
+    return fail(FP_E_INVALID_ARG, "%s: scales must be 4-byte aligned", what);
+  if (s.stride_head < 0 || (s.per_slot && s.stride_block < 0))
+    return fail(FP_E_INVALID_ARG, "%s: negative scale strides", what);
+  return FP_OK;
+}
+
+bool is_fp8(int32_t format) { return format == FP_CACHE_E4M3 || format == FP_CACHE_E5M2; }
+
+int paged8_valid(const fp_paged_fp8_args* a) {
+  if (!a) return fail(FP_E_INVALID_ARG, "paged arguments are NULL");
+  if (!is_fp8(a->format)) return fail(FP_E_UNSUPPORTED, "paged: cache format %d", a->format);
+  int rc = paged_valid(&a->base);
+  if (rc != FP_OK || a->base.num_tokens == 0) return rc;
+  const int64_t st[6] = {a->base.kc_stride_block, a->base.kc_stride_slot, a->base.kc_stride_head,
+                         a->base.vc_stride_block, a->base.vc_stride_slot, a->base.vc_stride_head};
+  for (int i = 0; i < 6; ++i)
+    if (st[i] % 16)
+      return fail(FP_E_INVALID_ARG, "paged: strides of an 8-bit cache must be multiples of 16");
+  for (const fp_kv_scales* s : {&a->k_scale, &a->v_scale}) {
+    if ((rc = scales_valid(*s, "paged")) != FP_OK) return rc;
+    if (s->per_slot && a->base.block_size % 16 == 0 &&
+        (!aligned16(s->data) || s->stride_block % 4 || s->stride_head % 4))
+      return fail(FP_E_INVALID_ARG, "paged: scales per slot must be 16-byte aligned with strides "
+                  "of multiples of 4 where block_size is a multiple of 16");
+  }
+  return FP_OK;
+}
+
+bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
+
+// The arguments that the 8-bit write and the read-back share. elem: bytes of a
+// cache element.
+int cache8_valid(const fp_kv_cache_args* a, const fp_kv_scales& ks, const fp_kv_scales& vs,
+                 const char* what, int elem) {
+  if (a->dtype != FP_DTYPE_BF16 && a->dtype != FP_DTYPE_F16)
+    return fail(FP_E_UNSUPPORTED, "%s: dtype %d unsupported (bf16 or fp16 only)", what, a->dtype);
+  if (a->num_tokens < 0 || a->num_blocks < 0 || a->block_size < 1 || a->num_kv_heads < 1 ||
+      a->head_dim < 8 || a->head_dim % 8)
+    return fail(FP_E_INVALID_ARG, "%s: sizes out of range (head_dim must be a multiple of 8)", what);
+  if (a->head_dim > 512) return fail(FP_E_UNSUPPORTED, "%s: head_dim %d above 512", what, a->head_dim);
+  if (a->num_tokens == 0) return FP_OK;
+  // a launch holds fewer than 2^32 threads: at most 64 per row, K and V rows of every
+  // head of a token
+  if (a->num_tokens * a->num_kv_heads >= (int64_t(1) << 25) &&
+      a->num_tokens * a->num_kv_heads * 2 * fp::row_lanes(a->head_dim) >= (int64_t(1) << 32) - 256)
+    return fail(FP_E_UNSUPPORTED, "%s: 2^32 or more threads' work in one call", what);
+  if (!a->key || !a->value || !a->key_cache || !a->value_cache)
+    return fail(FP_E_INVALID_ARG, "%s: NULL pointer", what);
+  if (!aligned16(a->key) || !aligned16(a->value))
+    return fail(FP_E_INVALID_ARG, "%s: key / value must be 16-byte aligned", what);
+  if (elem == 1 ? !aligned8(a->key_cache) || !aligned8(a->value_cache)
+                : !aligned16(a->key_cache) || !aligned16(a->value_cache))
+    return fail(FP_E_INVALID_ARG, "%s: the caches must be %d-byte aligned", what, 8 * elem);
+  const int64_t strides[10] = {a->k_stride_tok, a->k_stride_head, a->v_stride_tok, a->v_stride_head,
+                               a->kc_stride_block, a->kc_stride_slot, a->kc_stride_head,
+                               a->vc_stride_block, a->vc_stride_slot, a->vc_stride_head};
+  for (int i = 0; i < 10; ++i)
+    if (strides[i] < 0 || strides[i] % 8)
+      return fail(FP_E_INVALID_ARG, "%s: strides must be non-negative multiples of 8 elements", what);
+  const int rc = scales_valid(ks, what);
+  return rc != FP_OK ? rc : scales_valid(vs, what);
+}
+
+fp::Cache8Args cache8_args(const fp_kv_cache_args* a, const fp_kv_scales& ks,
+                           const fp_kv_scales& vs) {
+  fp::Cache8Args r;
+  r.c = cache_args(a);
+  r.c.elem_bytes = 1;
+  r.c.row_bytes = a->head_dim;
+  r.ks = scales(ks);
+  r.vs = scales(vs);
+  return r;
+}
+
 }  // namespace
 
 extern "C" {
@@ -737,46 +888,33 @@ int fp_paged_attention(const fp_paged_args* a, void* ws, void* stream) {
   const PagedSplit sp = paged_split(a);
   if (sp.bytes > 0 && !ws) return fail(FP_E_INVALID_ARG, "paged: workspace is NULL");
   if (!aligned16(ws)) return fail(FP_E_INVALID_ARG, "paged: workspace must be 16-byte aligned");
-  fp::PagedArgs r;
-  r.q = a->q;
-  r.o = a->o;
-  r.kc = a->key_cache;
-  r.vc = a->value_cache;
-  r.qst = a->q_stride_tok;
-  r.qhs = a->q_stride_head;
-  r.ost = a->o_stride_tok;
-  r.ohs = a->o_stride_head;
-  r.kcb = a->kc_stride_block;
-  r.kcs = a->kc_stride_slot;
-  r.kch = a->kc_stride_head;
-  r.vcb = a->vc_stride_block;
-  r.vcs = a->vc_stride_slot;
-  r.vch = a->vc_stride_head;
-  r.cu = a->cu_seqlens;
-  r.used = a->seqused;
-  r.table = a->block_table;
-  r.cu64 = a->cu_is64;
-  r.used64 = a->used_is64;
-  r.table64 = a->table_is64;
-  r.table_stride = a->table_stride;
-  r.T = a->num_tokens;
-  r.nblocks = a->num_blocks;
-  r.B = a->batch;
-  r.width = a->table_width;
-  r.bs = a->block_size;
-  r.bs_shift = -1;
-  for (int sh = 0; sh < 31; ++sh)
-    if ((1 << sh) == a->block_size) r.bs_shift = sh;
-  r.Hq = a->num_q_heads;
-  r.Hkv = a->num_kv_heads;
-  r.G = a->num_q_heads / a->num_kv_heads;
-  r.scale_log2 = a->softmax_scale * static_cast<float>(1.4426950408889634);
-  r.nc = sp.nc;
-  r.part = static_cast<float*>(ws);
-  r.ml = sp.nc > 1 ? static_cast<float*>(ws) + a->num_tokens * a->num_q_heads * sp.nc * a->head_dim
-                   : nullptr;
+  const fp::PagedArgs r = paged_args(a, sp, ws);
   const auto launch = sp.many ? fp::launch_paged_rows : fp::launch_paged;
   const hipError_t e = launch(r, a->dtype, a->head_dim, sp.tiles, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? FP_OK : hip_fail(e, "paged attention launch");
+}
+
+size_t fp_paged_fp8_workspace_bytes(const fp_paged_fp8_args* a) {
+  return paged8_valid(a) == FP_OK ? paged_split(&a->base).bytes : 0;
+}
+
+int fp_paged_attention_fp8(const fp_paged_fp8_args* a, void* ws, void* stream) {
+  const int rc = paged8_valid(a);
+  if (rc != FP_OK) return rc;
+  if (a->base.num_tokens == 0) return FP_OK;
+  const PagedSplit sp = paged_split(&a->base);
+  if (sp.bytes > 0 && !ws) return fail(FP_E_INVALID_ARG, "paged: workspace is NULL");
+  if (!aligned16(ws)) return fail(FP_E_INVALID_ARG, "paged: workspace must be 16-byte aligned");
+  fp::Paged8Args r;
+  r.a = paged_args(&a->base, sp, ws);
+  r.ks = scales(a->k_scale);
+  r.vs = scales(a->v_scale);
+  if (!r.vs.slot) {
+    r.a.vscale = r.vs.p;
+    r.a.vscale_head = static_cast<int32_t>(r.vs.sh);
+  }
+  const hipError_t e = fp::launch_paged8(r, a->base.dtype, a->format, a->base.head_dim, sp.many,
+                                         sp.tiles, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? FP_OK : hip_fail(e, "paged attention launch");
 }
 
@@ -800,30 +938,51 @@ int fp_kv_cache_write(const fp_kv_cache_args* a, void* stream) {
   for (int i = 0; i < 10; ++i)
     if (strides[i] < 0 || strides[i] % 8)
       return fail(FP_E_INVALID_ARG, "kv-cache strides must be non-negative multiples of 8 elements");
-  fp::KvCacheArgs k;
-  k.key = a->key;
-  k.value = a->value;
-  k.k_stride_tok = a->k_stride_tok;
-  k.k_stride_head = a->k_stride_head;
-  k.v_stride_tok = a->v_stride_tok;
-  k.v_stride_head = a->v_stride_head;
-  k.key_cache = a->key_cache;
-  k.value_cache = a->value_cache;
-  k.kc_stride_block = a->kc_stride_block;
-  k.kc_stride_slot = a->kc_stride_slot;
-  k.kc_stride_head = a->kc_stride_head;
-  k.vc_stride_block = a->vc_stride_block;
-  k.vc_stride_slot = a->vc_stride_slot;
-  k.vc_stride_head = a->vc_stride_head;
-  k.slot_mapping = a->slot_mapping;
-  k.num_tokens = a->num_tokens;
-  k.num_slots = a->num_blocks * a->block_size;
-  k.block_size = a->block_size;
-  k.num_kv_heads = a->num_kv_heads;
-  k.elem_bytes = 2;
-  k.row_bytes = a->head_dim * 2;
+  const fp::KvCacheArgs k = cache_args(a);
   const hipError_t e = fp::launch_kv_cache_write(k, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? FP_OK : hip_fail(e, "kv-cache write launch");
+}
+
+int fp_kv_cache_write_fp8(const fp_kv_cache_fp8_args* a, void* stream) {
+  if (!a) return fail(FP_E_INVALID_ARG, "kv-cache arguments are NULL");
+  if (!is_fp8(a->format)) return fail(FP_E_UNSUPPORTED, "kv-cache: cache format %d", a->format);
+  const int rc = cache8_valid(&a->base, a->k_scale, a->v_scale, "kv-cache", 1);
+  if (rc != FP_OK || a->base.num_tokens == 0) return rc;
+  if (!a->base.slot_mapping) return fail(FP_E_INVALID_ARG, "kv-cache: NULL pointer");
+  const hipError_t e =
+      fp::launch_kv_cache_write8(cache8_args(&a->base, a->k_scale, a->v_scale), a->base.dtype,
+                                 a->format, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? FP_OK : hip_fail(e, "kv-cache write launch");
+}
+
+int fp_kv_cache_gather(const fp_kv_gather_args* a, void* stream) {
+  if (!a) return fail(FP_E_INVALID_ARG, "kv-gather arguments are NULL");
+  if (!is_fp8(a->format) && a->format != FP_CACHE_16BIT)
+    return fail(FP_E_UNSUPPORTED, "kv-gather: cache format %d", a->format);
+  const int rc = cache8_valid(&a->base, a->k_scale, a->v_scale, "kv-gather",
+                              a->format == FP_CACHE_16BIT ? 2 : 1);
+  if (rc != FP_OK || a->base.num_tokens == 0) return rc;
+  if (a->batch < 1 || a->table_width < 0 || a->table_stride < 0)
+    return fail(FP_E_INVALID_ARG, "kv-gather: sizes out of range");
+  if (!a->cu_seqlens || (!a->block_table && a->table_width > 0))
+    return fail(FP_E_INVALID_ARG, "kv-gather: NULL pointer");
+  if (static_cast<int64_t>(a->table_width) * a->base.block_size >= (int64_t(1) << 30))
+    return fail(FP_E_UNSUPPORTED, "kv-gather: 2^30 or more tokens per sequence");
+  fp::GatherArgs r;
+  r.g = cache8_args(&a->base, a->k_scale, a->v_scale);
+  r.cu = a->cu_seqlens;
+  r.table = a->block_table;
+  r.starts = a->starts;
+  r.cu64 = a->cu_is64;
+  r.table64 = a->table_is64;
+  r.starts64 = a->starts_is64;
+  r.table_stride = a->table_stride;
+  r.num_blocks = a->base.num_blocks;
+  r.B = a->batch;
+  r.width = a->table_width;
+  const hipError_t e =
+      fp::launch_kv_cache_gather(r, a->base.dtype, a->format, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? FP_OK : hip_fail(e, "kv-gather launch");
 }
 
 int fp_read_status(const fp_problem* p, void* ws, void* stream, uint32_t* status) {

@@ -159,6 +159,52 @@ struct PagedArgs {
   int32_t nc;        // chunk slots per row
   float* part;       // [T * Hq][nc][d] unnormalised outputs
   float* ml;         // [T * Hq][nc] (m, l) pairs
+  // V scale of KV head h at [h * vscale_head], by which the merge multiplies a
+  // row's sum (8-bit caches with fixed scales), or null
+  const float* vscale;
+  int32_t vscale_head;
+};
+
+// Scales of an 8-bit cache: one for all (sh 0) or per KV head (sh 1), or one per
+// slot at p[block * sb + head * sh + slot]; null: 1.
+struct CacheScales {
+  float* p;
+  int64_t sb, sh;
+  int32_t slot;
+};
+
+// Attention over a paged 8-bit cache (fp_paged8.hip)
+struct Paged8Args {
+  PagedArgs a;
+  CacheScales ks, vs;
+};
+
+// Write of an 8-bit cache and the read-back of any (fp_kvcache.hip): `key` and
+// `value` are the 16-bit rows, read by the write, written by the read-back.
+struct Cache8Args {
+  KvCacheArgs c;
+  CacheScales ks, vs;
+};
+
+// Lanes of one row of head_dim elements, 8 of them each: a power of two, at most 64
+// (head dims up to 512)
+inline int row_lanes(int head_dim) {
+  int n = 1;
+  while (n < head_dim / 8) n *= 2;
+  return n;
+}
+
+constexpr int kGatherTokens = 16;  // tokens per workgroup of the read-back
+
+struct GatherArgs {
+  Cache8Args g;  // c.num_tokens: rows of key / value
+  const void* cu;
+  const void* table;
+  const void* starts;  // nullable
+  int32_t cu64, table64, starts64;
+  int64_t table_stride;
+  int64_t num_blocks;
+  int32_t B, width;
 };
 
 constexpr int kRopeMaxBatch = 64;  // sequences whose offsets k_rope takes
@@ -195,6 +241,13 @@ hipError_t launch_rope(const RopeArgs& a, int dtype, hipStream_t s);
 hipError_t launch_paged_rows(const PagedArgs& a, int dtype, int head_dim, int64_t tiles,
                              hipStream_t s);
 hipError_t launch_paged(const PagedArgs& a, int dtype, int head_dim, int64_t tiles, hipStream_t s);
+// combines the partials of either kernel's 8-bit form (rows: k_paged8_rows)
+hipError_t launch_paged_merge(const PagedArgs& a, int dtype, int head_dim, bool rows,
+                              hipStream_t s);
+hipError_t launch_paged8(const Paged8Args& a, int dtype, int format, int head_dim, bool rows,
+                         int64_t tiles, hipStream_t s);
+hipError_t launch_kv_cache_write8(const Cache8Args& a, int dtype, int format, hipStream_t s);
+hipError_t launch_kv_cache_gather(const GatherArgs& a, int dtype, int format, hipStream_t s);
 hipError_t launch_kv_cache_write(const KvCacheArgs& a, hipStream_t s);
 hipError_t launch_pool(const PoolArgs& a, int dtype, int head_dim, int64_t grid, hipStream_t s);
 // k_plan then k_pool as one launch (batch <= kSmallPlanBatch)

@@ -38,149 +38,9 @@
 // a 1 GiB copy reaches 5.24; k_paged_merge 6 us); one sequence of 65,000 tokens
 // 6.57 -> 0.056 ms a call among others of its kind, 0.066 with inputs that change
 // (127 chunks x 8 KV heads; k_paged 49 us = 5.4 TB/s, k_paged_merge 7).
-#include "fp_attn_common.h"
+#include "fp_paged_common.h"
 
 namespace fp {
-
-__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
-// entry x of a 32- or 64-bit integer array
-__device__ __forceinline__ int64_t ld_int(const void* p, int is64, int64_t x) {
-  return is64 ? static_cast<const int64_t*>(p)[x] : static_cast<const int32_t*>(p)[x];
-}
-
-// One sequence as the workgroups see it. `bad`: more tokens than the block
-// table has room for; its rows are written as NaN. `off`: its query offsets
-// descend or lie outside the call's rows.
-struct PagedSeq {
-  int64_t q0;  // first query row
-  int nq;      // query rows
-  int64_t nk;  // cached tokens
-  bool bad, off;
-};
-
-__device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b) {
-  PagedSeq s;
-  s.q0 = ld_int(a.cu, a.cu64, b);
-  const int64_t q1 = ld_int(a.cu, a.cu64, b + 1);
-  s.off = s.q0 < 0 || q1 > a.T || q1 < s.q0;
-  s.nq = s.off ? 0 : static_cast<int>(q1 - s.q0);
-  s.nk = ld_int(a.used, a.used64, b);
-  s.bad = s.nk > static_cast<int64_t>(a.width) * a.bs;
-  if (s.bad || s.nk < 0) s.nk = 0;
-  return s;
-}
-
-__device__ __forceinline__ int64_t shfl64(int64_t x, int lane) {
-  return static_cast<int64_t>(
-      (static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(x >> 32), lane))) << 32) |
-      static_cast<uint32_t>(__shfl(static_cast<int>(x), lane)));
-}
-
-// The sequence that owns row tile `x` (tiles of `rt` rows of nq * G, numbered
-// over the sequences) and the tile's index in it, or with tok >= 0 the one
-// that owns query row `tok`; and the chunk length all workgroups use. By one
-// wave (64 sequences at a time); b < 0 when there is none. Where some sequence's
-// offsets do not fit, which rows are whose is unknown: all rows of the call are
-// one sequence's then, and bad.
-struct PagedTile {
-  PagedSeq s;
-  int b, tl, chunk;
-};
-__device__ __forceinline__ PagedTile paged_find(const PagedArgs& a, int rt, int64_t x,
-                                                int64_t tok) {
-  const int lane = threadIdx.x & 63;
-  PagedTile r;
-  r.b = -1;
-  r.tl = 0;
-  r.s = PagedSeq{0, 0, 0, false, false};
-  int64_t carry = 0;
-  int maxlen = 0;
-  bool off = false;
-  for (int base = 0; base < a.B; base += 64) {
-    PagedSeq s{0, 0, 0, false, false};
-    if (base + lane < a.B) s = paged_seq(a, base + lane);
-    off = off || __ballot(s.off) != 0;
-    const int tiles =
-        static_cast<int>((static_cast<int64_t>(s.nq) * a.G + rt - 1) / rt);
-    if (s.nq > 0) maxlen = max(maxlen, static_cast<int>(s.nk));
-    int incl = tiles;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(incl, o);
-      if (lane >= o) incl += y;
-    }
-    const bool mine = tok >= 0 ? tok >= s.q0 && tok < s.q0 + s.nq
-                               : tiles > 0 && x >= carry + incl - tiles && x < carry + incl;
-    const uint64_t hit = __ballot(mine);
-    if (r.b < 0 && hit) {
-      const int l = __ffsll(static_cast<long long>(hit)) - 1;
-      r.b = base + l;
-      r.tl = static_cast<int>(x - carry) - __shfl(incl - tiles, l);
-      r.s.q0 = shfl64(s.q0, l);
-      r.s.nq = __shfl(s.nq, l);
-      r.s.nk = shfl64(s.nk, l);
-      r.s.bad = __shfl(static_cast<int>(s.bad), l) != 0;
-    }
-    carry += __shfl(incl, 63);
-  }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) maxlen = max(maxlen, __shfl_xor(maxlen, o));
-  const int per = (maxlen + a.nc - 1) / a.nc;
-  r.chunk = (max(per, kPagedMinChunk) + 127) / 128 * 128;
-  if (off) {
-    r.b = tok >= 0 || x < (a.T * a.G + rt - 1) / rt ? 0 : -1;
-    r.tl = static_cast<int>(x);
-    r.s = PagedSeq{0, static_cast<int>(a.T), 0, true, true};
-  }
-  // wave-uniform values in scalar registers
-  r.b = __builtin_amdgcn_readfirstlane(r.b);
-  r.tl = __builtin_amdgcn_readfirstlane(r.tl);
-  r.chunk = __builtin_amdgcn_readfirstlane(r.chunk);
-  r.s.nq = __builtin_amdgcn_readfirstlane(r.s.nq);
-  r.s.nk = __builtin_amdgcn_readfirstlane(static_cast<int>(r.s.nk));
-  r.s.q0 = __builtin_amdgcn_readfirstlane(static_cast<int>(r.s.q0));
-  return r;
-}
-
-// Page of cached token `key` of a sequence whose table row is `row`. A page
-// number below 0 counts from the end (as the index of a torch gather); one
-// outside the cache sets `bad` and reads page 0.
-// UNI: `key` is wave-uniform and the lookup goes through the scalar cache (a
-// vector load would wait for every K / V load issued before it).
-template <bool UNI>
-__device__ __forceinline__ int64_t paged_page(const PagedArgs& a, int64_t row, int key, bool& bad) {
-  int idx = a.bs_shift >= 0 ? key >> a.bs_shift : key / a.bs;
-  int64_t p;
-  if constexpr (UNI) {
-    idx = __builtin_amdgcn_readfirstlane(idx);
-    p = a.table64 ? sld(static_cast<const int64_t*>(a.table) + row + idx)
-                  : static_cast<int64_t>(sld(static_cast<const int32_t*>(a.table) + row + idx));
-  } else {
-    p = ld_int(a.table, a.table64, row + idx);
-  }
-  if (p < 0) p += a.nblocks;
-  if (p < 0 || p >= a.nblocks) {
-    bad = true;
-    p = 0;
-  }
-  return p;
-}
-
-// max / sum over the lanes l, l ^ 16, l ^ 32, l ^ 48 (one query row), in every lane
-__device__ __forceinline__ float row4_max(float x) {
-  x = fmaxf(x, __uint_as_float(xchg_xor<16>(__float_as_uint(x))));
-  return pair32_max(x);
-}
-__device__ __forceinline__ float row4_sum(float x) {
-  x += __uint_as_float(xchg_xor<16>(__float_as_uint(x)));
-  return pair32_sum(x);
-}
 
 // P16: the page size is a multiple of 16, so a 16-key tile lies in one page
 // (one scalar page lookup and wave-uniform bases); otherwise every lane looks
@@ -550,7 +410,8 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a) {
   for (int q = 0; q < XD; ++q) so[w][XD * lane + q] = acc[q];
   __syncthreads();
   if (t < D) {
-    const float o = (so[0][t] + so[1][t] + so[2][t] + so[3][t]) / L;
+    float o = (so[0][t] + so[1][t] + so[2][t] + so[3][t]) / L;
+    if (a.vscale != nullptr) o *= a.vscale[(hq / a.G) * a.vscale_head];
     static_cast<uint16_t*>(a.o)[tok * a.ost + static_cast<int64_t>(hq) * a.ohs + t] = T::from_f32(o);
   }
 }
@@ -590,18 +451,6 @@ __device__ __forceinline__ void part_pair(float x0, float x1, uint32_t (&u)[3]) 
     x0 -= T::to_f32(static_cast<uint16_t>(u[p]));
     x1 -= T::to_f32(static_cast<uint16_t>(u[p] >> 16));
   }
-}
-
-// V^T operand of a 16-key step: keys r .. r + 3 and r + 8 .. r + 11, dim xx of a
-// key-major tile
-template <typename T, int D>
-__device__ __forceinline__ typename T::vec8 read_vt(const uint16_t* sv16, int r, int xx) {
-  const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (__attribute__((address_space(3))) i16x4*)(sv16 + tile_elem<D>(r, xx)));
-  const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (__attribute__((address_space(3))) i16x4*)(sv16 + tile_elem<D>(r + 8, xx)));
-  const uint2 lo2 = __builtin_bit_cast(uint2, lo), hi2 = __builtin_bit_cast(uint2, hi);
-  return as_vec8<T>(make_uint4(lo2.x, lo2.y, hi2.x, hi2.y));
 }
 
 // One workgroup (4 waves) per (128-row tile of the G query heads of a KV head,
@@ -984,11 +833,32 @@ __global__ __launch_bounds__(256) void k_paged_merge_rows(PagedArgs a) {
     uint16_t* op = static_cast<uint16_t*>(a.o) + tok * a.ost +
                    static_cast<int64_t>(h0 + u) * a.ohs + XD * lane;
     const float rcp = 1.0f / L[u];
-    if constexpr (XD == 2)
-      *reinterpret_cast<uint32_t*>(op) = pack2<T>(acc[u][0] * rcp, acc[u][1] * rcp);
-    else
-      op[0] = T::from_f32(acc[u][0] * rcp);
+    float y[XD];
+#pragma unroll
+    for (int q = 0; q < XD; ++q) y[q] = acc[u][q] * rcp;
+    if (a.vscale != nullptr) {
+      const float vs = a.vscale[((h0 + u) / a.G) * a.vscale_head];
+#pragma unroll
+      for (int q = 0; q < XD; ++q) y[q] *= vs;
+    }
+    if constexpr (XD == 2) *reinterpret_cast<uint32_t*>(op) = pack2<T>(y[0], y[1]);
+    else op[0] = T::from_f32(y[0]);
   }
+}
+
+template <typename T, int D>
+hipError_t launch_merge_rows_t(const PagedArgs& a, hipStream_t s) {
+  const int64_t waves = a.T * ((a.Hq + kMergeHeads - 1) / kMergeHeads);
+  hipLaunchKernelGGL((k_paged_merge_rows<T, D>), dim3(static_cast<unsigned>((waves + 3) / 4)),
+                     dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+template <typename T, int D>
+hipError_t launch_merge_t(const PagedArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((k_paged_merge<T, D>), dim3(static_cast<unsigned>(a.T * a.Hq)), dim3(256), 0,
+                     s, a);
+  return hipGetLastError();
 }
 
 template <typename T, int D>
@@ -996,12 +866,7 @@ hipError_t launch_paged_rows_t(const PagedArgs& a, int64_t tiles, hipStream_t s)
   const dim3 grid(static_cast<unsigned>(tiles * a.Hkv), static_cast<unsigned>(a.nc));
   if (a.bs % 16 == 0) hipLaunchKernelGGL((k_paged_rows<T, D, true>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((k_paged_rows<T, D, false>), grid, dim3(256), 0, s, a);
-  if (a.nc > 1) {
-    const int64_t waves = a.T * ((a.Hq + kMergeHeads - 1) / kMergeHeads);
-    hipLaunchKernelGGL((k_paged_merge_rows<T, D>), dim3(static_cast<unsigned>((waves + 3) / 4)),
-                       dim3(256), 0, s, a);
-  }
-  return hipGetLastError();
+  return a.nc > 1 ? launch_merge_rows_t<T, D>(a, s) : hipGetLastError();
 }
 
 template <typename T, int D>
@@ -1009,10 +874,7 @@ hipError_t launch_paged_t(const PagedArgs& a, int64_t tiles, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(tiles * a.Hkv), static_cast<unsigned>(a.nc));
   if (a.bs % 16 == 0) hipLaunchKernelGGL((k_paged<T, D, true>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((k_paged<T, D, false>), grid, dim3(256), 0, s, a);
-  if (a.nc > 1)
-    hipLaunchKernelGGL((k_paged_merge<T, D>), dim3(static_cast<unsigned>(a.T * a.Hq)), dim3(256), 0,
-                       s, a);
-  return hipGetLastError();
+  return a.nc > 1 ? launch_merge_t<T, D>(a, s) : hipGetLastError();
 }
 
 hipError_t launch_paged_rows(const PagedArgs& a, int dtype, int head_dim, int64_t tiles,
@@ -1029,6 +891,20 @@ hipError_t launch_paged(const PagedArgs& a, int dtype, int head_dim, int64_t til
     constexpr int D = decltype(dc)::value;
     return dtype == FP_DTYPE_BF16 ? launch_paged_t<BF16, D>(a, tiles, s)
                                   : launch_paged_t<F16, D>(a, tiles, s);
+  });
+}
+
+hipError_t launch_paged_merge(const PagedArgs& a, int dtype, int head_dim, bool rows,
+                              hipStream_t s) {
+  if (rows && head_dim == 128)
+    return dtype == FP_DTYPE_BF16 ? launch_merge_rows_t<BF16, 128>(a, s)
+                                  : launch_merge_rows_t<F16, 128>(a, s);
+  if (rows)
+    return dtype == FP_DTYPE_BF16 ? launch_merge_rows_t<BF16, 64>(a, s)
+                                  : launch_merge_rows_t<F16, 64>(a, s);
+  return with_head_dim(head_dim, [&](auto dc) {
+    constexpr int D = decltype(dc)::value;
+    return dtype == FP_DTYPE_BF16 ? launch_merge_t<BF16, D>(a, s) : launch_merge_t<F16, D>(a, s);
   });
 }
 

@@ -21,7 +21,11 @@ The v1 forward mirrors what the 0.12 patch does to
   the cache (:201-225, vLLM's ``flash_attn_varlen_func``);
 * a profiling run (``attn_metadata is None``) zero-fills the output (:95-97),
   encoder attention and cascade attention are delegated unchanged (:104-114,
-  :226-252), fused output quantisation is rejected (:90-93).
+  :226-252), fused output quantisation is rejected (:90-93);
+* an fp8 ``kv_cache_dtype`` (:151-166) keeps the cache in 8-bit floats with the
+  layer's ``_k_scale`` / ``_v_scale``: written by the HIP kernel behind
+  ``fp_kv_cache_write_fp8``, attended by ``fp_paged_attention_fp8``. The query
+  stays in 16 bits.
 
 vLLM is not a dependency: the forward only touches the attributes of the
 impl object and the metadata that the reference's forward reads, and the two
@@ -60,50 +64,214 @@ DEFAULT_CONFIG = "flashprefill_qwen2"  # the reference patch's choice (:43)
 _DTYPES = {torch.bfloat16: _lib.FP_DTYPE_BF16, torch.float16: _lib.FP_DTYPE_F16}
 
 
-def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
-                      value_cache: torch.Tensor, slot_mapping: torch.Tensor) -> None:
-    """Write key / value (tokens, Hkv, d) into the paged caches
-    (num_blocks, block_size, Hkv, d) at ``slot_mapping`` (int64, one slot per
-    token; the mapping's length is the number of tokens written, negative
-    slots are padding and skipped), on the current stream."""
-    if key.dtype not in _DTYPES or value.dtype != key.dtype or key_cache.dtype != key.dtype or \
-            value_cache.dtype != key.dtype:
+# 8-bit cache types and their names in vLLM's kv_cache_dtype
+_FORMATS = {torch.float8_e4m3fn: _lib.FP_CACHE_E4M3, torch.float8_e5m2: _lib.FP_CACHE_E5M2}
+_FP8_NAMES = {"fp8": torch.float8_e4m3fn, "fp8_e4m3": torch.float8_e4m3fn,
+              "fp8_e5m2": torch.float8_e5m2}
+
+
+def _check_scales(cache: torch.Tensor, k_scale, v_scale) -> None:
+    """Refuse scales that are not of one of the forms that ``reshape_and_cache``
+    describes, or that come with a 16-bit cache."""
+    nb, bs, hkv = cache.shape[:3]
+    for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if s is None:
+            continue
+        if cache.dtype not in _FORMATS:
+            raise ValueError(f"{name}: scales belong to 8-bit caches, this one is {cache.dtype}")
+        if s.dtype != torch.float32:
+            raise ValueError(f"{name} must be float32, got {s.dtype}")
+        if s.dim() == 3:
+            if s.shape != (nb, hkv, bs) or s.device != cache.device or \
+                    (bs > 1 and s.stride(2) != 1):
+                raise ValueError(f"{name}: one scale per slot is (num_blocks, num_kv_heads, "
+                                 f"block_size) = {(nb, hkv, bs)} on the cache's device, slots "
+                                 f"contiguous; got {tuple(s.shape)} on {s.device}")
+        elif s.dim() > 1 or s.numel() not in (1, hkv):
+            raise ValueError(f"{name} must hold 1 or {hkv} values, or one per slot "
+                             f"{(nb, hkv, bs)}; got {tuple(s.shape)}")
+
+
+def _scale_args(scale: Optional[torch.Tensor], device) -> tuple:
+    """``fp_kv_scales`` of a checked scale, and the tensor whose memory it names."""
+    out = _lib.FpKvScales()
+    if scale is None:
+        return out, None
+    if scale.dim() == 3:
+        out.data, out.per_slot = scale.data_ptr(), 1
+        out.stride_block, out.stride_head = scale.stride(0), scale.stride(1)
+        return out, scale
+    scale = scale.to(device).view(-1).contiguous()
+    out.data, out.stride_head = scale.data_ptr(), int(scale.numel() > 1)
+    return out, scale
+
+
+def _check_rows(key, value, key_cache, value_cache, what: str) -> None:
+    """Types, layout and sizes that the cache's write and read-back share."""
+    if key.dtype not in _DTYPES or value.dtype != key.dtype or \
+            value_cache.dtype != key_cache.dtype or \
+            (key_cache.dtype != key.dtype and key_cache.dtype not in _FORMATS):
         raise NotImplementedError(
-            f"kv-cache write supports bf16 / fp16 caches of the key dtype, got key {key.dtype}, "
-            f"cache {key_cache.dtype} (fp8 caches are not built)")
+            f"{what} supports bf16 / fp16 rows and caches of their dtype, float8_e4m3fn or "
+            f"float8_e5m2, got key {key.dtype}, value {value.dtype}, caches {key_cache.dtype}, "
+            f"{value_cache.dtype}")
     for name, t in (("key", key), ("value", value), ("key_cache", key_cache),
                     ("value_cache", value_cache)):
         if t.stride(-1) != 1:
             raise ValueError(f"{name} must have a contiguous head dimension")
     if key_cache.dim() != 4 or value_cache.shape != key_cache.shape:
         raise ValueError("caches must be (num_blocks, block_size, num_kv_heads, head_dim)")
-    nb, bs, hkv, d = key_cache.shape
-    n = slot_mapping.numel()
-    if key.shape[1:] != (hkv, d) or value.shape[1:] != (hkv, d) or key.shape[0] < n or \
-            value.shape[0] < n:
+    if key.dim() != 3 or value.dim() != 3 or key.shape[1:] != key_cache.shape[2:] or \
+            value.shape[1:] != key_cache.shape[2:]:
         raise ValueError(f"key {tuple(key.shape)} / value {tuple(value.shape)} do not match the "
-                         f"cache {tuple(key_cache.shape)} and {n} slots")
-    slots = slot_mapping.to(dtype=torch.int64).contiguous()
-    a = _lib.FpKvCacheArgs()
+                         f"cache {tuple(key_cache.shape)}")
+
+
+def _check_written(*tensors) -> None:
+    """Refuse what torch's own in-place operations refuse: several elements in one
+    place, and inference tensors outside inference mode."""
+    for t in tensors:
+        if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+            raise RuntimeError("a tensor to be written has several elements in one memory "
+                               "location: clone() it first")
+        if t.is_inference() and not torch.is_inference_mode_enabled():
+            raise RuntimeError("an inference tensor cannot be written outside inference mode")
+
+
+def _cache_args(a, key, value, key_cache, value_cache, n: int) -> None:
+    nb, bs, hkv, d = key_cache.shape
     a.key, a.value = key.data_ptr(), value.data_ptr()
     a.k_stride_tok, a.k_stride_head = key.stride(0), key.stride(1)
     a.v_stride_tok, a.v_stride_head = value.stride(0), value.stride(1)
     a.key_cache, a.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
     a.kc_stride_block, a.kc_stride_slot, a.kc_stride_head = key_cache.stride()[:3]
     a.vc_stride_block, a.vc_stride_slot, a.vc_stride_head = value_cache.stride()[:3]
-    a.slot_mapping = slots.data_ptr()
     a.num_tokens, a.num_blocks = n, nb
     a.block_size, a.num_kv_heads, a.head_dim = bs, hkv, d
     a.dtype = _DTYPES[key.dtype]
+
+
+def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
+                      value_cache: torch.Tensor, slot_mapping: torch.Tensor,
+                      k_scale: Optional[torch.Tensor] = None,
+                      v_scale: Optional[torch.Tensor] = None) -> None:
+    """Write key / value (tokens, Hkv, d) into the paged caches
+    (num_blocks, block_size, Hkv, d) at ``slot_mapping`` (int64, one slot per
+    token; the mapping's length is the number of tokens written, negative
+    slots are padding and skipped), on the current stream.
+
+    Caches of key's dtype hold the rows as they are. Caches of float8_e4m3fn or
+    float8_e5m2 hold ``x / scale`` rounded to nearest even, what lies beyond the
+    format's largest finite value (infinities too) as that value, NaN as NaN.
+    The fp32 scales are
+
+    * fixed, and read: one value, or one per KV head (None: 1);
+    * one per slot and KV head, ``(num_blocks, Hkv, block_size)``: found from each
+      row, its largest finite magnitude over the format's largest finite value (1
+      for a row of zeros), and written beside it.
+
+    Slots named by two tokens hold either row, or parts of both."""
+    _check_rows(key, value, key_cache, value_cache, "kv-cache write")
+    _check_scales(key_cache, k_scale, v_scale)
+    n = slot_mapping.numel()
+    if key.shape[0] < n or value.shape[0] < n:
+        raise ValueError(f"key {tuple(key.shape)} / value {tuple(value.shape)} do not match the "
+                         f"cache {tuple(key_cache.shape)} and {n} slots")
+    dev = key.device
+    for t in (key, value, key_cache, value_cache):
+        if not t.is_cuda or t.device != dev:
+            raise ValueError("key, value and the caches must be on one GPU")
+    slots = slot_mapping.to(device=dev, dtype=torch.int64).contiguous()
     lib = _lib.load()
-    _lib.check(lib.fp_kv_cache_write(ctypes.byref(a),
-                                     torch.cuda.current_stream(key.device).cuda_stream))
+    if key_cache.dtype not in _FORMATS:
+        a = _lib.FpKvCacheArgs()
+        _cache_args(a, key, value, key_cache, value_cache, n)
+        a.slot_mapping = slots.data_ptr()
+        with torch.cuda.device(dev):
+            _lib.check(lib.fp_kv_cache_write(ctypes.byref(a),
+                                             torch.cuda.current_stream(dev).cuda_stream))
+        return
+    written = [key_cache, value_cache]
+    written += [s for s in (k_scale, v_scale) if s is not None and s.dim() == 3]
+    _check_written(*written)
+    a = _lib.FpKvCacheFp8Args()
+    _cache_args(a.base, key, value, key_cache, value_cache, n)
+    a.base.slot_mapping = slots.data_ptr()
+    a.format = _FORMATS[key_cache.dtype]
+    a.k_scale, k_keep = _scale_args(k_scale, dev)
+    a.v_scale, v_keep = _scale_args(v_scale, dev)
+    with torch.cuda.device(dev):
+        _lib.check(lib.fp_kv_cache_write_fp8(ctypes.byref(a),
+                                             torch.cuda.current_stream(dev).cuda_stream))
+    torch.autograd.graph.increment_version(written)
+
+
+def gather_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.Tensor,
+                 value: torch.Tensor, cu_seqlens: torch.Tensor, block_table: torch.Tensor,
+                 starts: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
+                 v_scale: Optional[torch.Tensor] = None) -> None:
+    """Read the paged caches back, the inverse of ``reshape_and_cache``: row
+    ``cu_seqlens[b] + i`` of key / value (tokens, Hkv, d; written) becomes cached
+    token ``starts[b] + i`` (``starts`` None: token i) of sequence b, whose pages
+    are ``block_table[b]``, for every row up to ``cu_seqlens[b + 1] - 1``; rows of
+    no sequence are left as they are. 8-bit caches give ``c * scale`` (scales as
+    ``reshape_and_cache`` takes them) in fp32, rounded once to key's dtype;
+    16-bit ones are copied.
+
+    No host synchronisation: what only the device sees is checked there. Offsets
+    that descend or leave the rows make every row NaN, tokens before the first or
+    past the room of the table, and pages outside the cache (a number below 0
+    counts from the end, as in an index), their own rows."""
+    _check_rows(key, value, key_cache, value_cache, "kv-cache read-back")
+    _check_scales(key_cache, k_scale, v_scale)
+    if value.shape != key.shape:
+        raise ValueError(f"key {tuple(key.shape)} and value {tuple(value.shape)} differ")
+    if cu_seqlens.dim() != 1 or block_table.dim() != 2 or \
+            (starts is not None and starts.dim() != 1):
+        raise ValueError("cu_seqlens and starts must have one dimension, block_table two")
+    B, dev = cu_seqlens.numel() - 1, key.device
+    if B < 0 or block_table.shape[0] < B or (starts is not None and starts.numel() < B):
+        raise ValueError(f"block_table {tuple(block_table.shape)} or starts do not match "
+                         f"{B} sequences")
+    for name, t in (("cu_seqlens", cu_seqlens), ("block_table", block_table), ("starts", starts)):
+        if t is not None and t.dtype not in _INDEX:
+            raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
+    if not cu_seqlens.is_cuda:  # known without a synchronisation
+        at = cu_seqlens.tolist()
+        if at[0] < 0 or at[-1] > key.shape[0] or any(x > y for x, y in zip(at, at[1:])):
+            raise ValueError(f"cu_seqlens {at} do not ascend within {key.shape[0]} rows")
+    for t in (key, value, key_cache, value_cache):
+        if not t.is_cuda or t.device != dev:
+            raise ValueError("key, value and the caches must be on one GPU")
+    _check_written(key, value)
+    if B == 0:
+        return
+    cu, table = cu_seqlens.to(dev).contiguous(), block_table.to(dev)
+    if table.stride(1) != 1:
+        table = table.contiguous()
+    a = _lib.FpKvGatherArgs()
+    _cache_args(a.base, key, value, key_cache, value_cache, key.shape[0])
+    a.format = _FORMATS.get(key_cache.dtype, _lib.FP_CACHE_16BIT)
+    a.k_scale, k_keep = _scale_args(k_scale, dev)
+    a.v_scale, v_keep = _scale_args(v_scale, dev)
+    a.batch, a.table_width, a.table_stride = B, table.shape[1], table.stride(0)
+    a.cu_seqlens, a.block_table = cu.data_ptr(), table.data_ptr()
+    a.cu_is64, a.table_is64 = cu.dtype == torch.int64, table.dtype == torch.int64
+    if starts is not None:
+        starts = starts.to(dev).contiguous()
+        a.starts, a.starts_is64 = starts.data_ptr(), starts.dtype == torch.int64
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().fp_kv_cache_gather(ctypes.byref(a),
+                                                  torch.cuda.current_stream(dev).cuda_stream))
+    torch.autograd.graph.increment_version([key, value])
 
 
 def paged_decode_attention(query: torch.Tensor, key_cache: torch.Tensor,
                            value_cache: torch.Tensor, out: torch.Tensor,
                            cu_seqlens_q: torch.Tensor, seqused_k: torch.Tensor,
-                           block_table: torch.Tensor, softmax_scale: float) -> None:
+                           block_table: torch.Tensor, softmax_scale: float,
+                           k_scale: Optional[torch.Tensor] = None,
+                           v_scale: Optional[torch.Tensor] = None) -> None:
     """Attention over the paged cache (the role of vLLM's
     ``flash_attn_varlen_func`` with a block table in the reference's decode
     branch): every query row of sequence b attends causally to the first
@@ -118,28 +286,37 @@ def paged_decode_attention(query: torch.Tensor, key_cache: torch.Tensor,
     cache, get NaN; offsets that descend or leave the query rows make every
     row NaN). Every other call (CPU, fp32, other head dims or layouts, offsets
     or lengths on the host that do not fit, inputs that require gradients)
-    takes the torch composition."""
+    takes the torch composition.
+
+    Caches of float8_e4m3fn or float8_e5m2 stand for their values times
+    ``k_scale`` / ``v_scale``, which are as ``reshape_and_cache`` takes them; query
+    and out stay in 16 bits, and no cached value is rounded on the way
+    (``fp_paged_attention_fp8``)."""
+    _check_scales(key_cache, k_scale, v_scale)
     if _paged_kernel_takes(query, key_cache, value_cache, out, cu_seqlens_q, seqused_k,
-                           block_table):
+                           block_table, k_scale, v_scale):
         _paged_attention_kernel(query, key_cache, value_cache, out, cu_seqlens_q, seqused_k,
-                                block_table, softmax_scale)
+                                block_table, softmax_scale, k_scale, v_scale)
     else:
         paged_attention_reference(query, key_cache, value_cache, out, cu_seqlens_q, seqused_k,
-                                  block_table, softmax_scale)
+                                  block_table, softmax_scale, k_scale, v_scale)
 
 
 _INDEX = (torch.int32, torch.int64)
 
 
 def _rows_ok(t: torch.Tensor) -> bool:
+    step = 16 // t.element_size()
     return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and all(s % 8 == 0 and s >= 0 for s in t.stride()[:-1]))
+            and all(s % step == 0 and s >= 0 for s in t.stride()[:-1]))
 
 
-def _paged_kernel_takes(query, key_cache, value_cache, out, cu, used, table) -> bool:
+def _paged_kernel_takes(query, key_cache, value_cache, out, cu, used, table, k_scale=None,
+                        v_scale=None) -> bool:
     """Whether the HIP kernels take this call as it is: 16-bit tensors of one
-    type on one GPU, head_dim 64 / 128 / 256, 16-byte aligned rows, int32 /
-    int64 metadata of matching shapes, no derivative, functional transform,
+    type on one GPU (or caches of one 8-bit type with scales that the kernels can
+    read in 16-byte pieces), head_dim 64 / 128 / 256, 16-byte aligned rows, int32
+    / int64 metadata of matching shapes, no derivative, functional transform,
     trace or dispatch mode to carry along (they see only torch operations)."""
     if not query.is_cuda or query.dtype not in _DTYPES:
         return False
@@ -155,8 +332,16 @@ def _paged_kernel_takes(query, key_cache, value_cache, out, cu, used, table) -> 
     if d not in (64, 128, 256) or dq != d or nb < 1 or bs < 1 or hkv < 1 or hq < 1 or hq % hkv or \
             out.shape[0] < T or out.shape[1:] != query.shape[1:]:
         return False
-    for t in (query, key_cache, value_cache, out):
-        if t.dtype != dt or t.device != dev or not _rows_ok(t):
+    cdt = key_cache.dtype
+    if cdt != dt and cdt not in _FORMATS:
+        return False
+    for t, want in ((query, dt), (key_cache, cdt), (value_cache, cdt), (out, dt)):
+        if t.dtype != want or t.device != dev or not _rows_ok(t):
+            return False
+    for s in (k_scale, v_scale):
+        if s is not None and s.dim() == 3 and (
+                min(s.stride()[:2]) < 0 or
+                bs % 16 == 0 and (s.data_ptr() % 16 or s.stride(0) % 4 or s.stride(1) % 4)):
             return False
     # torch refuses to write these, and so does the composition
     if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())) or \
@@ -179,10 +364,12 @@ def _paged_kernel_takes(query, key_cache, value_cache, out, cu, used, table) -> 
     if not used.is_cuda and any(n > table.shape[1] * bs for n in used[:B].tolist()):
         return False
     return not (torch.is_grad_enabled() and any(t.requires_grad for t in
-                                                (query, key_cache, value_cache, out)))
+                                                (query, key_cache, value_cache, out, k_scale,
+                                                 v_scale) if t is not None))
 
 
-def _paged_attention_kernel(query, key_cache, value_cache, out, cu, used, table, scale) -> None:
+def _paged_attention_kernel(query, key_cache, value_cache, out, cu, used, table, scale,
+                            k_scale=None, v_scale=None) -> None:
     dev = query.device
     nb, bs, hkv, d = key_cache.shape
     T, hq = query.shape[:2]
@@ -190,7 +377,18 @@ def _paged_attention_kernel(query, key_cache, value_cache, out, cu, used, table,
     table = table.to(dev)
     if table.stride(1) != 1:
         table = table.contiguous()
-    a = _lib.FpPagedArgs()
+    lib = _lib.load()
+    fp8 = key_cache.dtype in _FORMATS
+    if fp8:
+        call = _lib.FpPagedFp8Args()
+        a = call.base
+        call.format = _FORMATS[key_cache.dtype]
+        call.k_scale, k_keep = _scale_args(k_scale, dev)
+        call.v_scale, v_keep = _scale_args(v_scale, dev)
+        ws_bytes, launch = lib.fp_paged_fp8_workspace_bytes, lib.fp_paged_attention_fp8
+    else:
+        call = a = _lib.FpPagedArgs()
+        ws_bytes, launch = lib.fp_paged_workspace_bytes, lib.fp_paged_attention
     a.q, a.q_stride_tok, a.q_stride_head = query.data_ptr(), query.stride(0), query.stride(1)
     a.o, a.o_stride_tok, a.o_stride_head = out.data_ptr(), out.stride(0), out.stride(1)
     a.key_cache, a.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
@@ -204,15 +402,14 @@ def _paged_attention_kernel(query, key_cache, value_cache, out, cu, used, table,
     a.cu_is64, a.used_is64 = cu.dtype == torch.int64, used.dtype == torch.int64
     a.table_is64 = table.dtype == torch.int64
     a.softmax_scale = float(scale)
-    lib = _lib.load()
     with torch.cuda.device(dev):
         # A buffer of this call's own: threads that share a stream may interleave
         # their launches, and a shared one would be written between the chunks and
         # their merge. The caching allocator hands it on in stream order.
-        ws = torch.empty(max(int(lib.fp_paged_workspace_bytes(ctypes.byref(a))), 256),
-                         dtype=torch.uint8, device=dev)
-        _lib.check(lib.fp_paged_attention(ctypes.byref(a), ws.data_ptr(),
-                                          torch.cuda.current_stream(dev).cuda_stream))
+        ws = torch.empty(max(int(ws_bytes(ctypes.byref(call))), 256), dtype=torch.uint8,
+                         device=dev)
+        _lib.check(launch(ctypes.byref(call), ws.data_ptr(),
+                          torch.cuda.current_stream(dev).cuda_stream))
     # a graph that saved `out` finds it changed, as after any in-place operation
     torch.autograd.graph.increment_version(out)
 
@@ -220,7 +417,9 @@ def _paged_attention_kernel(query, key_cache, value_cache, out, cu, used, table,
 def paged_attention_reference(query: torch.Tensor, key_cache: torch.Tensor,
                               value_cache: torch.Tensor, out: torch.Tensor,
                               cu_seqlens_q: torch.Tensor, seqused_k: torch.Tensor,
-                              block_table: torch.Tensor, softmax_scale: float) -> None:
+                              block_table: torch.Tensor, softmax_scale: float,
+                              k_scale: Optional[torch.Tensor] = None,
+                              v_scale: Optional[torch.Tensor] = None) -> None:
     """The torch composition of ``paged_decode_attention`` in fp32 (one small
     gather per sequence): the kernels' reference, and the path of the calls
     they do not take."""
@@ -236,8 +435,8 @@ def paged_attention_reference(query: torch.Tensor, key_cache: torch.Tensor,
             continue
         nblk = (nk + bs - 1) // bs
         blocks = block_table[b, :nblk].long()
-        k = key_cache[blocks].reshape(nblk * bs, hkv, d)[:nk].float()
-        v = value_cache[blocks].reshape(nblk * bs, hkv, d)[:nk].float()
+        k = _pages_fp32(key_cache, blocks, k_scale).reshape(nblk * bs, hkv, d)[:nk]
+        v = _pages_fp32(value_cache, blocks, v_scale).reshape(nblk * bs, hkv, d)[:nk]
         q = query[q0:q1].float()  # (nq, hq, d)
         k = k.repeat_interleave(g, dim=1).permute(1, 2, 0).contiguous()  # (hq, d, nk)
         v = v.repeat_interleave(g, dim=1).permute(1, 0, 2).contiguous()  # (hq, nk, d)
@@ -249,17 +448,57 @@ def paged_attention_reference(query: torch.Tensor, key_cache: torch.Tensor,
         out[q0:q1] = o.permute(1, 0, 2).to(out.dtype)
 
 
+def _pages_fp32(cache: torch.Tensor, blocks: torch.Tensor,
+                scale: Optional[torch.Tensor]) -> torch.Tensor:
+    """The pages' values in fp32, (blocks, block_size, Hkv, d)."""
+    if cache.dtype not in _FORMATS:
+        return cache[blocks].float()
+    x = cache.view(torch.uint8)[blocks].view(cache.dtype).float()
+    if scale is None:
+        return x
+    if scale.dim() == 3:
+        return x * scale[blocks].transpose(1, 2).unsqueeze(-1)
+    return x * scale.to(x.device).view(-1, 1)
+
+
 @dataclass
 class HookOps:
     """The operations the hooked forward calls; the defaults are this
     package's (KV-cache write kernel, FlashPrefill, paged attention).
     ``encoder`` and ``cascade`` take the impl and the reference's arguments
-    and default to raising: they stay vLLM's."""
+    and default to raising: they stay vLLM's. ``cache_write_fp8`` and
+    ``decode_fp8`` serve layers with an fp8 cache: the operations above with the
+    scales as two more arguments."""
     cache_write: Callable[..., None] = reshape_and_cache
     prefill: Callable[..., None] = flash_prefill_varlen_func
     decode: Callable[..., None] = paged_decode_attention
     encoder: Optional[Callable[..., torch.Tensor]] = None
     cascade: Optional[Callable[..., torch.Tensor]] = None
+    cache_write_fp8: Callable[..., None] = reshape_and_cache
+    decode_fp8: Callable[..., None] = paged_decode_attention
+
+
+def _cache_ops(impl, layer, ops: HookOps, key_cache, value_cache):
+    """The layer's caches, its cache write and its attention over them: those of
+    ``ops``, or for an fp8 ``kv_cache_dtype`` the 8-bit forms with the layer's
+    ``_k_scale`` / ``_v_scale`` (1 where it has none) over the caches, which vLLM
+    allocates as bytes, in their type."""
+    name = str(getattr(impl, "kv_cache_dtype", "auto"))
+    if not name.startswith("fp8"):
+        return key_cache, value_cache, ops.cache_write, ops.decode
+    dtype = _FP8_NAMES.get(name)
+    if dtype is None or key_cache.dtype not in (torch.uint8, dtype):
+        raise NotImplementedError(f"kv_cache_dtype {name} with a cache of {key_cache.dtype} is not "
+                                  f"supported by this hook (8-bit caches: {sorted(_FP8_NAMES)})")
+    scales = getattr(layer, "_k_scale", None), getattr(layer, "_v_scale", None)
+
+    def write(key, value, kc, vc, slots):
+        ops.cache_write_fp8(key, value, kc, vc, slots, *scales)
+
+    def decode(q, kc, vc, out, cu, used, table, scale):
+        ops.decode_fp8(q, kc, vc, out, cu, used, table, scale, *scales)
+
+    return key_cache.view(dtype), value_cache.view(dtype), write, decode
 
 
 def _is_encoder(attn_type) -> bool:
@@ -288,12 +527,11 @@ def make_forward(cfg: Dict[str, Any], ops: Optional[HookOps] = None):
                 raise NotImplementedError("encoder attention is left to vLLM's backend")
             return ops.encoder(self, query[:n], key[:n], value[:n], output[:n], attn_metadata,
                                layer)
-        key_cache, value_cache = kv_cache.unbind(0)
+        key_cache, value_cache, cache_write, decode = _cache_ops(self, layer, ops,
+                                                                 *kv_cache.unbind(0))
         if getattr(self, "kv_sharing_target_layer_name", None) is None and key is not None \
                 and value is not None:
-            if str(getattr(self, "kv_cache_dtype", "auto")).startswith("fp8"):
-                raise NotImplementedError("fp8 KV caches are not supported by this hook")
-            ops.cache_write(key, value, key_cache, value_cache, attn_metadata.slot_mapping)
+            cache_write(key, value, key_cache, value_cache, attn_metadata.slot_mapping)
         if getattr(attn_metadata, "use_cascade", False):
             if ops.cascade is None:
                 raise NotImplementedError("cascade attention is left to vLLM's backend")
@@ -307,9 +545,9 @@ def make_forward(cfg: Dict[str, Any], ops: Optional[HookOps] = None):
                         attn_metadata.max_query_len, cfg["alpha"], cfg["block_size"],
                         cfg["attention_sink"], cfg["window_size"], cfg["last_n_full_block"])
         else:
-            ops.decode(query[:n], key_cache, value_cache, output[:n], cu_seqlens_q,
-                       attn_metadata.seq_lens, attn_metadata.block_table,
-                       getattr(self, "scale", 1.0 / math.sqrt(query.shape[-1])))
+            decode(query[:n], key_cache, value_cache, output[:n], cu_seqlens_q,
+                   attn_metadata.seq_lens, attn_metadata.block_table,
+                   getattr(self, "scale", 1.0 / math.sqrt(query.shape[-1])))
         return output
 
     return flash_prefill_forward
@@ -355,7 +593,7 @@ def make_forward_v0(cfg: Dict[str, Any], ops: Optional[HookOps] = None):
     (patches/patch_loader_vllm_0_10_0.py:78-376), closed over ``cfg``:
 
     * the step's key / value rows go into the paged cache at ``slot_mapping``
-      when the cache is allocated (:139-172); fp8 caches are rejected;
+      when the cache is allocated (:139-172), an fp8 cache with the layer's scales;
     * the batch's first ``num_prefill_tokens`` query rows are prefill, the
       ``num_decode_tokens`` after them decode (:186-195);
     * prefill without block tables (or with an empty cache) is FlashPrefill
@@ -386,16 +624,15 @@ def make_forward_v0(cfg: Dict[str, Any], ops: Optional[HookOps] = None):
                 raise NotImplementedError("encoder and encoder-decoder attention are left to "
                                           "vLLM's backend")
             return ops.encoder(self, query, key, value, output, attn_metadata, layer)
-        fp8 = str(getattr(self, "kv_cache_dtype", "auto")).startswith("fp8")
-        if fp8:
-            raise NotImplementedError("fp8 KV caches are not supported by this hook")
         scale = getattr(self, "scale", 1.0 / math.sqrt(query.shape[-1]))
         key_cache = value_cache = None
+        decode = ops.decode
         if kv_cache.numel() > 0:
-            key_cache, value_cache = kv_cache[0], kv_cache[1]
+            key_cache, value_cache, cache_write, decode = _cache_ops(self, layer, ops,
+                                                                     kv_cache[0], kv_cache[1])
             if key is not None and value is not None:
-                ops.cache_write(key, value, key_cache, value_cache,
-                                attn_metadata.slot_mapping.flatten())
+                cache_write(key, value, key_cache, value_cache,
+                            attn_metadata.slot_mapping.flatten())
         n_pre = attn_metadata.num_prefill_tokens
         n_dec = attn_metadata.num_decode_tokens
         prefill_meta = attn_metadata.prefill_metadata
@@ -407,9 +644,8 @@ def make_forward_v0(cfg: Dict[str, Any], ops: Optional[HookOps] = None):
                             cfg["alpha"], cfg["block_size"], cfg["attention_sink"],
                             cfg["window_size"], cfg["last_n_full_block"])
             else:  # prefix caching: the new queries end each cached sequence
-                ops.decode(query[:n_pre], key_cache, value_cache, output[:n_pre],
-                           prefill_meta.query_start_loc, prefill_meta.seq_lens_tensor, tables,
-                           scale)
+                decode(query[:n_pre], key_cache, value_cache, output[:n_pre],
+                       prefill_meta.query_start_loc, prefill_meta.seq_lens_tensor, tables, scale)
         decode_meta = attn_metadata.decode_metadata
         if decode_meta is not None:
             dq = query[n_pre:n_pre + n_dec]
@@ -419,8 +655,8 @@ def make_forward_v0(cfg: Dict[str, Any], ops: Optional[HookOps] = None):
             else:  # one query per sequence
                 cu = torch.arange(decode_meta.seq_lens_tensor.numel() + 1, dtype=torch.int32,
                                   device=query.device)
-            ops.decode(dq, key_cache, value_cache, dout, cu, decode_meta.seq_lens_tensor,
-                       decode_meta.block_tables, scale)
+            decode(dq, key_cache, value_cache, dout, cu, decode_meta.seq_lens_tensor,
+                   decode_meta.block_tables, scale)
         return output
 
     return flash_prefill_forward_v0

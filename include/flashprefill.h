@@ -29,7 +29,8 @@
  *   fp_sparse_attn_fwd     _flash_forward / _flash_block_sparse_varlen
  *                          ops/flashprefill_native_forward.py:227-344, ops/flashprefill_varlen_func.py:449-575
  *   fp_kv_cache_write      the paged KV-cache write the vLLM patch makes before attention
- *                          (reshape_and_cache_flash, patches/patch_loader_vllm_0_12_0.py:140-149)
+ *                          (reshape_and_cache_flash, patches/patch_loader_vllm_0_12_0.py:140-149);
+ *                          fp_kv_cache_write_fp8: into a cache of 8-bit floats
  */
 #ifndef FLASHPREFILL_H
 #define FLASHPREFILL_H
@@ -199,6 +200,56 @@ typedef struct fp_kv_cache_args {
 } fp_kv_cache_args;
 int fp_kv_cache_write(const fp_kv_cache_args* a, void* stream);
 
+/* Caches of 8-bit floats: element c of a row stands for c * s. */
+#define FP_CACHE_16BIT 0 /* the 16-bit input type (fp_kv_cache_gather) */
+#define FP_CACHE_E4M3 1  /* largest finite value 448, no infinity */
+#define FP_CACHE_E5M2 2  /* largest finite value 57344 */
+
+/* Scales s of the K or V rows of an 8-bit cache, fp32 in device memory. data NULL:
+ * 1. per_slot 0: fixed, data[h * stride_head] for KV head h (stride_head 0: one
+ * for all), stride_block unused. per_slot 1: data[block * stride_block +
+ * h * stride_head + slot], found and stored by the write. */
+typedef struct fp_kv_scales {
+  float* data;
+  int64_t stride_block, stride_head;
+  int32_t per_slot;
+} fp_kv_scales;
+
+/* fp_kv_cache_write into an 8-bit cache. base.dtype: key's and value's type; the
+ * cache strides count bytes (multiples of 8; bases 8-byte aligned); head_dim a
+ * multiple of 8 up to 512. Stores F(clamp(x / s, -M, M)): the fp32 quotient,
+ * rounded to nearest even, M the format's largest finite value; infinities
+ * saturate, NaN stays NaN. A scale per slot is max |x| / M over the row's finite
+ * values, 1 where that is 0. Slots that two tokens name hold either row, or parts
+ * of both. */
+typedef struct fp_kv_cache_fp8_args {
+  fp_kv_cache_args base;
+  fp_kv_scales k_scale, v_scale;
+  int32_t format; /* FP_CACHE_E4M3 or FP_CACHE_E5M2 */
+} fp_kv_cache_fp8_args;
+int fp_kv_cache_write_fp8(const fp_kv_cache_fp8_args* a, void* stream);
+
+/* Read-back of a paged cache into packed rows: row cu[b] + i of key / value, up to
+ * cu[b + 1] - 1, is cached token starts[b] + i (starts NULL: i) of sequence b, as
+ * c * s in fp32 rounded once to the 16-bit type (FP_CACHE_16BIT: a copy). Rows of
+ * no sequence are left as they are. What the host cannot see is checked by the
+ * kernel: offsets outside [0, num_tokens] or descending make every row NaN, tokens
+ * past the table's room or before the first one, and pages outside the cache (one
+ * below 0 counts from the end), their rows. The integer arrays hold 32- or 64-bit
+ * integers. base.slot_mapping is not used; base.key / value are written. */
+typedef struct fp_kv_gather_args {
+  fp_kv_cache_args base;
+  fp_kv_scales k_scale, v_scale;
+  int32_t format;
+  int32_t batch, table_width;
+  int32_t cu_is64, table_is64, starts_is64;
+  const void* cu_seqlens;  /* device, batch + 1 entries */
+  const void* block_table; /* device, batch rows of table_width entries */
+  const void* starts;      /* device, batch entries, or NULL */
+  int64_t table_stride;    /* entries between rows */
+} fp_kv_gather_args;
+int fp_kv_cache_gather(const fp_kv_gather_args* a, void* stream);
+
 /* Attention over a paged KV cache (decode steps, and prefill whose prefix is
  * cached): query rows cu[b] .. cu[b + 1] - 1 of sequence b are its last tokens,
  * i.e. row t attends to the first used[b] - (cu[b + 1] - 1 - t) cached tokens,
@@ -241,6 +292,20 @@ typedef struct fp_paged_args {
 } fp_paged_args;
 size_t fp_paged_workspace_bytes(const fp_paged_args* a); /* 0: none needed, or invalid */
 int fp_paged_attention(const fp_paged_args* a, void* workspace, void* stream);
+
+/* fp_paged_attention over an 8-bit cache: key c_k s_k, value c_v s_v. base.dtype:
+ * the type of q and o; the cache strides count bytes (multiples of 16); scales per
+ * slot are 16-byte aligned, with strides of multiples of 4, where block_size is a
+ * multiple of 16. No cached value is rounded: the scales multiply fp32 scores,
+ * probabilities and sums. A call of many rows holds the product of a probability
+ * and its value's scale to 2^-17. */
+typedef struct fp_paged_fp8_args {
+  fp_paged_args base;
+  fp_kv_scales k_scale, v_scale;
+  int32_t format; /* FP_CACHE_E4M3 or FP_CACHE_E5M2 */
+} fp_paged_fp8_args;
+size_t fp_paged_fp8_workspace_bytes(const fp_paged_fp8_args* a); /* 0: none needed, or invalid */
+int fp_paged_attention_fp8(const fp_paged_fp8_args* a, void* workspace, void* stream);
 
 /* Rotary position embedding (rotate-half) with optional per-head RMSNorm, in
  * place on the query and key heads of a decoder-layer attention block. No
