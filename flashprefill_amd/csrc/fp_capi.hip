@@ -709,16 +709,15 @@ int cache8_valid(const fp_kv_cache_args* a, const fp_kv_scales& ks, const fp_kv_
                  const char* what, int elem) {
   if (a->dtype != FP_DTYPE_BF16 && a->dtype != FP_DTYPE_F16)
     return fail(FP_E_UNSUPPORTED, "%s: dtype %d unsupported (bf16 or fp16 only)", what, a->dtype);
-  if (a->num_tokens < 0 || a->num_blocks < 0 || a->block_size < 1 || a->num_kv_heads < 1 ||
-      a->head_dim < 8 || a->head_dim % 8)
+  if (a->num_tokens < 0 || (a->num_tokens > 0 && a->num_blocks < 1) || a->block_size < 1 ||
+      a->num_kv_heads < 1 || a->head_dim < 8 || a->head_dim % 8)
     return fail(FP_E_INVALID_ARG, "%s: sizes out of range (head_dim must be a multiple of 8)", what);
   if (a->head_dim > 512) return fail(FP_E_UNSUPPORTED, "%s: head_dim %d above 512", what, a->head_dim);
   if (a->num_tokens == 0) return FP_OK;
-  // a launch holds fewer than 2^32 threads: at most 64 per row, K and V rows of every
-  // head of a token
-  if (a->num_tokens * a->num_kv_heads >= (int64_t(1) << 25) &&
-      a->num_tokens * a->num_kv_heads * 2 * fp::row_lanes(a->head_dim) >= (int64_t(1) << 32) - 256)
-    return fail(FP_E_UNSUPPORTED, "%s: 2^32 or more threads' work in one call", what);
+  // (a launch holds fewer than 2^32 threads)
+  if (a->num_tokens >= int64_t(fp::kRowTokens) << 24)
+    return fail(FP_E_UNSUPPORTED, "%s: %lld tokens in one call", what,
+                static_cast<long long>(a->num_tokens));
   if (!a->key || !a->value || !a->key_cache || !a->value_cache)
     return fail(FP_E_INVALID_ARG, "%s: NULL pointer", what);
   if (!aligned16(a->key) || !aligned16(a->value))

@@ -186,15 +186,28 @@ struct Cache8Args {
   CacheScales ks, vs;
 };
 
-// Lanes of one row of head_dim elements, 8 of them each: a power of two, at most 64
-// (head dims up to 512)
-inline int row_lanes(int head_dim) {
-  int n = 1;
-  while (n < head_dim / 8) n *= 2;
-  return n;
+// How the kernels that move rows of the cache walk them: a workgroup of 256 threads
+// takes `tokens` tokens (a power of two, at most kRowTokens) and all K and V heads
+// of each, 1 << lg lanes to a row of head_dim elements (8 each; head dims up to 512).
+// Rows are numbered (token, K heads, V heads); a thread's next row lies 256 >> lg
+// rows, i.e. `di` tokens and `dh` heads, further on.
+constexpr int kRowTokens = 16;
+struct RowWalk {
+  int32_t lg, tokens, di, dh;
+};
+inline RowWalk row_walk(int head_dim, int num_kv_heads, int64_t num_tokens) {
+  RowWalk w;
+  w.lg = 0;
+  while ((1 << w.lg) < head_dim / 8) ++w.lg;
+  const int step = 256 >> w.lg, per = 2 * num_kv_heads;
+  w.di = step / per;
+  w.dh = step % per;
+  // the most that leaves the card's 256 CUs four workgroups each (14,500 tokens of 4
+  // heads of 128 written: 16 us with four, 24 with eight)
+  w.tokens = kRowTokens;
+  while (w.tokens > 1 && num_tokens / w.tokens < 1024) w.tokens /= 2;
+  return w;
 }
-
-constexpr int kGatherTokens = 16;  // tokens per workgroup of the read-back
 
 struct GatherArgs {
   Cache8Args g;  // c.num_tokens: rows of key / value
