@@ -622,6 +622,29 @@ fp::KvCacheArgs cache_args(const fp_kv_cache_args* a) {
   return k;
 }
 
+// An 8-bit call: many rows as a 16-bit one. Few: kPaged8Groups workgroups, as many as
+// the card holds at a time, share the keys in units of 128 (more where the units would
+// not count in 31 bits); where the table has room for kWhole keys at most, each segment
+// (16 rows of a KV head's queries) is a workgroup's as a whole.
+PagedSplit paged8_split(const fp_paged_args* a, int* unit, int* groups) {
+  constexpr int kWhole = 512;
+  PagedSplit r = paged_split(a);
+  *unit = 128;
+  const int pair = a->head_dim == 64 && a->num_kv_heads % 2 == 0 ? 2 : 1;
+  *groups = a->num_kv_heads / pair;
+  if (r.many) return r;
+  const int64_t longest = static_cast<int64_t>(a->table_width) * a->block_size;
+  const int64_t segs = std::max<int64_t>(1, r.tiles * *groups);
+  const auto units = [&] { return segs * std::max<int64_t>(1, (longest + *unit - 1) / *unit); };
+  r.bytes = 0;
+  if (longest <= kWhole) *unit = 1 << 30;
+  while (*unit < 1 << 30 && units() >= int64_t(1) << 31) *unit *= 2;
+  r.nc = static_cast<int>(longest <= kWhole ? segs
+                                            : std::min<int64_t>(fp::kPaged8Groups, units()));
+  if (longest > kWhole) r.bytes = static_cast<size_t>(r.nc) * 2 * 16 * pair * (a->head_dim + 2) * 4;
+  return r;
+}
+
 // Argument block of the paged kernels; partials behind each other in the workspace.
 fp::PagedArgs paged_args(const fp_paged_args* a, const PagedSplit& sp, void* ws) {
   fp::PagedArgs r{};
@@ -642,9 +665,9 @@ fp::PagedArgs paged_args(const fp_paged_args* a, const PagedSplit& sp, void* ws)
   r.cu = a->cu_seqlens;
   r.used = a->seqused;
   r.table = a->block_table;
-  r.cu64 = a->cu_is64;
-  r.used64 = a->used_is64;
-  r.table64 = a->table_is64;
+  r.cu64 = a->cu_is64 != 0;
+  r.used64 = a->used_is64 != 0;
+  r.table64 = a->table_is64 != 0;
   r.table_stride = a->table_stride;
   r.T = a->num_tokens;
   r.nblocks = a->num_blocks;
@@ -659,9 +682,9 @@ fp::PagedArgs paged_args(const fp_paged_args* a, const PagedSplit& sp, void* ws)
   r.G = a->num_q_heads / a->num_kv_heads;
   r.scale_log2 = a->softmax_scale * static_cast<float>(1.4426950408889634);
   r.nc = sp.nc;
-  r.part = static_cast<float*>(ws);
-  r.ml = sp.nc > 1 ? static_cast<float*>(ws) + a->num_tokens * a->num_q_heads * sp.nc * a->head_dim
-                   : nullptr;
+  // partials, then their (m, l): head_dim + 2 floats each
+  r.part = sp.bytes > 0 ? static_cast<float*>(ws) : nullptr;
+  r.ml = sp.bytes > 0 ? r.part + sp.bytes / 4 / (a->head_dim + 2) * a->head_dim : nullptr;
   return r;
 }
 
@@ -894,17 +917,20 @@ int fp_paged_attention(const fp_paged_args* a, void* ws, void* stream) {
 }
 
 size_t fp_paged_fp8_workspace_bytes(const fp_paged_fp8_args* a) {
-  return paged8_valid(a) == FP_OK ? paged_split(&a->base).bytes : 0;
+  int unit, groups;
+  return paged8_valid(a) == FP_OK ? paged8_split(&a->base, &unit, &groups).bytes : 0;
 }
 
 int fp_paged_attention_fp8(const fp_paged_fp8_args* a, void* ws, void* stream) {
   const int rc = paged8_valid(a);
   if (rc != FP_OK) return rc;
   if (a->base.num_tokens == 0) return FP_OK;
-  const PagedSplit sp = paged_split(&a->base);
+  fp::Paged8Args r;
+  const PagedSplit sp = paged8_split(&a->base, &r.unit, &r.groups);
   if (sp.bytes > 0 && !ws) return fail(FP_E_INVALID_ARG, "paged: workspace is NULL");
   if (!aligned16(ws)) return fail(FP_E_INVALID_ARG, "paged: workspace must be 16-byte aligned");
-  fp::Paged8Args r;
+  r.min_share = r.unit == 128 ? 2 : 1;
+  r.segs = sp.tiles * r.groups;
   r.a = paged_args(&a->base, sp, ws);
   r.ks = scales(a->k_scale);
   r.vs = scales(a->v_scale);
@@ -972,9 +998,9 @@ int fp_kv_cache_gather(const fp_kv_gather_args* a, void* stream) {
   r.cu = a->cu_seqlens;
   r.table = a->block_table;
   r.starts = a->starts;
-  r.cu64 = a->cu_is64;
-  r.table64 = a->table_is64;
-  r.starts64 = a->starts_is64;
+  r.cu64 = a->cu_is64 != 0;
+  r.table64 = a->table_is64 != 0;
+  r.starts64 = a->starts_is64 != 0;
   r.table_stride = a->table_stride;
   r.num_blocks = a->base.num_blocks;
   r.B = a->batch;

@@ -159,8 +159,8 @@ struct PagedArgs {
   int32_t nc;        // chunk slots per row
   float* part;       // [T * Hq][nc][d] unnormalised outputs
   float* ml;         // [T * Hq][nc] (m, l) pairs
-  // V scale of KV head h at [h * vscale_head], by which the merge multiplies a
-  // row's sum (8-bit caches with fixed scales), or null
+  // V scale of KV head h at [h * vscale_head], by which k_paged_merge_rows multiplies
+  // a row's sum (8-bit caches with fixed scales), or null
   const float* vscale;
   int32_t vscale_head;
 };
@@ -173,10 +173,16 @@ struct CacheScales {
   int32_t slot;
 };
 
-// Attention over a paged 8-bit cache (fp_paged8.hip)
+// Attention over a paged 8-bit cache (fp_paged8.hip). k_paged8: a.nc workgroups, whose
+// shares are whole units of `unit` keys, min_share at least; a.part and a.ml hold two
+// partials of 16 rows for each (null: a segment is one workgroup's).
+constexpr int kPaged8Groups = 512;  // workgroups where they share the keys, at most
 struct Paged8Args {
   PagedArgs a;
   CacheScales ks, vs;
+  int32_t unit, min_share;
+  int32_t groups;  // KV heads, or pairs of them that a segment serves together
+  int64_t segs;    // segments at most
 };
 
 // Write of an 8-bit cache and the read-back of any (fp_kvcache.hip): `key` and
@@ -254,9 +260,8 @@ hipError_t launch_rope(const RopeArgs& a, int dtype, hipStream_t s);
 hipError_t launch_paged_rows(const PagedArgs& a, int dtype, int head_dim, int64_t tiles,
                              hipStream_t s);
 hipError_t launch_paged(const PagedArgs& a, int dtype, int head_dim, int64_t tiles, hipStream_t s);
-// combines the partials of either kernel's 8-bit form (rows: k_paged8_rows)
-hipError_t launch_paged_merge(const PagedArgs& a, int dtype, int head_dim, bool rows,
-                              hipStream_t s);
+// combines the partials of k_paged_rows and its 8-bit form
+hipError_t launch_paged_merge_rows(const PagedArgs& a, int dtype, int head_dim, hipStream_t s);
 hipError_t launch_paged8(const Paged8Args& a, int dtype, int format, int head_dim, bool rows,
                          int64_t tiles, hipStream_t s);
 hipError_t launch_kv_cache_write8(const Cache8Args& a, int dtype, int format, hipStream_t s);

@@ -25,8 +25,112 @@ __device__ __forceinline__ void bf16_parts(float x0, float x1, uint32_t (&u)[N])
   }
 }
 
-// Few rows: a workgroup takes (16 rows of a KV head's queries, KV head, chunk of
-// keys), its four waves 32 keys in turn, straight from the pages into registers.
+// ---------------------------------------------------------------------------
+// Few rows
+// ---------------------------------------------------------------------------
+// A segment is 16 rows of the queries of one (sequence, KV head or pair of them) with all
+// its keys, in units of `unit` keys; the segments of a call lie behind each other
+// (sequence, heads, row tile) and every workgroup takes an equal share of the units, whatever segments
+// they belong to: a decode step reads each cached byte once, so equal bytes take equal
+// times, and no workgroup starts for keys that are not there (the host cannot see the
+// lengths without a synchronisation). A segment that is one workgroup's is written out,
+// the others as partials (O, m, l), the first and the last of a workgroup at most, which
+// k_paged8_merge combines. Where the table has room for few keys, a unit is a whole
+// sequence and a segment a workgroup's: no merge.
+struct Work {
+  int total, share;  // units of the call, and of a workgroup
+  PagedSeq s;        // the sequence at the place asked for
+  int b;             // (below 0: no such place)
+  int units, segs;   // units and segments of the sequences before it
+};
+
+__device__ __forceinline__ int seq_tiles(const PagedArgs& a, const PagedSeq& s) {
+  return static_cast<int>((static_cast<int64_t>(s.nq) * a.G + 15) / 16);
+}
+// (unit: a power of two)
+__device__ __forceinline__ int seq_units(int unit, const PagedSeq& s) {
+  return max(static_cast<int>((s.nk + unit - 1) >> (31 - __clz(unit))), 1);
+}
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return static_cast<int64_t>(
+      static_cast<uint64_t>(static_cast<uint32_t>(
+          __builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32)))) << 32 |
+      static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x))));
+}
+__device__ __forceinline__ PagedSeq uniform_seq(const PagedSeq& s) {
+  return PagedSeq{uniform64(s.q0), __builtin_amdgcn_readfirstlane(s.nq), uniform64(s.nk),
+                  __builtin_amdgcn_readfirstlane(static_cast<int>(s.bad)) != 0, false};
+}
+// sums over the lanes up to this one: within rows of 16 lanes, then across them
+__device__ __forceinline__ int lane_prefix(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+
+// By one wave, 64 sequences at a time: the place of workgroup wg's first unit, or with
+// seg >= 0 that of a segment. Where some sequence's offsets do not fit, which rows are
+// whose is unknown: all rows of the call are one sequence's then, and bad.
+__device__ __forceinline__ Work find_work(const Paged8Args& pa, int wg, int64_t seg) {
+  const PagedArgs& a = pa.a;
+  const int lane = threadIdx.x & 63;
+  Work r;
+  r.b = -1;
+  r.units = r.segs = r.total = 0;
+  r.s = PagedSeq{0, 0, 0, false, false};
+  bool off = false;
+  PagedSeq s = r.s;
+  int ns = 0, nu = 0, is = 0, iu = 0;  // the lane's segments and units; with the lanes below
+  const auto load = [&](int base) {
+    s = paged_seq(a, min(base + lane, a.B - 1));
+    if (base + lane >= a.B) s = PagedSeq{0, 0, 0, false, false};
+    ns = seq_tiles(a, s) * pa.groups;
+    nu = ns * seq_units(pa.unit, s);
+    is = lane_prefix(ns);
+    iu = lane_prefix(nu);
+  };
+  for (int base = 0; base < a.B; base += 64) {
+    load(base);
+    off = off || __ballot(s.off) != 0;
+    r.total += __builtin_amdgcn_readlane(iu, 63);
+  }
+  if (off) {
+    r.s = PagedSeq{0, static_cast<int>(a.T), 0, true, true};
+    r.total = seq_tiles(a, r.s) * pa.groups;
+  }
+  r.share = max((r.total + a.nc - 1) / a.nc, pa.min_share);
+  const int64_t x = static_cast<int64_t>(wg) * r.share;
+  if (seg < 0 && x >= r.total) return r;
+  if (off) {
+    r.b = seg < r.total ? 0 : -1;
+    return r;
+  }
+  for (int base = 0; base < a.B; base += 64) {
+    if (a.B > 64) load(base);
+    const int64_t y = seg >= 0 ? seg - r.segs : x - r.units;
+    const bool mine = seg >= 0 ? y >= is - ns && y < is : y >= iu - nu && y < iu;
+    const uint64_t hit = __ballot(mine);
+    if (hit != 0) {
+      const int l = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<long long>(hit)) - 1);
+      r.b = base + l;
+      r.s = uniform_seq(PagedSeq{shfl64(s.q0, l), __shfl(s.nq, l), shfl64(s.nk, l),
+                                 __shfl(static_cast<int>(s.bad), l) != 0, false});
+      r.units += __builtin_amdgcn_readlane(iu - nu, l);
+      r.segs += __builtin_amdgcn_readlane(is - ns, l);
+      return r;
+    }
+    r.units += __builtin_amdgcn_readlane(iu, 63);
+    r.segs += __builtin_amdgcn_readlane(is, 63);
+  }
+  return r;
+}
+
+// The four waves of a workgroup take 32 keys in turn, straight from the pages into
+// registers, a round ahead of their use:
 //
 //   S^T (keys x rows) = K . Q^T on v_mfma_f32_16x16x32: a lane (r = l % 16,
 //     g = l / 16) loads 16-byte pieces of key r, whose two halves are the operands
@@ -36,362 +140,499 @@ __device__ __forceinline__ void bf16_parts(float x0, float x1, uint32_t (&u)[N])
 //     dim E m + e, byte e of the E = D / 16 bytes that lane m loads of each of its
 //     8 keys: whole rows are loaded and nothing crosses lanes. v_perm pairs the
 //     bytes of two keys, one conversion each makes them an operand word.
-template <typename T, int F, int D, bool P16>
-__global__ __launch_bounds__(256, D > 128 || !P16 ? 2 : 3) void k_paged8(Paged8Args pa) {
+//
+// HP: KV heads of a segment, each served by 4 / HP of the waves. A key of 64 bytes is half
+// a cache line, and the other half its neighbour head's: served apart they are fetched
+// twice (16 sequences of 40 .. 9,000 tokens, 8 KV heads, d = 64, 4 queries each: 35 us with
+// one head per segment).
+//
+// P16: the page size is a multiple of 16, so a 16-key tile lies in one page: a wave
+// looks up 64 of them at a time, one per lane, and reads a tile's place from its lane.
+// PS: all scales are per slot. Other pages, and scales of which only K's or only V's are
+// per slot, take the general form (neither).
+template <typename T, int F, int D, bool P16, bool PS, int HP>
+__global__ __launch_bounds__(256, 2) void k_paged8(Paged8Args pa) {
   constexpr int KS = D / 32;  // MFMA k-steps over the head dim
   constexpr int KP = D / 64;  // 16-byte pieces of a key per lane
   constexpr int E = D / 16;   // V bytes per lane and key
   constexpr int VW = E / 4;   // the same in words
   constexpr int OS = D + 4;   // padded row of the merge buffer (floats)
   constexpr int NP = 3;       // parts of P
+  constexpr bool kScaled = PS || !P16;
+  constexpr int NW = 4 / HP;  // waves of a head
+  constexpr int RK = 32 * NW;  // keys of a round, all waves of a head
   __shared__ float sm[4][16][OS];
   __shared__ float sml[4][16][2];
   const PagedArgs& a = pa.a;
-  const int h = static_cast<int>(blockIdx.x % a.Hkv);
-  const int64_t x = blockIdx.x / a.Hkv;
-  const int c = static_cast<int>(blockIdx.y);
-  const PagedTile tile = paged_find(a, 16, x, -1);
-  if (tile.b < 0) return;
-  const PagedSeq& sq = tile.s;
-  const int nk = static_cast<int>(sq.nk), nq = sq.nq;
-  const int k0 = c * tile.chunk;
-  if (k0 >= nk && c > 0) return;
-  const bool single = nk <= tile.chunk;
-  const int k1 = min(k0 + tile.chunk, nk);
+  const Work work = find_work(pa, static_cast<int>(blockIdx.x), -1);
+  if (work.b < 0) return;
   const int t = threadIdx.x, lane = t & 63;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int hw = w / NW, kw = w % NW;  // the wave's head of the segment, and its turn
   const int r16 = lane & 15, g = lane >> 4;
+  int b = work.b;
+  PagedSeq sq = work.s;
+  const int start = static_cast<int>(blockIdx.x) * work.share;
+  int left = min(work.share, work.total - start);
+  int tiles = seq_tiles(a, sq), units = seq_units(pa.unit, sq);
+  int seg = __builtin_amdgcn_readfirstlane((start - work.units) / units);
+  int u = start - work.units - seg * units;
+  for (bool first = true;; first = false) {
+    const int hg = __builtin_amdgcn_readfirstlane(seg / tiles), tl = seg - hg * tiles;
+    const int h = hg * HP + hw;
+    const int take = min(units - u, left);
+    const bool single = take == units;
+    const int nk = static_cast<int>(sq.nk), nq = sq.nq;
+    const int k0 = u * pa.unit;
+    const int k1 = single ? nk : min(k0 + take * pa.unit, nk);
 
-  // this lane's query row (B operand column) and its last visible key
-  const int rr = tile.tl * 16 + r16;
-  const bool rvalid = rr < nq * a.G;
-  const int qi = rvalid ? rr / a.G : 0;
-  const int lim = rvalid ? nk - nq + qi : nk - 1;
-  typename T::vec8 qb[KS];
-  {
-    const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (sq.q0 + qi) * a.qst +
-                         static_cast<int64_t>(h * a.G + (rvalid ? rr % a.G : 0)) * a.qhs + 16 * g;
+    // this lane's query row (B operand column) and its last visible key
+    const int rr = tl * 16 + r16;
+    const bool rvalid = rr < nq * a.G;
+    const int qi = rvalid ? rr / a.G : 0;
+    const int lim = rvalid ? nk - nq + qi : nk - 1;
+    typename T::vec8 qb[KS];
+    {
+      const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (sq.q0 + qi) * a.qst +
+                           static_cast<int64_t>(h * a.G + (rvalid ? rr % a.G : 0)) * a.qhs + 16 * g;
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
-      qb[s] = as_vec8<T>(rvalid ? ld16(qp + 64 * (s >> 1) + 8 * (s & 1)) : zero4());
-  }
+      for (int s = 0; s < KS; ++s) {
+        const uint4 x = ld16(qp + 64 * (s >> 1) + 8 * (s & 1));
+        qb[s] = as_vec8<T>(rvalid ? x : zero4());
+      }
+    }
 
-  f32x4 acc[E];
+    f32x4 acc[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = f32x4{};
-  float m_run = -INFINITY, l_part = 0.0f;
-  bool bad = false;
-  const int64_t row = static_cast<int64_t>(tile.b) * a.table_stride;
-  const uint8_t* kc = static_cast<const uint8_t*>(a.kc) + static_cast<int64_t>(h) * a.kch;
-  const uint8_t* vc = static_cast<const uint8_t*>(a.vc) + static_cast<int64_t>(h) * a.vch;
-  const float* kss = pa.ks.p + h * pa.ks.sh;  // read when there is one per slot
-  const float* vss = pa.vs.p + h * pa.vs.sh;
-  const float scale = a.scale_log2 * fixed_scale(pa.ks, h);
+    for (int e = 0; e < E; ++e) acc[e] = f32x4{};
+    float m_run = -INFINITY, l_part = 0.0f;
+    bool bad = false;
+    const int64_t row = static_cast<int64_t>(b) * a.table_stride;
+    const uint8_t* kc = static_cast<const uint8_t*>(a.kc) + static_cast<int64_t>(h) * a.kch;
+    const uint8_t* vc = static_cast<const uint8_t*>(a.vc) + static_cast<int64_t>(h) * a.vch;
+    const float* kss = pa.ks.p + h * pa.ks.sh;  // read where there is one per slot
+    const float* vss = pa.vs.p + h * pa.vs.sh;
+    const float scale = a.scale_log2 * fixed_scale(pa.ks, h);
 
-  uint4 kf[2][KP];
-  uint32_t vf[2][4][VW];
-  float ksc[2][4], vsc[2][4];
+    // what a round loads: 32 keys, lanes as above
+    struct {
+      uint4 k[2][KP];
+      uint32_t v[2][4][VW];
+      f32x4 ks[2], vs[2];
+    } r;
+    // places of the 64 16-key tiles from key `win`, one per lane (P16; tiles past the
+    // sequence repeat the last one, their scores are masked)
+    int win = k0;
+    int64_t kat = 0, vat = 0, ksat = 0, vsat = 0;
+    const int last16 = (nk - 1) & ~15;
+    auto look = [&](int from) {
+      win = from;
+      const int key = min(from + 16 * lane, last16);
+      const int64_t pg = paged_page<false>(a, row, key, bad);
+      const int in = a.bs_shift >= 0 ? key & (a.bs - 1) : key % a.bs;
+      kat = pg * a.kcb + in * a.kcs;
+      vat = pg * a.vcb + in * a.vcs;
+      if constexpr (PS) {
+        ksat = pg * pa.ks.sb + in;
+        vsat = pg * pa.vs.sb + in;
+      }
+    };
+    auto place = [&](int64_t x, int tile) {
+      return static_cast<int64_t>(
+          static_cast<uint64_t>(static_cast<uint32_t>(
+              __builtin_amdgcn_readlane(static_cast<int>(x >> 32), tile))) << 32 |
+          static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), tile)));
+    };
+    // a lane's offsets in a tile
+    const uint32_t koff = static_cast<uint32_t>(r16 * static_cast<int>(a.kcs) + 16 * g);
+    uint32_t voff[4];
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+    for (int v = 0; v < 4; ++v)
+      voff[v] = static_cast<uint32_t>((4 * g + v) * static_cast<int>(a.vcs) + E * r16);
+    auto load_k = [&](int base) {
+      if constexpr (P16) {
+        if (base >= win + 1024) look(k0 + ((base - k0) & ~1023));
 #pragma unroll
-    for (int v = 0; v < 4; ++v) ksc[j][v] = vsc[j][v] = 1.0f;
-  // pages and in-page offsets of the two 16-key tiles from `base` (P16); a
-  // tile past the sequence repeats the last one (its scores are masked)
-  const int last16 = (nk - 1) & ~15;
-  int64_t page[2] = {0, 0};
-  int inpage[2] = {0, 0};
-  auto lookup = [&](int base) {
-    if constexpr (P16) {
+        for (int j = 0; j < 2; ++j) {
+          const int tile = ((base - win) >> 4) + j;
+          const uint8_t* p = kc + place(kat, tile);
+#pragma unroll
+          for (int s = 0; s < KP; ++s) r.k[j][s] = ld16(p + koff + 64 * s);
+          if constexpr (PS)
+            r.ks[j] = *reinterpret_cast<const f32x4*>(kss + place(ksat, tile) + 4 * g);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int key = min(base + 16 * j + r16, nk - 1);
+          const int64_t pg = paged_page<false>(a, row, key, bad);
+          const uint8_t* p = kc + pg * a.kcb + static_cast<int64_t>(key % a.bs) * a.kcs + 16 * g;
+#pragma unroll
+          for (int s = 0; s < KP; ++s) r.k[j][s] = ld16(p + 64 * s);
+          float f[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+          if (pa.ks.slot)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              const int kv = min(base + 16 * j + 4 * g + v, nk - 1);
+              f[v] = kss[paged_page<false>(a, row, kv, bad) * pa.ks.sb + kv % a.bs];
+            }
+          r.ks[j] = f32x4{f[0], f[1], f[2], f[3]};
+        }
+      }
+    };
+    auto load_v = [&](int base) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int tb = min(base + 16 * j, last16);
-        page[j] = paged_page<true>(a, row, tb, bad);
-        inpage[j] = a.bs_shift >= 0 ? tb & (a.bs - 1) : tb % a.bs;
-      }
-    }
-  };
-  auto load_scales = [&](float (&dst)[2][4], const CacheScales& cs, const float* sp, int base) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if constexpr (P16) {
-        const float4 u = *reinterpret_cast<const float4*>(sp + page[j] * cs.sb + inpage[j] + 4 * g);
-        dst[j][0] = u.x; dst[j][1] = u.y; dst[j][2] = u.z; dst[j][3] = u.w;
-      } else {
+        const int tile = ((base - win) >> 4) + j;
+        float f[4] = {1.0f, 1.0f, 1.0f, 1.0f};
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const int key = min(base + 16 * j + 4 * g + v, nk - 1);
-          dst[j][v] = sp[paged_page<false>(a, row, key, bad) * cs.sb + key % a.bs];
+          const uint8_t* p;
+          if constexpr (P16) {
+            p = vc + place(vat, tile) + voff[v];
+          } else {
+            const int key = min(base + 16 * j + 4 * g + v, nk - 1);
+            const int64_t pg = paged_page<false>(a, row, key, bad);
+            const int in = key % a.bs;
+            p = vc + pg * a.vcb + static_cast<int64_t>(in) * a.vcs + E * r16;
+            if (pa.vs.slot) f[v] = vss[pg * pa.vs.sb + in];
+          }
+          if constexpr (VW == 1) {
+            r.v[j][v][0] = *reinterpret_cast<const uint32_t*>(p);
+          } else if constexpr (VW == 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(p);
+            r.v[j][v][0] = x.x; r.v[j][v][1] = x.y;
+          } else {
+            const uint4 x = ld16(p);
+            r.v[j][v][0] = x.x; r.v[j][v][1] = x.y; r.v[j][v][2] = x.z; r.v[j][v][3] = x.w;
+          }
         }
+        if constexpr (P16 && PS)
+          r.vs[j] = *reinterpret_cast<const f32x4*>(vss + place(vsat, tile) + 4 * g);
+        else if constexpr (!P16)
+          r.vs[j] = f32x4{f[0], f[1], f[2], f[3]};
       }
-    }
-  };
-  auto load_k = [&](int base) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const uint8_t* p;
-      if constexpr (P16) {
-        p = kc + page[j] * a.kcb + static_cast<int64_t>(inpage[j]) * a.kcs;
-        p += static_cast<uint32_t>(r16 * static_cast<int>(a.kcs) + 16 * g);
-      } else {
-        const int key = min(base + 16 * j + r16, nk - 1);
-        const int64_t pg = paged_page<false>(a, row, key, bad);
-        p = kc + pg * a.kcb + static_cast<int64_t>(key % a.bs) * a.kcs + 16 * g;
-      }
-#pragma unroll
-      for (int s = 0; s < KP; ++s) kf[j][s] = ld16(p + 64 * s);
-    }
-    if (pa.ks.slot) load_scales(ksc, pa.ks, kss, base);
-  };
-  auto load_v = [&](int base) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const uint8_t* p;
-        if constexpr (P16) {
-          p = vc + page[j] * a.vcb + static_cast<int64_t>(inpage[j] + v) * a.vcs;
-          p += static_cast<uint32_t>(4 * g * static_cast<int>(a.vcs));
-        } else {
-          const int key = min(base + 16 * j + 4 * g + v, nk - 1);
-          const int64_t pg = paged_page<false>(a, row, key, bad);
-          p = vc + pg * a.vcb + static_cast<int64_t>(key % a.bs) * a.vcs;
-        }
-        p += E * r16;
-        if constexpr (VW == 1) {
-          vf[j][v][0] = *reinterpret_cast<const uint32_t*>(p);
-        } else if constexpr (VW == 2) {
-          const uint2 u = *reinterpret_cast<const uint2*>(p);
-          vf[j][v][0] = u.x; vf[j][v][1] = u.y;
-        } else {
-          const uint4 u = ld16(p);
-          vf[j][v][0] = u.x; vf[j][v][1] = u.y; vf[j][v][2] = u.z; vf[j][v][3] = u.w;
-        }
-      }
-    if (pa.vs.slot) load_scales(vsc, pa.vs, vss, base);
-  };
-
-  int base = k0 + 32 * w;
-  if (base < k1) {
-    lookup(base);
-    load_k(base);
-    load_v(base);
-  }
-  for (; base < k1; base += 128) {
-    const int next = base + 128;
-    const bool more = next < k1;
+    };
     f32x4 s[2];
+    auto scores = [&]() {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      s[j] = f32x4{};
+      for (int j = 0; j < 2; ++j) {
+        s[j] = f32x4{};
 #pragma unroll
-      for (int i = 0; i < KP; ++i) {
-        s[j] = mfma16(as_vec8<T>(widen8<T, F>(kf[j][i].x, kf[j][i].y)), qb[2 * i], s[j]);
-        s[j] = mfma16(as_vec8<T>(widen8<T, F>(kf[j][i].z, kf[j][i].w)), qb[2 * i + 1], s[j]);
+        for (int i = 0; i < KP; ++i) {
+          s[j] = mfma16(as_vec8<T>(widen8<T, F>(r.k[j][i].x, r.k[j][i].y)), qb[2 * i], s[j]);
+          s[j] = mfma16(as_vec8<T>(widen8<T, F>(r.k[j][i].z, r.k[j][i].w)), qb[2 * i + 1], s[j]);
+        }
+        if constexpr (kScaled) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) s[j][v] *= scale * r.ks[j][v];
+        } else {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) s[j][v] *= scale;
+        }
       }
-    }
+    };
+    auto softmax_pv = [&](int base) {
+      if (base + 31 > nk - nq) {  // some row's causal limit or the end lies in this round
+        asm volatile("");  // (a branch: as selects they would be in every round)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) s[j][v] *= scale * ksc[j][v];
-    // the next round's keys fly during this round's softmax and P.V
-    if (more) {
-      lookup(next);
-      load_k(next);
-    }
-    if (base + 31 > nk - nq) {  // some row's causal limit or the end lies in this round
+          for (int v = 0; v < 4; ++v) {
+            const int key = base + 16 * j + 4 * g + v;
+            if (key > lim) s[j][v] = -INFINITY;
+            if (key >= nk) {  // slots past the end may hold anything
+              if constexpr (kScaled) r.vs[j][v] = 0.0f;
+#pragma unroll
+              for (int q = 0; q < VW; ++q) r.v[j][v][q] = 0u;
+            }
+          }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) mx = fmaxf(mx, s[j][v]);
+      const float m_new = fmaxf(m_run, row4_max(mx));
+      if (__ballot(m_new > m_run) != 0) {
+        // rows with no visible key yet keep m = -inf: their factors are 0
+        const float ms = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m_run - ms);
+        m_run = m_new;
+        l_part *= alpha;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) acc[e][v] *= alpha;
+      }
+      const float ms = m_run == -INFINITY ? 0.0f : m_run;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const int key = base + 16 * j + 4 * g + v;
-          if (key > lim) s[j][v] = -INFINITY;
-          if (key >= nk) {  // slots past the end may hold anything
-            vsc[j][v] = 0.0f;
-#pragma unroll
-            for (int q = 0; q < VW; ++q) vf[j][v][q] = 0u;
-          }
+          s[j][v] = __builtin_amdgcn_exp2f(s[j][v] - ms);
+          l_part += s[j][v];
+          if constexpr (kScaled) s[j][v] *= r.vs[j][v];
         }
+      uint32_t pw[4][NP];  // [keys 2 i, 2 i + 1 of this lane][part]
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        bf16_parts<NP>(s[i >> 1][2 * (i & 1)], s[i >> 1][2 * (i & 1) + 1], pw[i]);
+      typename BF16::vec8 pb[NP];
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+        pb[p] = as_vec8<BF16>(make_uint4(pw[0][p], pw[1][p], pw[2][p], pw[3][p]));
+#pragma unroll
+      for (int q = 0; q < VW; ++q) {
+        uint32_t pr[4][2];  // bytes (a0 b0 a1 b1) and (a2 b2 a3 b3) of a pair of keys a, b
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t ka = r.v[i >> 1][2 * (i & 1)][q], kb = r.v[i >> 1][2 * (i & 1) + 1][q];
+          pr[i][0] = __builtin_amdgcn_perm(kb, ka, 0x05010400u);
+          pr[i][1] = __builtin_amdgcn_perm(kb, ka, 0x07030602u);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            x[i] = e & 1 ? widen2<BF16, F, true>(pr[i][e >> 1])
+                         : widen2<BF16, F, false>(pr[i][e >> 1]);
+          const auto va = as_vec8<BF16>(make_uint4(x[0], x[1], x[2], x[3]));
+#pragma unroll
+          for (int p = NP - 1; p >= 0; --p) acc[4 * q + e] = mfma16(va, pb[p], acc[4 * q + e]);
+        }
+      }
+    };
+
+    // A round's keys are loaded while the one before is used, its values after that: the
+    // last round, which loads nothing, stands apart, since with the loads under a branch
+    // the compiler waits for all of them at the next use. The steps are kept in order: as
+    // one block they were interleaved into more registers than a wave has.
+    int base = k0 + 32 * kw;
+    if (base < k1) {
+      if constexpr (P16) look(k0);
+      load_k(base);
+      load_v(base);
+      for (; base + RK < k1; base += RK) {
+        scores();
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(base + RK);
+        __builtin_amdgcn_sched_barrier(0);
+        softmax_pv(base);
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(base + RK);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      scores();
+      softmax_pv(base);
     }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) mx = fmaxf(mx, s[j][v]);
-    const float m_new = fmaxf(m_run, row4_max(mx));
-    if (__ballot(m_new > m_run) != 0) {
-      // rows with no visible key yet keep m = -inf: their factors are 0
-      const float ms = m_new == -INFINITY ? 0.0f : m_new;
-      const float alpha = __builtin_amdgcn_exp2f(m_run - ms);
-      m_run = m_new;
-      l_part *= alpha;
+
+    // O not finite: P.V again over the keys that each row sees (a masked key's infinite
+    // or NaN value times P = 0 is NaN, and so is an infinite one times the parts of P),
+    // with P and l 2^off times smaller (m larger), so that values near the largest do
+    // not overflow before the division by l
+    {
+      float nf = 0.0f;
 #pragma unroll
       for (int e = 0; e < E; ++e)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) acc[e][v] *= alpha;
-    }
-    const float ms = m_run == -INFINITY ? 0.0f : m_run;
+        for (int v = 0; v < 4; ++v) nf = fmaf(acc[e][v], 0.0f, nf);
+      if (__ballot(nf != 0.0f) != 0) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        s[j][v] = __builtin_amdgcn_exp2f(s[j][v] - ms);
-        l_part += s[j][v];
-        s[j][v] *= vsc[j][v];
-      }
-    uint32_t pw[4][NP];  // [keys 2 i, 2 i + 1 of this lane][part]
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      bf16_parts<NP>(s[i >> 1][2 * (i & 1)], s[i >> 1][2 * (i & 1) + 1], pw[i]);
-    typename BF16::vec8 pb[NP];
-#pragma unroll
-    for (int p = 0; p < NP; ++p)
-      pb[p] = as_vec8<BF16>(make_uint4(pw[0][p], pw[1][p], pw[2][p], pw[3][p]));
-#pragma unroll
-    for (int q = 0; q < VW; ++q) {
-      uint32_t pr[4][2];  // bytes (a0 b0 a1 b1) and (a2 b2 a3 b3) of a pair of keys a, b
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t ka = vf[i >> 1][2 * (i & 1)][q], kb = vf[i >> 1][2 * (i & 1) + 1][q];
-        pr[i][0] = __builtin_amdgcn_perm(kb, ka, 0x05010400u);
-        pr[i][1] = __builtin_amdgcn_perm(kb, ka, 0x07030602u);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t u[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          u[i] = e & 1 ? widen2<BF16, F, true>(pr[i][e >> 1])
-                       : widen2<BF16, F, false>(pr[i][e >> 1]);
-        const auto va = as_vec8<BF16>(make_uint4(u[0], u[1], u[2], u[3]));
-#pragma unroll
-        for (int p = NP - 1; p >= 0; --p) acc[4 * q + e] = mfma16(va, pb[p], acc[4 * q + e]);
-      }
-    }
-    if (more) load_v(next);
-  }
-
-  // O not finite: P.V again over the keys that each row sees (a masked key's infinite
-  // or NaN value times P = 0 is NaN, and so is an infinite one times the parts of P),
-  // with P and l 2^off times smaller (m larger), so that values near the largest do
-  // not overflow before the division by l
-  {
-    float nf = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) nf = fmaf(acc[e][v], 0.0f, nf);
-    if (__ballot(nf != 0.0f) != 0) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = f32x4{};
-      const float off = static_cast<float>(32 - __clz(k1 - k0));
-      m_run += off;
-      l_part *= __builtin_amdgcn_exp2f(-off);
-      const float ms = m_run == -INFINITY ? 0.0f : m_run;
-      int lane2 = static_cast<int>(threadIdx.x);  // (formed here, not kept across the loop)
-      asm volatile("" : "+v"(lane2));
-      const int g2 = (lane2 >> 4) & 3;
+        for (int e = 0; e < E; ++e) acc[e] = f32x4{};
+        const float off = static_cast<float>(32 - __clz(k1 - k0));
+        m_run += off;
+        l_part *= __builtin_amdgcn_exp2f(-off);
+        const float ms = m_run == -INFINITY ? 0.0f : m_run;
+        int lane2 = static_cast<int>(threadIdx.x);  // (formed here, not kept across the loop)
+        asm volatile("" : "+v"(lane2));
+        const int g2 = (lane2 >> 4) & 3;
 #pragma unroll 1
-      for (int i = 0; i < 32 * ((k1 - k0 + 127) / 128); ++i) {
-        const int key = k0 + 32 * w + 128 * (i >> 5) + (i & 31);
-        if (key >= k1) break;
-        const int64_t pg = paged_page<true>(a, row, key, bad);
-        const int in = key % a.bs;
-        const uint8_t* kp = kc + pg * a.kcb + static_cast<int64_t>(in) * a.kcs + 16 * g2;
-        const uint8_t* vp = vc + pg * a.vcb + static_cast<int64_t>(in) * a.vcs;
-        float d = 0.0f;  // the lane's dims of q . c_k
+        for (int i = 0; i < 32 * ((k1 - k0 + RK - 1) / RK); ++i) {
+          const int key = k0 + 32 * kw + RK * ((i >> 5)) + (i & 31);
+          if (key >= k1) break;
+          const int64_t pg = paged_page<true>(a, row, key, bad);
+          const int in = key % a.bs;
+          const uint8_t* kp = kc + pg * a.kcb + static_cast<int64_t>(in) * a.kcs + 16 * g2;
+          const uint8_t* vp = vc + pg * a.vcb + static_cast<int64_t>(in) * a.vcs;
+          float d = 0.0f;  // the lane's dims of q . c_k
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const uint2 u = *reinterpret_cast<const uint2*>(kp + 64 * (ks >> 1) + 8 * (ks & 1));
-          const uint4 qu = __builtin_bit_cast(uint4, qb[ks]);
-          const uint32_t qw[4] = {qu.x, qu.y, qu.z, qu.w};
-          const f32x2 kv[4] = {
-              Float8<F>::template to_f32<false>(u.x), Float8<F>::template to_f32<true>(u.x),
-              Float8<F>::template to_f32<false>(u.y), Float8<F>::template to_f32<true>(u.y)};
+          for (int ks = 0; ks < KS; ++ks) {
+            const uint2 x = *reinterpret_cast<const uint2*>(kp + 64 * (ks >> 1) + 8 * (ks & 1));
+            const uint4 qu = __builtin_bit_cast(uint4, qb[ks]);
+            const uint32_t qw[4] = {qu.x, qu.y, qu.z, qu.w};
+            const f32x2 kv[4] = {
+                Float8<F>::template to_f32<false>(x.x), Float8<F>::template to_f32<true>(x.x),
+                Float8<F>::template to_f32<false>(x.y), Float8<F>::template to_f32<true>(x.y)};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            d = fmaf(T::to_f32(static_cast<uint16_t>(qw[e])), kv[e][0], d);
-            d = fmaf(T::to_f32(static_cast<uint16_t>(qw[e] >> 16)), kv[e][1], d);
+            for (int e = 0; e < 4; ++e) {
+              d = fmaf(T::to_f32(static_cast<uint16_t>(qw[e])), kv[e][0], d);
+              d = fmaf(T::to_f32(static_cast<uint16_t>(qw[e] >> 16)), kv[e][1], d);
+            }
+          }
+          d = row4_sum(d) * (kScaled && pa.ks.slot ? scale * kss[pg * pa.ks.sb + in] : scale);
+          if (key > lim) continue;
+          float p = __builtin_amdgcn_exp2f(d - ms);
+          if (kScaled && pa.vs.slot) p *= vss[pg * pa.vs.sb + in];
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+#pragma unroll
+            for (int q = 0; q < VW; ++q) {
+              const uint32_t x = *reinterpret_cast<const uint32_t*>(vp + E * (4 * g2 + v) + 4 * q);
+              const f32x2 lo = Float8<F>::template to_f32<false>(x);
+              const f32x2 hi = Float8<F>::template to_f32<true>(x);
+              acc[4 * q][v] = fmaf(p, lo[0], acc[4 * q][v]);
+              acc[4 * q + 1][v] = fmaf(p, lo[1], acc[4 * q + 1][v]);
+              acc[4 * q + 2][v] = fmaf(p, hi[0], acc[4 * q + 2][v]);
+              acc[4 * q + 3][v] = fmaf(p, hi[1], acc[4 * q + 3][v]);
+            }
+        }
+      }
+    }
+
+    // acc[e][v] is dim E (4 g + v) + e of row r16
+    float l = row4_sum(l_part);
+    if (__ballot(bad) != 0) l = __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        *reinterpret_cast<float4*>(&sm[w][r16][E * (4 * g + v) + e]) =
+            make_float4(acc[e][v], acc[e + 1][v], acc[e + 2][v], acc[e + 3][v]);
+    if (g == 0) {
+      sml[w][r16][0] = m_run;
+      sml[w][r16][1] = l;
+    }
+    __syncthreads();
+    const int orow = t >> 4, od = E * (t & 15);
+    const int orr = tl * 16 + orow;
+    if (orr < nq * a.G) {
+#pragma unroll
+      for (int x = 0; x < HP; ++x) {
+        float M = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < NW; ++k) M = fmaxf(M, sml[x * NW + k][orow][0]);
+        float L = 0.0f, o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NW; ++k) {
+          const float mk = sml[x * NW + k][orow][0], lk = sml[x * NW + k][orow][1];
+          // (a quarter each: four finite sums add up to a finite one)
+          const float f = mk == -INFINITY ? 0.0f : 0.25f * __builtin_amdgcn_exp2f(mk - M);
+          // (a wave without keys has m = -inf and l = 0; NaN scores leave m = -inf
+          // with l = NaN, which the sum keeps)
+          L += mk == -INFINITY ? lk : f * lk;
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] += f * sm[x * NW + k][orow][od + e];
+        }
+        if (single) {
+          const int ho = hg * HP + x;
+          const int64_t tok = sq.q0 + orr / a.G;
+          const int hq = ho * a.G + orr % a.G;
+          uint16_t* op =
+              static_cast<uint16_t*>(a.o) + tok * a.ost + static_cast<int64_t>(hq) * a.ohs + od;
+          const float rcp = 1.0f / L, vs = fixed_scale(pa.vs, ho);
+          uint32_t pk[E / 2];
+#pragma unroll
+          for (int q = 0; q < E / 2; ++q) {
+            float lo = o[2 * q] * rcp * vs, hi = o[2 * q + 1] * rcp * vs;
+            if (nk == 0) lo = hi = sq.bad ? __uint_as_float(0x7fc00000u) : 0.0f;
+            pk[q] = pack2<T>(lo, hi);
+          }
+#pragma unroll
+          for (int q = 0; q < E / 2; q += 2)
+            *reinterpret_cast<uint2*>(op + 2 * q) = make_uint2(pk[q], pk[q + 1]);
+        } else {
+          const int64_t part =
+              ((2 * static_cast<int64_t>(blockIdx.x) + !first) * HP + x) * 16 + orow;
+          float* pp = a.part + part * D + od;
+#pragma unroll
+          for (int e = 0; e < E; e += 4)
+            *reinterpret_cast<float4*>(pp + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          if ((t & 15) == 0) {
+            a.ml[2 * part] = M;
+            a.ml[2 * part + 1] = L;
           }
         }
-        d = row4_sum(d) * (pa.ks.slot ? scale * kss[pg * pa.ks.sb + in] : scale);
-        if (key > lim) continue;
-        float p = __builtin_amdgcn_exp2f(d - ms);
-        if (pa.vs.slot) p *= vss[pg * pa.vs.sb + in];
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-#pragma unroll
-          for (int q = 0; q < VW; ++q) {
-            const uint32_t u = *reinterpret_cast<const uint32_t*>(vp + E * (4 * g2 + v) + 4 * q);
-            const f32x2 lo = Float8<F>::template to_f32<false>(u);
-            const f32x2 hi = Float8<F>::template to_f32<true>(u);
-            acc[4 * q][v] = fmaf(p, lo[0], acc[4 * q][v]);
-            acc[4 * q + 1][v] = fmaf(p, lo[1], acc[4 * q + 1][v]);
-            acc[4 * q + 2][v] = fmaf(p, hi[0], acc[4 * q + 2][v]);
-            acc[4 * q + 3][v] = fmaf(p, hi[1], acc[4 * q + 3][v]);
-          }
       }
     }
+    left -= take;
+    if (left <= 0) return;
+    u = 0;
+    if (++seg == tiles * pa.groups) {  // the next sequence with rows (there are units left)
+      seg = 0;
+      do sq = uniform_seq(paged_seq(a, ++b));
+      while (sq.nq == 0);
+      tiles = seq_tiles(a, sq);
+      units = seq_units(pa.unit, sq);
+    }
+    __syncthreads();  // (the merge buffer)
   }
+}
 
-  // acc[e][v] is dim E (4 g + v) + e of row r16
-  float l = row4_sum(l_part);
-  if (__ballot(bad) != 0) l = __uint_as_float(0x7fc00000u);
+// One head of a segment per workgroup of 16 waves: its rows' partials, weighted by
+// exp2(m - max m) and divided by their l. They are the first of workgroups w0 + 1 .. w1
+// and the first or last of w0. As many waves as there are share a row's partials.
+template <typename T, int D, int HP>
+__global__ __launch_bounds__(1024) void k_paged8_merge(Paged8Args pa) {
+  constexpr int XD = D / 64;  // dims per lane
+  typedef float vec __attribute__((ext_vector_type(XD)));
+  __shared__ float so[16][D], sl[16];
+  const PagedArgs& a = pa.a;
+  const Work work = find_work(pa, 0, blockIdx.x / HP);
+  if (work.b < 0) return;
+  const int tiles = seq_tiles(a, work.s), units = seq_units(pa.unit, work.s);
+  const int seg = static_cast<int>(blockIdx.x / HP) - work.segs, hh = blockIdx.x % HP;
+  const int x0 = work.units + seg * units;
+  const int w0 = __builtin_amdgcn_readfirstlane(x0 / work.share);
+  const int n = __builtin_amdgcn_readfirstlane((x0 + units - 1) / work.share) - w0 + 1;
+  if (n == 1) return;  // written by k_paged8
+  const int h = seg / tiles * HP + hh, tl = seg % tiles;
+  const int rows = min(work.s.nq * a.G - 16 * tl, 16);
+  const int lgr = rows > 1 ? 32 - __clz(rows - 1) : 0;  // rows as a power of two
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int row = w & ((1 << lgr) - 1), share = 16 >> lgr;
+  if (row < rows) {
+    const int first = 2 * w0 + (x0 != w0 * work.share);
+    const auto part = [&](int j) {
+      return static_cast<int64_t>(((j == 0 ? first : 2 * (w0 + j)) * HP + hh) * 16 + row);
+    };
+    float M = -INFINITY;
+    for (int j = lane; j < n; j += 64) M = fmaxf(M, a.ml[2 * part(j)]);
+    M = wave_max(M);
+    vec acc{};
+    float L = 0.0f;
+#pragma unroll 4
+    for (int j = w >> lgr; j < n; j += share) {
+      const int64_t p = part(j);
+      const vec x = *reinterpret_cast<const vec*>(a.part + p * D + XD * lane);
+      const float m = a.ml[2 * p], l = a.ml[2 * p + 1];
+      // (2^-10: the sum over the partials, at most 512, stays finite)
+      static_assert(kPaged8Groups <= 1024, "weights");
+      const float f = m == -INFINITY ? 0.0f : 0x1p-10f * __builtin_amdgcn_exp2f(m - M);
+      L += m == -INFINITY ? l : f * l;
 #pragma unroll
-  for (int v = 0; v < 4; ++v)
+      for (int q = 0; q < XD; ++q) acc[q] = fmaf(f, x[q], acc[q]);
+    }
 #pragma unroll
-    for (int e = 0; e < E; e += 4)
-      *reinterpret_cast<float4*>(&sm[w][r16][E * (4 * g + v) + e]) =
-          make_float4(acc[e][v], acc[e + 1][v], acc[e + 2][v], acc[e + 3][v]);
-  if (g == 0) {
-    sml[w][r16][0] = m_run;
-    sml[w][r16][1] = l;
+    for (int q = 0; q < XD; ++q) so[w][XD * lane + q] = acc[q];
+    if (lane == 0) sl[w] = L;
   }
   __syncthreads();
-  const int orow = t >> 4, od = E * (t & 15);
-  const int orr = tile.tl * 16 + orow;
-  if (orr >= nq * a.G) return;
-  const int64_t tok = sq.q0 + orr / a.G;
-  const int hq = h * a.G + orr % a.G;
-  float M = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) M = fmaxf(M, sml[k][orow][0]);
-  float L = 0.0f, o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.0f;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float mk = sml[k][orow][0];
-    // (a quarter each: four finite sums add up to a finite one)
-    const float f = mk == -INFINITY ? 0.0f : 0.25f * __builtin_amdgcn_exp2f(mk - M);
-    // (a wave without keys has m = -inf and l = 0; NaN scores leave m = -inf
-    // with l = NaN, which the sum keeps)
-    L += mk == -INFINITY ? sml[k][orow][1] : f * sml[k][orow][1];
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] += f * sm[k][orow][od + e];
-  }
-  if (single) {
-    uint16_t* op = static_cast<uint16_t*>(a.o) + tok * a.ost + static_cast<int64_t>(hq) * a.ohs + od;
-    const float rcp = 1.0f / L, vs = fixed_scale(pa.vs, h);
-    uint32_t pk[E / 2];
-#pragma unroll
-    for (int q = 0; q < E / 2; ++q) {
-      float lo = o[2 * q] * rcp * vs, hi = o[2 * q + 1] * rcp * vs;
-      if (nk == 0) lo = hi = sq.bad ? __uint_as_float(0x7fc00000u) : 0.0f;
-      pk[q] = pack2<T>(lo, hi);
+  const float vs = fixed_scale(pa.vs, h);
+  for (int i = t; i < rows * D; i += 1024) {
+    const int r = i / D, d = i % D;
+    float o = 0.0f, L = 0.0f;
+    for (int k = r; k < 16; k += 1 << lgr) {
+      o += so[k][d];
+      L += sl[k];
     }
-#pragma unroll
-    for (int q = 0; q < E / 2; q += 2)
-      *reinterpret_cast<uint2*>(op + 2 * q) = make_uint2(pk[q], pk[q + 1]);
-  } else {
-    const int64_t slot = (tok * a.Hq + hq) * a.nc + c;
-    float* pp = a.part + slot * D + od;
-#pragma unroll
-    for (int e = 0; e < E; e += 4)
-      *reinterpret_cast<float4*>(pp + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-    if ((t & 15) == 0) {
-      a.ml[2 * slot] = M;
-      a.ml[2 * slot + 1] = L;
-    }
+    const int rr = 16 * tl + r;
+    static_cast<uint16_t*>(a.o)[(work.s.q0 + rr / a.G) * a.ost +
+                                static_cast<int64_t>(h * a.G + rr % a.G) * a.ohs + d] =
+        T::from_f32(o / L * vs);
   }
 }
 
@@ -724,42 +965,51 @@ __global__ __launch_bounds__(256, 2) void k_paged8_rows(Paged8Args pa) {
 }
 
 template <typename T, int F, int D>
-hipError_t launch_paged8_t(const Paged8Args& p, bool rows, int64_t tiles, hipStream_t s) {
-  const PagedArgs& a = p.a;
-  const dim3 grid(static_cast<unsigned>(tiles * a.Hkv), static_cast<unsigned>(a.nc));
-  const bool p16 = a.bs % 16 == 0;
-  if constexpr (D <= 128) {
-    if (rows) {
-      if (p16) hipLaunchKernelGGL((k_paged8_rows<T, F, D, true>), grid, dim3(256), 0, s, p);
-      else hipLaunchKernelGGL((k_paged8_rows<T, F, D, false>), grid, dim3(256), 0, s, p);
-      return hipGetLastError();
-    }
-  }
-  if (p16) hipLaunchKernelGGL((k_paged8<T, F, D, true>), grid, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((k_paged8<T, F, D, false>), grid, dim3(256), 0, s, p);
+hipError_t launch_rows_t(const Paged8Args& p, int64_t tiles, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(tiles * p.a.Hkv), static_cast<unsigned>(p.a.nc)), b(256);
+  if (p.a.bs % 16 == 0) hipLaunchKernelGGL((k_paged8_rows<T, F, D, true>), grid, b, 0, s, p);
+  else hipLaunchKernelGGL((k_paged8_rows<T, F, D, false>), grid, b, 0, s, p);
   return hipGetLastError();
 }
 
-template <typename T, int F>
-hipError_t launch_paged8_d(const Paged8Args& p, int head_dim, bool rows, int64_t tiles,
-                           hipStream_t s) {
-  return with_head_dim(head_dim, [&](auto dc) {
-    return launch_paged8_t<T, F, decltype(dc)::value>(p, rows, tiles, s);
-  });
+template <typename T, int F, int D, int HP>
+hipError_t launch_few_t(const Paged8Args& p, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(p.a.nc)), b(256);
+  if (p.a.bs % 16 != 0 || p.ks.slot != p.vs.slot)
+    hipLaunchKernelGGL((k_paged8<T, F, D, false, false, HP>), grid, b, 0, s, p);
+  else if (p.ks.slot)
+    hipLaunchKernelGGL((k_paged8<T, F, D, true, true, HP>), grid, b, 0, s, p);
+  else
+    hipLaunchKernelGGL((k_paged8<T, F, D, true, false, HP>), grid, b, 0, s, p);
+  if (p.a.part != nullptr)
+    hipLaunchKernelGGL((k_paged8_merge<T, D, HP>), dim3(static_cast<unsigned>(p.segs * HP)),
+                       dim3(1024), 0, s, p);
+  return hipGetLastError();
 }
 
 hipError_t launch_paged8(const Paged8Args& p, int dtype, int format, int head_dim, bool rows,
                          int64_t tiles, hipStream_t s) {
-  const bool bf = dtype == FP_DTYPE_BF16;
-  hipError_t e;
-  if (format == FP_CACHE_E4M3)
-    e = bf ? launch_paged8_d<BF16, FP_CACHE_E4M3>(p, head_dim, rows, tiles, s)
-           : launch_paged8_d<F16, FP_CACHE_E4M3>(p, head_dim, rows, tiles, s);
-  else
-    e = bf ? launch_paged8_d<BF16, FP_CACHE_E5M2>(p, head_dim, rows, tiles, s)
-           : launch_paged8_d<F16, FP_CACHE_E5M2>(p, head_dim, rows, tiles, s);
-  if (e != hipSuccess || p.a.nc <= 1) return e;
-  return launch_paged_merge(p.a, dtype, head_dim, rows, s);
+  const auto run = [&](auto t, auto f) -> hipError_t {
+    using T = decltype(t);
+    constexpr int F = decltype(f)::value;
+    if (!rows)
+      return with_head_dim(head_dim, [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        if constexpr (D == 64) {
+          if (p.groups < p.a.Hkv) return launch_few_t<T, F, D, 2>(p, s);
+        }
+        return launch_few_t<T, F, D, 1>(p, s);
+      });
+    const hipError_t e = head_dim == 128 ? launch_rows_t<T, F, 128>(p, tiles, s)
+                                         : launch_rows_t<T, F, 64>(p, tiles, s);
+    if (e != hipSuccess || p.a.nc <= 1) return e;
+    return launch_paged_merge_rows(p.a, dtype, head_dim, s);
+  };
+  if (dtype == FP_DTYPE_BF16)
+    return format == FP_CACHE_E4M3 ? run(BF16{}, IntC<FP_CACHE_E4M3>{})
+                                   : run(BF16{}, IntC<FP_CACHE_E5M2>{});
+  return format == FP_CACHE_E4M3 ? run(F16{}, IntC<FP_CACHE_E4M3>{})
+                                 : run(F16{}, IntC<FP_CACHE_E5M2>{});
 }
 
 }  // namespace fp

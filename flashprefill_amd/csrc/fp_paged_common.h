@@ -14,9 +14,14 @@ __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// entry x of a 32- or 64-bit integer array
+// entry x of a 32- or 64-bit (is64 1) integer array. Loads under no branch: several of
+// them are in flight together, where a branch makes the compiler wait for each.
 __device__ __forceinline__ int64_t ld_int(const void* p, int is64, int64_t x) {
-  return is64 ? static_cast<const int64_t*>(p)[x] : static_cast<const int32_t*>(p)[x];
+  const int32_t* q = static_cast<const int32_t*>(p) + (x << is64);
+  const int32_t lo = q[0], hi = q[is64];
+  return is64 ? static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 |
+                                     static_cast<uint32_t>(lo))
+              : static_cast<int64_t>(lo);
 }
 
 // One sequence as the workgroups see it. `bad`: more tokens than the block

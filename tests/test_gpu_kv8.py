@@ -175,6 +175,16 @@ def test_many_rows_at_tile_edges(page, d, dtype, fmt, mode):
                1 / math.sqrt(d))
 
 
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("d,news", [(64, 1), (128, 1), (256, 3), (128, 40)])
+@pytest.mark.parametrize("slot", ["key", "value"])
+def test_scales_of_two_kinds(page, d, news, slot):
+    """K's scales per slot beside one of V, and the other way round."""
+    args = attention_case([700, 33, 260], [news] * 3, 8, 2, d, page, BF, E4M3, "slot", seed=2)
+    args[7 if slot == "key" else 6] = torch.tensor([0.02])
+    _check(args, 0.1)
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("news", [1, 40])
 @pytest.mark.parametrize("scale", [0.5, -0.3, 1e-3])
