@@ -643,17 +643,19 @@ __global__ __launch_bounds__(1024) void k_paged8_merge(Paged8Args pa) {
 // each product, an eighth of what rounding the output to fp16 may lose and a 256th
 // of its cached value's own step, where a third part would add half as many MFMAs
 // to P.V again.
-template <typename T, int F, int D, bool P16>
+template <typename T, int F, int D, bool P16, bool PS>
 __global__ __launch_bounds__(256, 2) void k_paged8_rows(Paged8Args pa) {
   constexpr int KT = 64, TT = KT / 32;
   constexpr int KS = D / 16, DT = D / 32, CH = D / 8;
   constexpr int LPR = D / 16;        // lanes per key (16 bytes each)
   constexpr int NL = 16 * LPR / 64;  // load instructions per wave and tile
   constexpr int NP = 2;
+  constexpr float kStep = 8.0f;
+  constexpr bool kScaled = PS || !P16;
   __shared__ uint4 sk[2][KT * CH];
   __shared__ uint4 sv[2][KT * CH];
-  __shared__ float ssk[2][KT];  // scale * log2 e * s_k, and s_v (one per slot) or 1
-  __shared__ float ssv[2][KT];
+  __shared__ float ssk[kScaled ? 2 : 1][KT];  // scale * log2 e * s_k, and s_v
+  __shared__ float ssv[kScaled ? 2 : 1][KT];
   __shared__ int s_bad;  // some wave looked up a page outside the cache
   const PagedArgs& a = pa.a;
   const int h = static_cast<int>(blockIdx.x % a.Hkv);
@@ -688,12 +690,23 @@ __global__ __launch_bounds__(256, 2) void k_paged8_rows(Paged8Args pa) {
   const int k1 = __builtin_amdgcn_readfirstlane(
       min(min(k0 + tile.chunk, nk), max(nk - nq + last_row / a.G + 1, 0)));
 
+  // (fixed scales: one factor, its sign in q, so that the largest score is that of the
+  // largest product)
+  const float signed_scale = a.scale_log2 * fixed_scale(pa.ks, h);
+  // (not 0, by which a masked score would be NaN)
+  const float scale = kScaled ? signed_scale
+                              : signed_scale == 0.0f ? 0x1p-126f : fabsf(signed_scale);
+  const uint32_t flip = !kScaled && signed_scale < 0.0f ? 0x80008000u : 0u;
   typename T::vec8 qb[KS];
   {
     const uint16_t* qp = static_cast<const uint16_t*>(a.q) + tok * a.qst +
                          static_cast<int64_t>(hq) * a.qhs + 8 * half;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qb[s] = as_vec8<T>(rvalid ? ld16(qp + 16 * s) : zero4());
+    for (int s = 0; s < KS; ++s) {
+      const uint4 x = ld16(qp + 16 * s);
+      qb[s] = as_vec8<T>(rvalid ? make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip)
+                                : zero4());
+    }
   }
   f32x16 o[DT];
 #pragma unroll
@@ -706,11 +719,13 @@ __global__ __launch_bounds__(256, 2) void k_paged8_rows(Paged8Args pa) {
   const uint8_t* vc = static_cast<const uint8_t*>(a.vc) + static_cast<int64_t>(h) * a.vch;
   const float* kss = pa.ks.p + h * pa.ks.sh;  // read when there is one per slot
   const float* vss = pa.vs.p + h * pa.vs.sh;
-  const float scale = a.scale_log2 * fixed_scale(pa.ks, h);
 
-  // 16 bytes per lane of the wave's 16 keys, and lane 4 i's (P16: lane i's) scales
+  // the lane's row of a load (d = 128: in an order in which the eight lanes of a row and
+  // the next eight write to banks of their own, rows 0 4 1 5 2 6 3 7)
+  const int lrow = D == 128 ? 4 * ((lane >> 3) & 1) + (lane >> 4) : lane / LPR;
+  // 16 bytes per lane of the wave's 16 keys, and lane i's scales (every 16 lanes)
   uint4 kr[NL], vr[NL];
-  float kscr = scale, vscr = 1.0f;
+  float kscr = 1.0f, vscr = 1.0f;
   const int last16 = (nk - 1) & ~15;
   // tile of keys base .. base + 63; keys past the sequence read its last 16-key
   // group (P16) or its last key
@@ -723,16 +738,18 @@ __global__ __launch_bounds__(256, 2) void k_paged8_rows(Paged8Args pa) {
       const uint8_t* vp = vc + pg * a.vcb + static_cast<int64_t>(in) * a.vcs;
 #pragma unroll
       for (int q = 0; q < NL; ++q) {
-        const int r = q * (64 / LPR) + lane / LPR;
+        const int r = q * (64 / LPR) + lrow;
         kr[q] = ld16(kp + static_cast<uint32_t>(r * static_cast<int>(a.kcs) + 16 * (lane % LPR)));
         vr[q] = ld16(vp + static_cast<uint32_t>(r * static_cast<int>(a.vcs) + 16 * (lane % LPR)));
       }
-      if (pa.ks.slot) kscr = scale * kss[pg * pa.ks.sb + in + (lane & 15)];
-      if (pa.vs.slot) vscr = vss[pg * pa.vs.sb + in + (lane & 15)];
+      if constexpr (PS) {
+        kscr = kss[pg * pa.ks.sb + in + (lane & 15)];
+        vscr = vss[pg * pa.vs.sb + in + (lane & 15)];
+      }
     } else {
 #pragma unroll
       for (int q = 0; q < NL; ++q) {
-        const int key = min(base + 16 * w + q * (64 / LPR) + lane / LPR, nk - 1);
+        const int key = min(base + 16 * w + q * (64 / LPR) + lrow, nk - 1);
         const int64_t pg = paged_page<false>(a, row, key, bad);
         const int64_t in = key % a.bs;
         kr[q] = ld16(kc + pg * a.kcb + in * a.kcs + 16 * (lane % LPR));
@@ -741,7 +758,7 @@ __global__ __launch_bounds__(256, 2) void k_paged8_rows(Paged8Args pa) {
       if (pa.ks.slot || pa.vs.slot) {
         const int key = min(base + 16 * w + (lane & 15), nk - 1);
         const int64_t pg = paged_page<false>(a, row, key, bad);
-        if (pa.ks.slot) kscr = scale * kss[pg * pa.ks.sb + key % a.bs];
+        if (pa.ks.slot) kscr = kss[pg * pa.ks.sb + key % a.bs];
         if (pa.vs.slot) vscr = vss[pg * pa.vs.sb + key % a.bs];
       }
     }
@@ -751,15 +768,16 @@ __global__ __launch_bounds__(256, 2) void k_paged8_rows(Paged8Args pa) {
   auto store = [&](int base, int buf) {
 #pragma unroll
     for (int q = 0; q < NL; ++q) {
-      const int r = 16 * w + q * (64 / LPR) + lane / LPR, ch = 2 * (lane % LPR);
+      const int r = 16 * w + q * (64 / LPR) + lrow;
+      const int c0 = r * CH + ((2 * (lane % LPR)) ^ swz<D>(r));
       const uint4 u = kr[q], v = base + r < nk ? vr[q] : zero4();
-      sk[buf][r * CH + (ch ^ swz<D>(r))] = widen8<T, F>(u.x, u.y);
-      sk[buf][r * CH + ((ch + 1) ^ swz<D>(r))] = widen8<T, F>(u.z, u.w);
-      sv[buf][r * CH + (ch ^ swz<D>(r))] = widen8<BF16, F>(v.x, v.y);
-      sv[buf][r * CH + ((ch + 1) ^ swz<D>(r))] = widen8<BF16, F>(v.z, v.w);
+      sk[buf][c0] = widen8<T, F>(u.x, u.y);
+      sk[buf][c0 ^ 1] = widen8<T, F>(u.z, u.w);
+      sv[buf][c0] = widen8<BF16, F>(v.x, v.y);
+      sv[buf][c0 ^ 1] = widen8<BF16, F>(v.z, v.w);
     }
-    if (lane < 16) {
-      ssk[buf][16 * w + lane] = kscr;
+    if (kScaled && lane < 16) {
+      ssk[buf][16 * w + lane] = scale * kscr;
       ssv[buf][16 * w + lane] = base + 16 * w + lane < nk ? vscr : 0.0f;
     }
   };
@@ -782,33 +800,45 @@ __global__ __launch_bounds__(256, 2) void k_paged8_rows(Paged8Args pa) {
     if (base <= lim_hi) {  // (else no key of this tile is visible to the wave)
       f32x16 s[TT];
 #pragma unroll
-      for (int t4 = 0; t4 < TT; ++t4) s[t4] = f32x16{};
-#pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int t4 = 0; t4 < TT; ++t4) {
           const int r = 32 * t4 + l32;
           const uint4 kop = sk[buf][r * CH + ((2 * ks + half) ^ swz<D>(r))];
-          s[t4] = T::mfma32(as_vec8<T>(kop), qb[ks], s[t4]);
+          s[t4] = T::mfma32(as_vec8<T>(kop), qb[ks], ks == 0 ? f32x16{} : s[t4]);
         }
-      const bool edge = base + KT - 1 > lim_lo;
+      if constexpr (kScaled) {
+#pragma unroll
+        for (int t4 = 0; t4 < TT; ++t4)
+#pragma unroll
+          for (int g4 = 0; g4 < 4; ++g4) {
+            const float4 f =
+                *reinterpret_cast<const float4*>(&ssk[buf][32 * t4 + 8 * g4 + 4 * half]);
+            s[t4][4 * g4] *= f.x;
+            s[t4][4 * g4 + 1] *= f.y;
+            s[t4][4 * g4 + 2] *= f.z;
+            s[t4][4 * g4 + 3] *= f.w;
+          }
+      }
+      if (base + KT - 1 > lim_lo) {
+        asm volatile("");  // (a branch: as selects they would be in every tile)
+#pragma unroll
+        for (int t4 = 0; t4 < TT; ++t4)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            if (base + 32 * t4 + 8 * (v >> 2) + 4 * half + (v & 3) > lim) s[t4][v] = -INFINITY;
+      }
       float mx = -INFINITY;
 #pragma unroll
       for (int t4 = 0; t4 < TT; ++t4)
 #pragma unroll
-        for (int g4 = 0; g4 < 4; ++g4) {
-          const float4 f = *reinterpret_cast<const float4*>(&ssk[buf][32 * t4 + 8 * g4 + 4 * half]);
-          const float fe[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float y = s[t4][4 * g4 + e] * fe[e];
-            if (edge && base + 32 * t4 + 8 * g4 + 4 * half + e > lim) y = -INFINITY;
-            s[t4][4 * g4 + e] = y;
-            mx = fmaxf(mx, y);
-          }
-        }
-      const float m_new = fmaxf(m_run, pair32_max(mx));
-      if (__ballot(m_new > m_run) != 0) {
+        for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[t4][v]);
+      mx = pair32_max(mx);
+      if constexpr (!kScaled) mx *= scale;
+      // m moves only where it must, so that P stays below 2^kStep: not in every tile that
+      // has a new largest score for one of the wave's rows
+      if (__ballot(mx > m_run + kStep) != 0) {
+        const float m_new = fmaxf(m_run, mx);
         const float ms = m_new == -INFINITY ? 0.0f : m_new;
         const float alpha = __builtin_amdgcn_exp2f(m_run - ms);
         m_run = m_new;
@@ -824,10 +854,11 @@ __global__ __launch_bounds__(256, 2) void k_paged8_rows(Paged8Args pa) {
       for (int t4 = 0; t4 < TT; ++t4) {
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          s[t4][v] = __builtin_amdgcn_exp2f(s[t4][v] - ms);
+          const float x = kScaled ? s[t4][v] - ms : fmaf(s[t4][v], scale, -ms);
+          s[t4][v] = __builtin_amdgcn_exp2f(x);
           l_part += s[t4][v];
         }
-        if (pa.vs.slot) {
+        if constexpr (kScaled) {
 #pragma unroll
           for (int g4 = 0; g4 < 4; ++g4) {
             const float4 f =
@@ -850,12 +881,15 @@ __global__ __launch_bounds__(256, 2) void k_paged8_rows(Paged8Args pa) {
             pb[p] = as_vec8<BF16>(make_uint4(u[0][p], u[1][p], u[2][p], u[3][p]));
           const uint16_t* sv16 = reinterpret_cast<const uint16_t*>(sv[buf]);
           const int r = 32 * t4 + 16 * hh + tr_row;
+          __builtin_amdgcn_sched_barrier(0);
+          typename BF16::vec8 va[DT];
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            const auto va = read_vt<BF16, D>(sv16, r, 32 * dt + tr_col);
+          for (int dt = 0; dt < DT; ++dt) va[dt] = read_vt<BF16, D>(sv16, r, 32 * dt + tr_col);
+          // (a dim tile's two products apart: the second would wait for the first)
 #pragma unroll
-            for (int p = NP - 1; p >= 0; --p) o[dt] = BF16::mfma32(va, pb[p], o[dt]);
-          }
+          for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[dt] = BF16::mfma32(va[dt], pb[p], o[dt]);
         }
       }
     }
@@ -904,7 +938,7 @@ __global__ __launch_bounds__(256, 2) void k_paged8_rows(Paged8Args pa) {
           d = fmaf(T::to_f32(static_cast<uint16_t>(qw[e] >> 16)), kv[e][1], d);
         }
       }
-      d = pair32_sum(d) * (pa.ks.slot ? scale * kss[pg * pa.ks.sb + in] : scale);
+      d = pair32_sum(d) * (kScaled && pa.ks.slot ? scale * kss[pg * pa.ks.sb + in] : scale);
       if (key > lim) continue;
       float p = __builtin_amdgcn_exp2f(d - ms);
       if (pa.vs.slot) p *= vss[pg * pa.vs.sb + in];
@@ -967,8 +1001,12 @@ __global__ __launch_bounds__(256, 2) void k_paged8_rows(Paged8Args pa) {
 template <typename T, int F, int D>
 hipError_t launch_rows_t(const Paged8Args& p, int64_t tiles, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(tiles * p.a.Hkv), static_cast<unsigned>(p.a.nc)), b(256);
-  if (p.a.bs % 16 == 0) hipLaunchKernelGGL((k_paged8_rows<T, F, D, true>), grid, b, 0, s, p);
-  else hipLaunchKernelGGL((k_paged8_rows<T, F, D, false>), grid, b, 0, s, p);
+  if (p.a.bs % 16 != 0 || p.ks.slot != p.vs.slot)
+    hipLaunchKernelGGL((k_paged8_rows<T, F, D, false, false>), grid, b, 0, s, p);
+  else if (p.ks.slot)
+    hipLaunchKernelGGL((k_paged8_rows<T, F, D, true, true>), grid, b, 0, s, p);
+  else
+    hipLaunchKernelGGL((k_paged8_rows<T, F, D, true, false>), grid, b, 0, s, p);
   return hipGetLastError();
 }
 

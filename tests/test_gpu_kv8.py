@@ -187,7 +187,7 @@ def test_scales_of_two_kinds(page, d, news, slot):
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("news", [1, 40])
-@pytest.mark.parametrize("scale", [0.5, -0.3, 1e-3])
+@pytest.mark.parametrize("scale", [0.5, -0.3, 1e-3, 0.0])
 @pytest.mark.parametrize("mode", ["head", "slot"])
 def test_peaked_and_flat_rows(dtype, news, scale, mode):
     args = attention_case([3000, 700], [news, news], 8, 2, 128, 16, dtype, E4M3, mode, seed=9)
