@@ -73,6 +73,8 @@ _FP8_NAMES = {"fp8": torch.float8_e4m3fn, "fp8_e4m3": torch.float8_e4m3fn,
 def _check_scales(cache: torch.Tensor, k_scale, v_scale) -> None:
     """Refuse scales that are not of one of the forms that ``reshape_and_cache``
     describes, or that come with a 16-bit cache."""
+    if k_scale is None and v_scale is None:
+        return
     nb, bs, hkv = cache.shape[:3]
     for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
         if s is None:
@@ -94,16 +96,22 @@ def _check_scales(cache: torch.Tensor, k_scale, v_scale) -> None:
 
 def _scale_args(scale: Optional[torch.Tensor], device) -> tuple:
     """``fp_kv_scales`` of a checked scale, and the tensor whose memory it names."""
-    out = _lib.FpKvScales()
     if scale is None:
-        return out, None
+        return _lib.FpKvScales(), None
     if scale.dim() == 3:
-        out.data, out.per_slot = scale.data_ptr(), 1
-        out.stride_block, out.stride_head = scale.stride(0), scale.stride(1)
-        return out, scale
-    scale = scale.to(device).view(-1).contiguous()
-    out.data, out.stride_head = scale.data_ptr(), int(scale.numel() > 1)
-    return out, scale
+        return _lib.FpKvScales(scale.data_ptr(), scale.stride(0), scale.stride(1), 1), scale
+    if scale.device != device or not scale.is_contiguous():
+        scale = scale.to(device).contiguous()
+    return _lib.FpKvScales(scale.data_ptr(), 0, 1 if scale.numel() > 1 else 0, 0), scale
+
+
+def _launch(device: torch.device, fn, *args) -> None:
+    """``fn(*args, stream)`` with ``device`` current, on torch's current stream there."""
+    if torch.cuda.current_device() == device.index:
+        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))
+        return
+    with torch.cuda.device(device):
+        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))
 
 
 def _check_rows(key, value, key_cache, value_cache, what: str) -> None:
@@ -131,24 +139,19 @@ def _check_written(*tensors) -> None:
     """Refuse what torch's own in-place operations refuse: several elements in one
     place, and inference tensors outside inference mode."""
     for t in tensors:
-        if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+        if 0 in t.stride() and any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
             raise RuntimeError("a tensor to be written has several elements in one memory "
                                "location: clone() it first")
         if t.is_inference() and not torch.is_inference_mode_enabled():
             raise RuntimeError("an inference tensor cannot be written outside inference mode")
 
 
-def _cache_args(a, key, value, key_cache, value_cache, n: int) -> None:
+def _cache_args(key, value, key_cache, value_cache, slots: int, n: int) -> _lib.FpKvCacheArgs:
     nb, bs, hkv, d = key_cache.shape
-    a.key, a.value = key.data_ptr(), value.data_ptr()
-    a.k_stride_tok, a.k_stride_head = key.stride(0), key.stride(1)
-    a.v_stride_tok, a.v_stride_head = value.stride(0), value.stride(1)
-    a.key_cache, a.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
-    a.kc_stride_block, a.kc_stride_slot, a.kc_stride_head = key_cache.stride()[:3]
-    a.vc_stride_block, a.vc_stride_slot, a.vc_stride_head = value_cache.stride()[:3]
-    a.num_tokens, a.num_blocks = n, nb
-    a.block_size, a.num_kv_heads, a.head_dim = bs, hkv, d
-    a.dtype = _DTYPES[key.dtype]
+    return _lib.FpKvCacheArgs(key.data_ptr(), value.data_ptr(), *key.stride()[:2],
+                              *value.stride()[:2], key_cache.data_ptr(), value_cache.data_ptr(),
+                              *key_cache.stride()[:3], *value_cache.stride()[:3], slots, n, nb,
+                              bs, hkv, d, _DTYPES[key.dtype])
 
 
 def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
@@ -183,26 +186,16 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.T
             raise ValueError("key, value and the caches must be on one GPU")
     slots = slot_mapping.to(device=dev, dtype=torch.int64).contiguous()
     lib = _lib.load()
+    base = _cache_args(key, value, key_cache, value_cache, slots.data_ptr(), n)
     if key_cache.dtype not in _FORMATS:
-        a = _lib.FpKvCacheArgs()
-        _cache_args(a, key, value, key_cache, value_cache, n)
-        a.slot_mapping = slots.data_ptr()
-        with torch.cuda.device(dev):
-            _lib.check(lib.fp_kv_cache_write(ctypes.byref(a),
-                                             torch.cuda.current_stream(dev).cuda_stream))
+        _launch(dev, lib.fp_kv_cache_write, ctypes.byref(base))
         return
     written = [key_cache, value_cache]
     written += [s for s in (k_scale, v_scale) if s is not None and s.dim() == 3]
     _check_written(*written)
-    a = _lib.FpKvCacheFp8Args()
-    _cache_args(a.base, key, value, key_cache, value_cache, n)
-    a.base.slot_mapping = slots.data_ptr()
-    a.format = _FORMATS[key_cache.dtype]
-    a.k_scale, k_keep = _scale_args(k_scale, dev)
-    a.v_scale, v_keep = _scale_args(v_scale, dev)
-    with torch.cuda.device(dev):
-        _lib.check(lib.fp_kv_cache_write_fp8(ctypes.byref(a),
-                                             torch.cuda.current_stream(dev).cuda_stream))
+    (ks, k_keep), (vs, v_keep) = _scale_args(k_scale, dev), _scale_args(v_scale, dev)
+    _launch(dev, lib.fp_kv_cache_write_fp8,
+            ctypes.byref(_lib.FpKvCacheFp8Args(base, ks, vs, _FORMATS[key_cache.dtype])))
     torch.autograd.graph.increment_version(written)
 
 
@@ -249,20 +242,16 @@ def gather_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.
     cu, table = cu_seqlens.to(dev).contiguous(), block_table.to(dev)
     if table.stride(1) != 1:
         table = table.contiguous()
-    a = _lib.FpKvGatherArgs()
-    _cache_args(a.base, key, value, key_cache, value_cache, key.shape[0])
-    a.format = _FORMATS.get(key_cache.dtype, _lib.FP_CACHE_16BIT)
-    a.k_scale, k_keep = _scale_args(k_scale, dev)
-    a.v_scale, v_keep = _scale_args(v_scale, dev)
-    a.batch, a.table_width, a.table_stride = B, table.shape[1], table.stride(0)
-    a.cu_seqlens, a.block_table = cu.data_ptr(), table.data_ptr()
-    a.cu_is64, a.table_is64 = cu.dtype == torch.int64, table.dtype == torch.int64
     if starts is not None:
         starts = starts.to(dev).contiguous()
-        a.starts, a.starts_is64 = starts.data_ptr(), starts.dtype == torch.int64
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().fp_kv_cache_gather(ctypes.byref(a),
-                                                  torch.cuda.current_stream(dev).cuda_stream))
+    (ks, k_keep), (vs, v_keep) = _scale_args(k_scale, dev), _scale_args(v_scale, dev)
+    a = _lib.FpKvGatherArgs(
+        _cache_args(key, value, key_cache, value_cache, 0, key.shape[0]), ks, vs,
+        _FORMATS.get(key_cache.dtype, _lib.FP_CACHE_16BIT), B, table.shape[1],
+        cu.dtype == torch.int64, table.dtype == torch.int64,
+        starts is not None and starts.dtype == torch.int64, cu.data_ptr(), table.data_ptr(),
+        None if starts is None else starts.data_ptr(), table.stride(0))
+    _launch(dev, _lib.load().fp_kv_cache_gather, ctypes.byref(a))
     torch.autograd.graph.increment_version([key, value])
 
 
@@ -307,8 +296,13 @@ _INDEX = (torch.int32, torch.int64)
 
 def _rows_ok(t: torch.Tensor) -> bool:
     step = 16 // t.element_size()
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and all(s % step == 0 and s >= 0 for s in t.stride()[:-1]))
+    *rest, last = t.stride()
+    if last != 1 or t.data_ptr() % 16:
+        return False
+    for s in rest:
+        if s % step or s < 0:
+            return False
+    return True
 
 
 def _paged_kernel_takes(query, key_cache, value_cache, out, cu, used, table, k_scale=None,
@@ -344,7 +338,7 @@ def _paged_kernel_takes(query, key_cache, value_cache, out, cu, used, table, k_s
                 bs % 16 == 0 and (s.data_ptr() % 16 or s.stride(0) % 4 or s.stride(1) % 4)):
             return False
     # torch refuses to write these, and so does the composition
-    if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())) or \
+    if (0 in out.stride() and any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride()))) or \
             (out.is_inference() and not torch.is_inference_mode_enabled()):
         return False
     if key_cache.stride(1) >= 1 << 24 or value_cache.stride(1) >= 1 << 24:
@@ -363,9 +357,12 @@ def _paged_kernel_takes(query, key_cache, value_cache, out, cu, used, table, k_s
             return False
     if not used.is_cuda and any(n > table.shape[1] * bs for n in used[:B].tolist()):
         return False
-    return not (torch.is_grad_enabled() and any(t.requires_grad for t in
-                                                (query, key_cache, value_cache, out, k_scale,
-                                                 v_scale) if t is not None))
+    if not torch.is_grad_enabled():
+        return True
+    for t in (query, key_cache, value_cache, out, k_scale, v_scale):
+        if t is not None and t.requires_grad:
+            return False
+    return True
 
 
 def _paged_attention_kernel(query, key_cache, value_cache, out, cu, used, table, scale,
@@ -378,38 +375,24 @@ def _paged_attention_kernel(query, key_cache, value_cache, out, cu, used, table,
     if table.stride(1) != 1:
         table = table.contiguous()
     lib = _lib.load()
-    fp8 = key_cache.dtype in _FORMATS
-    if fp8:
-        call = _lib.FpPagedFp8Args()
-        a = call.base
-        call.format = _FORMATS[key_cache.dtype]
-        call.k_scale, k_keep = _scale_args(k_scale, dev)
-        call.v_scale, v_keep = _scale_args(v_scale, dev)
+    call = _lib.FpPagedArgs(
+        query.data_ptr(), *query.stride()[:2], out.data_ptr(), *out.stride()[:2],
+        key_cache.data_ptr(), value_cache.data_ptr(), *key_cache.stride()[:3],
+        *value_cache.stride()[:3], cu.data_ptr(), used.data_ptr(), table.data_ptr(),
+        table.stride(0), T, nb, cu.numel() - 1, table.shape[1], bs, hq, hkv, d,
+        _DTYPES[query.dtype], cu.dtype == torch.int64, used.dtype == torch.int64,
+        table.dtype == torch.int64, float(scale))
+    ws_bytes, launch = lib.fp_paged_workspace_bytes, lib.fp_paged_attention
+    if key_cache.dtype in _FORMATS:
+        (ks, k_keep), (vs, v_keep) = _scale_args(k_scale, dev), _scale_args(v_scale, dev)
+        call = _lib.FpPagedFp8Args(call, ks, vs, _FORMATS[key_cache.dtype])
         ws_bytes, launch = lib.fp_paged_fp8_workspace_bytes, lib.fp_paged_attention_fp8
-    else:
-        call = a = _lib.FpPagedArgs()
-        ws_bytes, launch = lib.fp_paged_workspace_bytes, lib.fp_paged_attention
-    a.q, a.q_stride_tok, a.q_stride_head = query.data_ptr(), query.stride(0), query.stride(1)
-    a.o, a.o_stride_tok, a.o_stride_head = out.data_ptr(), out.stride(0), out.stride(1)
-    a.key_cache, a.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
-    a.kc_stride_block, a.kc_stride_slot, a.kc_stride_head = key_cache.stride()[:3]
-    a.vc_stride_block, a.vc_stride_slot, a.vc_stride_head = value_cache.stride()[:3]
-    a.cu_seqlens, a.seqused, a.block_table = cu.data_ptr(), used.data_ptr(), table.data_ptr()
-    a.table_stride, a.num_tokens, a.num_blocks = table.stride(0), T, nb
-    a.batch, a.table_width, a.block_size = cu.numel() - 1, table.shape[1], bs
-    a.num_q_heads, a.num_kv_heads, a.head_dim = hq, hkv, d
-    a.dtype = _DTYPES[query.dtype]
-    a.cu_is64, a.used_is64 = cu.dtype == torch.int64, used.dtype == torch.int64
-    a.table_is64 = table.dtype == torch.int64
-    a.softmax_scale = float(scale)
-    with torch.cuda.device(dev):
-        # A buffer of this call's own: threads that share a stream may interleave
-        # their launches, and a shared one would be written between the chunks and
-        # their merge. The caching allocator hands it on in stream order.
-        ws = torch.empty(max(int(ws_bytes(ctypes.byref(call))), 256), dtype=torch.uint8,
-                         device=dev)
-        _lib.check(launch(ctypes.byref(call), ws.data_ptr(),
-                          torch.cuda.current_stream(dev).cuda_stream))
+    # A buffer of this call's own: threads that share a stream may interleave
+    # their launches, and a shared one would be written between the chunks and
+    # their merge. The caching allocator hands it on in stream order.
+    n = ws_bytes(ctypes.byref(call))
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    _launch(dev, launch, ctypes.byref(call), None if ws is None else ws.data_ptr())
     # a graph that saved `out` finds it changed, as after any in-place operation
     torch.autograd.graph.increment_version(out)
 
