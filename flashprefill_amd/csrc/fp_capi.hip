@@ -927,6 +927,10 @@ int fp_paged_attention_fp8(const fp_paged_fp8_args* a, void* ws, void* stream) {
   if (a->base.num_tokens == 0) return FP_OK;
   fp::Paged8Args r;
   const PagedSplit sp = paged8_split(&a->base, &r.unit, &r.groups);
+  // (the merge's launch holds fewer than 2^32 threads, 1024 for each head of a segment)
+  if (!sp.many && sp.tiles * a->base.num_kv_heads >= int64_t(1) << 22)
+    return fail(FP_E_UNSUPPORTED, "paged: %lld tiles of query rows in one call",
+                static_cast<long long>(sp.tiles));
   if (sp.bytes > 0 && !ws) return fail(FP_E_INVALID_ARG, "paged: workspace is NULL");
   if (!aligned16(ws)) return fail(FP_E_INVALID_ARG, "paged: workspace must be 16-byte aligned");
   r.min_share = r.unit == 128 ? 2 : 1;

@@ -908,9 +908,9 @@ __global__ __launch_bounds__(256, 2) void k_paged8_rows(Paged8Args pa) {
   if (__ballot(nf != 0.0f) != 0) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
-    // P and l 2^off times smaller (m larger): the sum of P V then stays below the
-    // largest value, as that of normalised weights does
-    const float off = static_cast<float>(32 - __clz(k1 - k0));
+    // P (at most 2^kStep) and l 2^off times smaller (m larger): the sum of P V then stays
+    // below the largest value, as that of normalised weights does
+    const float off = static_cast<float>(32 - __clz(k1 - k0)) + kStep;
     m_run += off;
     l_part *= __builtin_amdgcn_exp2f(-off);
     const float ms = m_run == -INFINITY ? 0.0f : m_run;

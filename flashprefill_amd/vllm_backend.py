@@ -136,14 +136,17 @@ def _check_rows(key, value, key_cache, value_cache, what: str) -> None:
 
 
 def _check_written(*tensors) -> None:
-    """Refuse what torch's own in-place operations refuse: several elements in one
-    place, and inference tensors outside inference mode."""
+    """Refuse what torch's own in-place operations refuse, or would record: several
+    elements in one place, inference tensors outside inference mode, and tensors that
+    require a gradient (the kernels have none)."""
     for t in tensors:
         if 0 in t.stride() and any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
             raise RuntimeError("a tensor to be written has several elements in one memory "
                                "location: clone() it first")
         if t.is_inference() and not torch.is_inference_mode_enabled():
             raise RuntimeError("an inference tensor cannot be written outside inference mode")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("a tensor to be written requires a gradient: use torch.no_grad()")
 
 
 def _cache_args(key, value, key_cache, value_cache, slots: int, n: int) -> _lib.FpKvCacheArgs:
@@ -173,7 +176,8 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.T
       row, its largest finite magnitude over the format's largest finite value (1
       for a row of zeros), and written beside it.
 
-    Slots named by two tokens hold either row, or parts of both."""
+    Slots named by two tokens hold either row, or parts of both. No derivative is
+    recorded."""
     _check_rows(key, value, key_cache, value_cache, "kv-cache write")
     _check_scales(key_cache, k_scale, v_scale)
     n = slot_mapping.numel()
@@ -193,6 +197,8 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.T
     written = [key_cache, value_cache]
     written += [s for s in (k_scale, v_scale) if s is not None and s.dim() == 3]
     _check_written(*written)
+    if len({t.data_ptr() for t in written}) < len(written):
+        raise ValueError("the caches and the scales to be written must be memory of their own")
     (ks, k_keep), (vs, v_keep) = _scale_args(k_scale, dev), _scale_args(v_scale, dev)
     _launch(dev, lib.fp_kv_cache_write_fp8,
             ctypes.byref(_lib.FpKvCacheFp8Args(base, ks, vs, _FORMATS[key_cache.dtype])))
@@ -214,7 +220,8 @@ def gather_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.
     No host synchronisation: what only the device sees is checked there. Offsets
     that descend or leave the rows make every row NaN, tokens before the first or
     past the room of the table, and pages outside the cache (a number below 0
-    counts from the end, as in an index), their own rows."""
+    counts from the end, as in an index), their own rows. No derivative is
+    recorded."""
     _check_rows(key, value, key_cache, value_cache, "kv-cache read-back")
     _check_scales(key_cache, k_scale, v_scale)
     if value.shape != key.shape:
@@ -237,6 +244,8 @@ def gather_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.
         if not t.is_cuda or t.device != dev:
             raise ValueError("key, value and the caches must be on one GPU")
     _check_written(key, value)
+    if key.numel() and key.data_ptr() == value.data_ptr():
+        raise ValueError("key and value must be memory of their own")
     if B == 0:
         return
     cu, table = cu_seqlens.to(dev).contiguous(), block_table.to(dev)

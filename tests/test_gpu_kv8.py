@@ -209,6 +209,14 @@ def test_wide_tables_many_sequences_and_every_chunk():
     lens = [(37 * i) % 300 + 1 for i in range(150)]
     _check(attention_case(lens, [1 + (i % 3 == 0) for i in range(150)], 4, 2, 64, 16, BF, E4M3,
                           "head"), 0.125)
+    # the same where the workgroups share the keys (a table with room for more)
+    lens = [(41 * i) % 1500 + 1 for i in range(150)]
+    for d, hkv in ((64, 2), (64, 3), (128, 2), (256, 1)):
+        _check(attention_case(lens, [i % 3 for i in range(150)], 2 * hkv, hkv, d, 16, BF, E4M3,
+                              "slot"), 1 / math.sqrt(d))
+    _check(attention_case([1, 9000, 0, 513, 130], [2, 1, 3, 0, 31], 6, 3, 64, 16, HF, E4M3,
+                          "head"), 0.125)
+    _check(attention_case([2500, 1300], [90, 200], 8, 2, 256, 16, BF, E4M3, "slot"), 0.06)
     _check(attention_case([40000], [1], 4, 1, 128, 16, BF, E5M2, "slot"), 0.09)
     _check(attention_case([20000], [70], 2, 1, 64, 16, HF, E4M3, "slot"), 0.12)
 
@@ -295,6 +303,48 @@ def test_small_probabilities(d, news, mode):
     step = torch.clamp(2.0 ** (want.abs().clamp_min(1e-30).log2().floor() - 10), min=2.0 ** -24)
     assert ((got - want).abs() <= 0.5 * step + 2.0 ** -16 * want.abs()).all(), \
         ((got - want).abs() / step).max()
+
+
+@pytest.mark.parametrize("d,page,mode", [(64, 16, "head"), (128, 16, "head"), (128, 16, "slot"),
+                                         (128, 24, "slot")])
+def test_values_near_the_largest_behind_a_low_maximum(d, page, mode):
+    """Values of 448 x 7e35 at keys whose scores all lie 7.5 (of 2^x) above those of the
+    first tile, so that the running maximum need not move: their mean is that value."""
+    n, new = 3000, 40
+    args = attention_case([n, 200], [new] * 2, 8, 2, d, page, BF, E4M3, mode, seed=5)
+    q, kc, vc, cu, used, table, ks, vs = args
+    q.zero_()
+    q[..., 0] = 1.0
+    for i, s in ((6, ks), (7, vs)):
+        args[i] = torch.where(s.isnan(), s, torch.full_like(s, 1.0 if i == 6 else 7e35))
+    k8, v8 = kc.view(torch.uint8), vc.view(torch.uint8)
+    k8[..., 0] = torch.tensor(7.5).to(E4M3).view(torch.uint8)
+    for b in range(2):
+        for t in range(64):
+            k8[table[b, t // page], t % page, :, 0] = 0
+    v8[:, :, 0, 3] = 0x7e
+    v8[:, :, 1, d - 2] = 0xfe
+    want, size = attention(*args, math.log(2.0))
+    assert want.isfinite().all()
+    got = _run(args, math.log(2.0)).double()
+    assert ((got - want).abs() <= bound(want, size, BF)).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("fmt,step", [(E4M3, 2.0 ** -9), (E5M2, 2.0 ** -16)])
+@pytest.mark.parametrize("news,d", [(1, 128), (40, 128), (1, 64), (40, 64), (1, 256)])
+def test_the_smallest_codes(dtype, fmt, step, news, d):
+    """K and V of subnormal codes (fp16 holds e5m2's as its own subnormals) and scales that
+    make them ordinary numbers."""
+    args = attention_case([700, 33], [news] * 2, 8, 2, d, 16, dtype, fmt, "tensor", seed=8)
+    g = torch.Generator().manual_seed(9)
+    for i in (1, 2):
+        codes = args[i].view(torch.uint8)
+        small = torch.randint(0, 4, codes.shape, generator=g).to(torch.uint8) | \
+            (torch.randint(0, 2, codes.shape, generator=g) << 7).to(torch.uint8)
+        args[i].view(torch.uint8).copy_(torch.where(codes == NAN_CODE, codes, small))
+    args[6], args[7] = torch.tensor([0.5 / step]), torch.tensor([1.0 / step])
+    _check(args, 1 / math.sqrt(d))
 
 
 def test_strided_inputs_and_untouched_rows():
@@ -717,6 +767,11 @@ def test_refusals():
         vb.reshape_and_cache(x, x, cache[0], cache[1, :1].expand(4, 16, 2, 64), slots)
     with pytest.raises(ValueError, match="one GPU"):
         vb.reshape_and_cache(x, x.cpu(), cache[0], cache[1], slots)
+    for kc, vc, ks, vs in ((cache[0], cache[0], sc, sc.clone()), (cache[0], cache[1], sc, sc)):
+        with pytest.raises(ValueError, match="of their own"):
+            vb.reshape_and_cache(x, x, kc, vc, slots, ks, vs)
+    with pytest.raises(RuntimeError, match="gradient"):
+        vb.reshape_and_cache(x, x, cache[0], cache[1], slots, sc.clone().requires_grad_(), sc)
     with pytest.raises(ValueError, match="device"):
         vb.reshape_and_cache(x, x, cache[0], cache[1], slots, sc.cpu(), sc)
     with torch.inference_mode():
@@ -731,4 +786,9 @@ def test_refusals():
     cu, table = torch.tensor([0, 3], device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV)
     with pytest.raises(RuntimeError, match="one memory"):
         vb.gather_cache(cache[0], cache[1], x, x[:1].expand(3, 2, 64), cu, table)
+    with pytest.raises(ValueError, match="of their own"):
+        vb.gather_cache(cache[0], cache[1], x, x, cu, table)
+    y = torch.ones_like(x, requires_grad=True)
+    with pytest.raises(RuntimeError, match="gradient"):
+        vb.gather_cache(cache[0], cache[1], x, y, cu, table)
     assert TOP[E4M3] == 448.0
