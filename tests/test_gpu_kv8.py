@@ -200,7 +200,7 @@ def test_peaked_and_flat_rows(dtype, news, scale, mode):
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("new", [1, 41])
 def test_head_counts(hq, hkv, d, new):
-    _check(attention_case([1300, 70, 700, 40], [new, 33 if new > 1 else 1, new, 0], hq, hkv, d, 16,
+    _check(attention_case([1900, 70, 700, 40], [new, 33 if new > 1 else 1, new, 0], hq, hkv, d, 16,
                           BF, E4M3, "head"), 1 / math.sqrt(d))
 
 
@@ -222,11 +222,14 @@ def test_wide_tables_many_sequences_and_every_chunk():
 
 
 @pytest.mark.parametrize("news", [1, 40])
-@pytest.mark.parametrize("d,page,mode", [(128, 16, "slot"), (64, 24, "head"), (128, 24, "slot")])
-def test_infinite_values(news, d, page, mode):
+@pytest.mark.parametrize("d,page,mode", [(128, 16, "slot"), (64, 24, "head"), (128, 24, "slot"),
+                                         (64, 16, "slot")])
+@pytest.mark.parametrize("width", [None, 200])
+def test_infinite_values(news, d, page, mode, width):
     """+inf and -inf (e5m2) in V at keys that every row sees: those dims are infinite, the
     others what they are without; in several chunks and in one."""
-    args = attention_case([1000, 200], [news] * 2, 8, 2, d, page, BF, E5M2, mode, seed=3)
+    args = attention_case([1000, 200], [news] * 2, 8, 2, d, page, BF, E5M2, mode, seed=3,
+                          width=width)
     codes = args[2].view(torch.uint8)
     for b, key in ((0, 500), (1, 77)):
         at = int(args[5][b, key // page]), key % page
@@ -242,9 +245,10 @@ def test_infinite_values(news, d, page, mode):
 
 @pytest.mark.parametrize("news,d", [(40, 128), (3, 128), (3, 64), (3, 256), (40, 64)])
 @pytest.mark.parametrize("what", ["value", "value scale", "key scale"])
-def test_a_token_that_a_row_does_not_see(what, news, d):
+@pytest.mark.parametrize("width", [None, 100])
+def test_a_token_that_a_row_does_not_see(what, news, d, width):
     """A NaN in the last new token's value, or in its scales, reaches the last query only."""
-    args = attention_case([500], [news], 8, 2, d, 16, BF, E4M3, "slot", seed=4)
+    args = attention_case([500], [news], 8, 2, d, 16, BF, E4M3, "slot", seed=4, width=width)
     want, size = attention(*args, 0.1)
     page, at = args[5][0, 499 // 16], 499 % 16
     if what == "value":
@@ -367,11 +371,13 @@ def test_strided_inputs_and_untouched_rows():
 
 
 @pytest.mark.parametrize("page", [16, 24, 64])
-@pytest.mark.parametrize("d,news", [(128, 1), (128, 40), (64, 40), (256, 2)])
-def test_what_only_the_device_sees(page, d, news):
+@pytest.mark.parametrize("d,news,width", [(128, 1, None), (128, 1, 200), (64, 1, 200), (128, 40, None),
+                                          (64, 40, None), (256, 2, 200)])
+def test_what_only_the_device_sees(page, d, news, width):
     """A length beyond the table and pages outside the cache: NaN rows, the other
     sequence as it is; offsets that do not fit: every row NaN."""
-    args = attention_case([1000, 200], [news] * 2, 8, 2, d, page, BF, E4M3, "slot", seed=page)
+    args = attention_case([1000, 200], [news] * 2, 8, 2, d, page, BF, E4M3, "slot", seed=page,
+                          width=width)
     want = _run(args, 0.1)
     for b, first in ((0, 384), (1, 64)):
         rows, rest = slice(news * b, news * b + news), slice(news * (1 - b), news * (2 - b))
