@@ -672,21 +672,23 @@ __global__ __launch_bounds__(256, 2) void k_paged8_rows(Paged8Args pa) {
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int half = lane >> 5, l32 = lane & 31;
   const int rows = nq * a.G;
+  // (a sequence's last rows see most keys and start first)
+  const int tl = (rows + 127) / 128 - 1 - tile.tl;
 
   // this lane's query row and its last visible key
-  const int rr = tile.tl * 128 + 32 * w + l32;
+  const int rr = tl * 128 + 32 * w + l32;
   const bool rvalid = rr < rows;
   const int qi = (rvalid ? rr : rows - 1) / a.G;
   const int64_t tok = sq.q0 + qi;
   const int hq = h * a.G + (rvalid ? rr : rows - 1) % a.G;
   const int lim = nk - nq + qi;
   // the wave's first and last visible keys' bounds (wave-uniform)
-  const int r0 = min(tile.tl * 128 + 32 * w, rows - 1);
-  const int r1 = min(tile.tl * 128 + 32 * w + 31, rows - 1);
+  const int r0 = min(tl * 128 + 32 * w, rows - 1);
+  const int r1 = min(tl * 128 + 32 * w + 31, rows - 1);
   const int lim_lo = __builtin_amdgcn_readfirstlane(nk - nq + r0 / a.G);
   const int lim_hi = __builtin_amdgcn_readfirstlane(nk - nq + r1 / a.G);
   // keys past the last row of the tile are visible to none of its rows
-  const int last_row = min(tile.tl * 128 + 127, rows - 1);
+  const int last_row = min(tl * 128 + 127, rows - 1);
   const int k1 = __builtin_amdgcn_readfirstlane(
       min(min(k0 + tile.chunk, nk), max(nk - nq + last_row / a.G + 1, 0)));
 
