@@ -159,8 +159,8 @@ struct PagedArgs {
   int32_t nc;        // chunk slots per row
   float* part;       // [T * Hq][nc][d] unnormalised outputs
   float* ml;         // [T * Hq][nc] (m, l) pairs
-  // V scale of KV head h at [h * vscale_head], by which k_paged_merge_rows multiplies
-  // a row's sum (8-bit caches with fixed scales), or null
+  // V scale of KV head h at [h * vscale_head], by which the merges multiply a row's sum
+  // (8-bit caches with fixed scales), or null
   const float* vscale;
   int32_t vscale_head;
 };
@@ -260,8 +260,10 @@ hipError_t launch_rope(const RopeArgs& a, int dtype, hipStream_t s);
 hipError_t launch_paged_rows(const PagedArgs& a, int dtype, int head_dim, int64_t tiles,
                              hipStream_t s);
 hipError_t launch_paged(const PagedArgs& a, int dtype, int head_dim, int64_t tiles, hipStream_t s);
-// combines the partials of k_paged_rows and its 8-bit form
-hipError_t launch_paged_merge_rows(const PagedArgs& a, int dtype, int head_dim, hipStream_t s);
+// combines the partials of k_paged8_rows: up to kMergeRowChunks chunk slots a wave takes
+// the rows of several heads and their chunks in turn, above a workgroup a row's chunks
+constexpr int kMergeRowChunks = 4;
+hipError_t launch_paged_merge8(const PagedArgs& a, int dtype, int head_dim, hipStream_t s);
 hipError_t launch_paged8(const Paged8Args& a, int dtype, int format, int head_dim, bool rows,
                          int64_t tiles, hipStream_t s);
 hipError_t launch_kv_cache_write8(const Cache8Args& a, int dtype, int format, hipStream_t s);

@@ -410,7 +410,8 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a) {
   for (int q = 0; q < XD; ++q) so[w][XD * lane + q] = acc[q];
   __syncthreads();
   if (t < D) {
-    const float o = (so[0][t] + so[1][t] + so[2][t] + so[3][t]) / L;
+    float o = (so[0][t] + so[1][t] + so[2][t] + so[3][t]) / L;
+    if (a.vscale != nullptr) o *= a.vscale[(hq / a.G) * a.vscale_head];
     static_cast<uint16_t*>(a.o)[tok * a.ost + static_cast<int64_t>(hq) * a.ohs + t] = T::from_f32(o);
   }
 }
@@ -854,6 +855,13 @@ hipError_t launch_merge_rows_t(const PagedArgs& a, hipStream_t s) {
 }
 
 template <typename T, int D>
+hipError_t launch_merge_t(const PagedArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((k_paged_merge<T, D>), dim3(static_cast<unsigned>(a.T * a.Hq)), dim3(256), 0,
+                     s, a);
+  return hipGetLastError();
+}
+
+template <typename T, int D>
 hipError_t launch_paged_rows_t(const PagedArgs& a, int64_t tiles, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(tiles * a.Hkv), static_cast<unsigned>(a.nc));
   if (a.bs % 16 == 0) hipLaunchKernelGGL((k_paged_rows<T, D, true>), grid, dim3(256), 0, s, a);
@@ -866,10 +874,7 @@ hipError_t launch_paged_t(const PagedArgs& a, int64_t tiles, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(tiles * a.Hkv), static_cast<unsigned>(a.nc));
   if (a.bs % 16 == 0) hipLaunchKernelGGL((k_paged<T, D, true>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((k_paged<T, D, false>), grid, dim3(256), 0, s, a);
-  if (a.nc > 1)
-    hipLaunchKernelGGL((k_paged_merge<T, D>), dim3(static_cast<unsigned>(a.T * a.Hq)), dim3(256), 0,
-                       s, a);
-  return hipGetLastError();
+  return a.nc > 1 ? launch_merge_t<T, D>(a, s) : hipGetLastError();
 }
 
 hipError_t launch_paged_rows(const PagedArgs& a, int dtype, int head_dim, int64_t tiles,
@@ -889,12 +894,14 @@ hipError_t launch_paged(const PagedArgs& a, int dtype, int head_dim, int64_t til
   });
 }
 
-hipError_t launch_paged_merge_rows(const PagedArgs& a, int dtype, int head_dim, hipStream_t s) {
-  if (head_dim == 128)
-    return dtype == FP_DTYPE_BF16 ? launch_merge_rows_t<BF16, 128>(a, s)
-                                  : launch_merge_rows_t<F16, 128>(a, s);
-  return dtype == FP_DTYPE_BF16 ? launch_merge_rows_t<BF16, 64>(a, s)
-                                : launch_merge_rows_t<F16, 64>(a, s);
+hipError_t launch_paged_merge8(const PagedArgs& a, int dtype, int head_dim, hipStream_t s) {
+  const bool bf = dtype == FP_DTYPE_BF16;
+  if (a.nc > kMergeRowChunks)
+    return head_dim == 128 ? (bf ? launch_merge_t<BF16, 128>(a, s) : launch_merge_t<F16, 128>(a, s))
+                           : (bf ? launch_merge_t<BF16, 64>(a, s) : launch_merge_t<F16, 64>(a, s));
+  return head_dim == 128
+             ? (bf ? launch_merge_rows_t<BF16, 128>(a, s) : launch_merge_rows_t<F16, 128>(a, s))
+             : (bf ? launch_merge_rows_t<BF16, 64>(a, s) : launch_merge_rows_t<F16, 64>(a, s));
 }
 
 }  // namespace fp

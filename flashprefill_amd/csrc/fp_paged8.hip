@@ -1043,7 +1043,7 @@ hipError_t launch_paged8(const Paged8Args& p, int dtype, int format, int head_di
     const hipError_t e = head_dim == 128 ? launch_rows_t<T, F, 128>(p, tiles, s)
                                          : launch_rows_t<T, F, 64>(p, tiles, s);
     if (e != hipSuccess || p.a.nc <= 1) return e;
-    return launch_paged_merge_rows(p.a, dtype, head_dim, s);
+    return launch_paged_merge8(p.a, dtype, head_dim, s);
   };
   if (dtype == FP_DTYPE_BF16)
     return format == FP_CACHE_E4M3 ? run(BF16{}, IntC<FP_CACHE_E4M3>{})
