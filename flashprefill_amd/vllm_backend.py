@@ -197,7 +197,7 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.T
     written = [key_cache, value_cache]
     written += [s for s in (k_scale, v_scale) if s is not None and s.dim() == 3]
     _check_written(*written)
-    if len({t.data_ptr() for t in written}) < len(written):
+    if n and len({t.data_ptr() for t in written}) < len(written):
         raise ValueError("the caches and the scales to be written must be memory of their own")
     (ks, k_keep), (vs, v_keep) = _scale_args(k_scale, dev), _scale_args(v_scale, dev)
     _launch(dev, lib.fp_kv_cache_write_fp8,

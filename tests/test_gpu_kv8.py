@@ -221,6 +221,16 @@ def test_wide_tables_many_sequences_and_every_chunk():
     _check(attention_case([20000], [70], 2, 1, 64, 16, HF, E4M3, "slot"), 0.12)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("mode", ["tensor", "head", "slot"])
+def test_few_and_many_chunks_of_many_rows(dtype, d, mode):
+    # 2 .. 4 chunk slots per row, and more (their partials are merged in two ways)
+    for lens, news in (([900, 500], [40, 33]), ([6000, 1000, 0], [65, 70, 3])):
+        _check(attention_case(lens, news, 8, 2, d, 16, dtype, E4M3, mode, seed=5),
+               1 / math.sqrt(d))
+
+
 @pytest.mark.parametrize("news", [1, 40])
 @pytest.mark.parametrize("d,page,mode", [(128, 16, "slot"), (64, 24, "head"), (128, 24, "slot"),
                                          (64, 16, "slot")])
