@@ -94,12 +94,19 @@ def _check_scales(cache: torch.Tensor, k_scale, v_scale) -> None:
                              f"{(nb, hkv, bs)}; got {tuple(s.shape)}")
 
 
+def _slot_scale_strides(scale: torch.Tensor) -> tuple:
+    """Strides of scales per slot between pages and between heads, 0 where there is one
+    (torch may give such a dimension any stride)."""
+    nb, hkv, _ = scale.shape
+    return scale.stride(0) if nb > 1 else 0, scale.stride(1) if hkv > 1 else 0
+
+
 def _scale_args(scale: Optional[torch.Tensor], device) -> tuple:
     """``fp_kv_scales`` of a checked scale, and the tensor whose memory it names."""
     if scale is None:
         return _lib.FpKvScales(), None
     if scale.dim() == 3:
-        return _lib.FpKvScales(scale.data_ptr(), scale.stride(0), scale.stride(1), 1), scale
+        return _lib.FpKvScales(scale.data_ptr(), *_slot_scale_strides(scale), 1), scale
     if scale.device != device or not scale.is_contiguous():
         scale = scale.to(device).contiguous()
     return _lib.FpKvScales(scale.data_ptr(), 0, 1 if scale.numel() > 1 else 0, 0), scale
@@ -342,9 +349,8 @@ def _paged_kernel_takes(query, key_cache, value_cache, out, cu, used, table, k_s
         if t.dtype != want or t.device != dev or not _rows_ok(t):
             return False
     for s in (k_scale, v_scale):
-        if s is not None and s.dim() == 3 and (
-                min(s.stride()[:2]) < 0 or
-                bs % 16 == 0 and (s.data_ptr() % 16 or s.stride(0) % 4 or s.stride(1) % 4)):
+        if s is not None and s.dim() == 3 and bs % 16 == 0 and \
+                (s.data_ptr() % 16 or any(st % 4 for st in _slot_scale_strides(s))):
             return False
     # torch refuses to write these, and so does the composition
     if (0 in out.stride() and any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride()))) or \

@@ -406,6 +406,21 @@ def test_what_only_the_device_sees(page, d, news, width):
         assert got.isnan().all(), cu
 
 
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("d", [64, 256])
+def test_one_head_or_one_page_of_any_stride(new, d):
+    # torch gives a dimension of one entry any stride, and contiguous() keeps it
+    for lens, page in (([100, 260], 16), ([700, 650], 128), ([40], 48)):
+        args = attention_case(lens, [new] * len(lens), 4, 1, d, page, BF, E4M3, "slot", seed=new)
+        for i in (6, 7):
+            args[i] = args[i].transpose(1, 2).contiguous().transpose(1, 2)
+            args[i] = args[i].as_strided(args[i].shape, (args[i].stride(0), 1, 1))
+            if args[i].shape[0] == 1:
+                args[i] = args[i].as_strided(args[i].shape, (7, 1, 1))
+        assert args[6].is_contiguous() and args[6].stride(1) == 1
+        _check(args, 0.1)
+
+
 def test_offsets_past_32_bits():
     """Pages behind the first 4 GiB of a cache, written, attended and read back."""
     hkv, d, page, n = 8, 128, 16, 200
