@@ -580,19 +580,29 @@ struct PagedSplit {
   int nc;
   size_t bytes;
 };
+// tiles of rt query rows, at most
+int64_t row_tiles(const fp_paged_args* a, int64_t rt) {
+  const int64_t G = a->num_q_heads / a->num_kv_heads, T = a->num_tokens;
+  return std::min<int64_t>(T * ((G + rt - 1) / rt), T * G / rt + a->batch);
+}
+// of nc chunks per row
+size_t partial_bytes(const fp_paged_args* a, int nc) {
+  return nc > 1 ? static_cast<size_t>(a->num_tokens * a->num_q_heads * nc) * (a->head_dim + 2) * 4
+                : 0;
+}
 PagedSplit paged_split(const fp_paged_args* a) {
   constexpr int64_t kManyRows = 32;
   PagedSplit r;
   const int64_t G = a->num_q_heads / a->num_kv_heads, T = a->num_tokens;
   r.many = a->head_dim <= 128 && T * G >= kManyRows * a->batch;
   const int64_t kTarget = r.many ? 512 : 8192, rt = r.many ? 128 : 16;
-  r.tiles = std::min<int64_t>(T * ((G + rt - 1) / rt), T * G / rt + a->batch);
+  r.tiles = row_tiles(a, rt);
   const int64_t longest = static_cast<int64_t>(a->table_width) * a->block_size;
   const int64_t wgs = std::max<int64_t>(1, r.tiles * a->num_kv_heads);
   int64_t nc = std::min<int64_t>(fp::kPagedMaxChunks, (kTarget + wgs - 1) / wgs);
   nc = std::min<int64_t>(nc, (longest + fp::kPagedMinChunk - 1) / fp::kPagedMinChunk);
   r.nc = static_cast<int>(std::max<int64_t>(1, nc));
-  r.bytes = r.nc > 1 ? static_cast<size_t>(T * a->num_q_heads * r.nc) * (a->head_dim + 2) * 4 : 0;
+  r.bytes = partial_bytes(a, r.nc);
   return r;
 }
 
@@ -622,21 +632,42 @@ fp::KvCacheArgs cache_args(const fp_kv_cache_args* a) {
   return k;
 }
 
-// An 8-bit call: many rows as a 16-bit one. Few: kPaged8Groups workgroups, as many as
-// the card holds at a time, share the keys in units of 128 (more where the units would
-// not count in 31 bits); where the table has room for kWhole keys at most, each segment
-// (16 rows of a KV head's queries) is a workgroup's as a whole. Shared and whole, 32 q / 8
-// kv heads, d = 128: 1, 32 and 128 sequences of 333 tokens 13.8, 18.5 and 37 us and 8.2,
-// 10.5 and 27; of 1,000 tokens 12.3, 23 and 71, and 12.0, 17 and 65; of 2,000 tokens 12.7, 39
-// and 117, and 18, 32 and 114.
+// An 8-bit call. Many rows up to head_dim 128: as a 16-bit call (512 workgroups with
+// 768, 1024 and 1536: 512 new of 8,192 tokens 118 us, 130, 130, 141; 100 of 30,000 106,
+// 132, 138, 160; 3 x 500 new of 6,144, 2,500 and 1,111 146, 152, 149, 137).
+//
+// At head_dim 256 k_paged8_rows runs one workgroup per CU, and pays from 128 rows per
+// sequence and 2^17 (row tile, head, key) triples on: for about 256 workgroups, chunks of
+// 512 keys at least. With and without it: 3 sequences of 5,000 tokens with 600 new ones,
+// 32 q / 4 kv heads, 591 and 1,236 us; of 2,500 with 350, 8 / 8, 82 and 128; of 1,100 with
+// 300, 32 / 8, 82 and 180; one of 2,000 with 500, 8 / 2 (2^16 triples), 49 and 40; 8 of
+// 3,000 with 16, 32 / 8 (64 rows each), 85 and 77.
+//
+// Few rows: kPaged8Groups workgroups, as many as the card holds at a time, share the keys
+// in units of 128 (more where the units would not count in 31 bits); where the table has
+// room for kWhole keys at most, each segment (16 rows of a KV head's queries) is a
+// workgroup's as a whole. Shared and whole, 32 q / 8 kv heads, d = 128: 1, 32 and 128
+// sequences of 333 tokens 13.8, 18.5 and 37 us and 8.2, 10.5 and 27; of 1,000 tokens 12.3,
+// 23 and 71, and 12.0, 17 and 65; of 2,000 tokens 12.7, 39 and 117, and 18, 32 and 114.
 PagedSplit paged8_split(const fp_paged_args* a, int* unit, int* groups) {
   constexpr int kWhole = 1024;
   PagedSplit r = paged_split(a);
   *unit = 128;
   const int pair = a->head_dim == 64 && a->num_kv_heads % 2 == 0 ? 2 : 1;
   *groups = a->num_kv_heads / pair;
-  if (r.many) return r;
   const int64_t longest = static_cast<int64_t>(a->table_width) * a->block_size;
+  const int64_t rows = a->num_tokens * (a->num_q_heads / a->num_kv_heads);
+  if (a->head_dim == 256 && rows >= int64_t(128) * a->batch) {
+    const int64_t tiles = row_tiles(a, 128), wgs = tiles * a->num_kv_heads;
+    if (wgs * longest >= int64_t(1) << 17) {
+      r.many = true;
+      r.tiles = tiles;
+      r.nc = static_cast<int>(
+          std::max<int64_t>(1, std::min<int64_t>((256 + wgs / 2) / wgs, longest / 512)));
+      r.bytes = partial_bytes(a, r.nc);
+    }
+  }
+  if (r.many) return r;
   const int64_t segs = std::max<int64_t>(1, r.tiles * *groups);
   const auto units = [&] { return segs * std::max<int64_t>(1, (longest + *unit - 1) / *unit); };
   r.bytes = 0;

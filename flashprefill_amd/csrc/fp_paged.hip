@@ -841,7 +841,9 @@ __global__ __launch_bounds__(256) void k_paged_merge_rows(PagedArgs a) {
 #pragma unroll
       for (int q = 0; q < XD; ++q) y[q] *= vs;
     }
-    if constexpr (XD == 2) *reinterpret_cast<uint32_t*>(op) = pack2<T>(y[0], y[1]);
+    if constexpr (XD == 4)
+      *reinterpret_cast<uint2*>(op) = make_uint2(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]));
+    else if constexpr (XD == 2) *reinterpret_cast<uint32_t*>(op) = pack2<T>(y[0], y[1]);
     else op[0] = T::from_f32(y[0]);
   }
 }
@@ -896,12 +898,12 @@ hipError_t launch_paged(const PagedArgs& a, int dtype, int head_dim, int64_t til
 
 hipError_t launch_paged_merge8(const PagedArgs& a, int dtype, int head_dim, hipStream_t s) {
   const bool bf = dtype == FP_DTYPE_BF16;
-  if (a.nc > kMergeRowChunks)
-    return head_dim == 128 ? (bf ? launch_merge_t<BF16, 128>(a, s) : launch_merge_t<F16, 128>(a, s))
-                           : (bf ? launch_merge_t<BF16, 64>(a, s) : launch_merge_t<F16, 64>(a, s));
-  return head_dim == 128
-             ? (bf ? launch_merge_rows_t<BF16, 128>(a, s) : launch_merge_rows_t<F16, 128>(a, s))
-             : (bf ? launch_merge_rows_t<BF16, 64>(a, s) : launch_merge_rows_t<F16, 64>(a, s));
+  return with_head_dim(head_dim, [&](auto dc) {
+    constexpr int D = decltype(dc)::value;
+    if (a.nc > kMergeRowChunks)
+      return bf ? launch_merge_t<BF16, D>(a, s) : launch_merge_t<F16, D>(a, s);
+    return bf ? launch_merge_rows_t<BF16, D>(a, s) : launch_merge_rows_t<F16, D>(a, s);
+  });
 }
 
 }  // namespace fp

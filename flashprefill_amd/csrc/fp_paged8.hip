@@ -644,7 +644,7 @@ __global__ __launch_bounds__(1024) void k_paged8_merge(Paged8Args pa) {
 // of its cached value's own step, where a third part would add half as many MFMAs
 // to P.V again.
 template <typename T, int F, int D, bool P16, bool PS>
-__global__ __launch_bounds__(256, 2) void k_paged8_rows(Paged8Args pa) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged8_rows(Paged8Args pa) {
   constexpr int KT = 64, TT = KT / 32;
   constexpr int KS = D / 16, DT = D / 32, CH = D / 8;
   constexpr int LPR = D / 16;        // lanes per key (16 bytes each)
@@ -1040,8 +1040,8 @@ hipError_t launch_paged8(const Paged8Args& p, int dtype, int format, int head_di
         }
         return launch_few_t<T, F, D, 1>(p, s);
       });
-    const hipError_t e = head_dim == 128 ? launch_rows_t<T, F, 128>(p, tiles, s)
-                                         : launch_rows_t<T, F, 64>(p, tiles, s);
+    const hipError_t e = with_head_dim(
+        head_dim, [&](auto d) { return launch_rows_t<T, F, decltype(d)::value>(p, tiles, s); });
     if (e != hipSuccess || p.a.nc <= 1) return e;
     return launch_paged_merge8(p.a, dtype, head_dim, s);
   };

@@ -361,6 +361,54 @@ def test_the_smallest_codes(dtype, fmt, step, news, d):
     _check(args, 1 / math.sqrt(d))
 
 
+@pytest.fixture
+def roomy(monkeypatch):
+    """Cases whose tables have room for 40,000 keys: at head_dim 256 the kernel of many
+    rows takes calls of 128 rows per sequence that may be long."""
+    plain = attention_case
+
+    def case(lens, news, hq, hkv, d, page, *args, width=None, **more):
+        return plain(lens, news, hq, hkv, d, page, *args, width=40000 // page, **more)
+    monkeypatch.setitem(globals(), "attention_case", case)
+
+
+@pytest.mark.parametrize("lens,news", [([900, 0, 1300], [200, 3, 130]), ([1500], [700]),
+                                       ([127, 128, 129, 64], [31, 32, 33, 64]), ([3, 50], [6, 60]),
+                                       ([2049, 1000, 65, 320, 30], [97, 65, 65, 1, 40])])
+@pytest.mark.parametrize("page,mode", [(16, "slot"), (16, "head"), (24, "slot"), (24, "none"),
+                                       (1, "tensor"), (64, "none")])
+@pytest.mark.parametrize("dtype,fmt", [(BF, E4M3), (HF, E5M2)])
+def test_many_rows_of_256(lens, news, page, mode, dtype, fmt, roomy):
+    _check(attention_case(lens, news, 8, 2, 256, page, dtype, fmt, mode), 1 / 16)
+
+
+def test_many_rows_of_256_with_other_head_counts(roomy):
+    for hq, hkv in ((5, 5), (7, 1), (34, 2)):
+        _check(attention_case([1900, 70, 700], [150, 30, 141], hq, hkv, 256, 16, BF, E4M3, "head"),
+               1 / 16)
+
+
+@pytest.mark.parametrize("page,mode", [(16, "slot"), (16, "head"), (24, "slot")])
+def test_many_rows_of_256_and_extreme_values(page, mode, roomy):
+    test_infinite_values(40, 256, page, mode, None)
+    test_values_near_the_largest(40, 256, page, mode)
+    test_values_near_the_largest_behind_a_low_maximum(256, page, mode)
+    for fmt, step in ((E4M3, 2.0 ** -9), (E5M2, 2.0 ** -16)):
+        test_the_smallest_codes(HF, fmt, step, 40, 256)
+    for scale in (0.5, -0.3, 1e-3, 0.0):
+        test_peaked_and_flat_rows(BF, 40, scale, mode)
+    test_small_probabilities(256, 40, "slot" if mode == "slot" else "none")
+
+
+def test_many_rows_of_256_and_what_only_the_device_sees(roomy):
+    for page in (16, 24, 64):
+        test_what_only_the_device_sees(page, 256, 40, None)
+    for what in ("value", "value scale", "key scale"):
+        test_a_token_that_a_row_does_not_see(what, 40, 256, None)
+    for slot in ("key", "value"):
+        test_scales_of_two_kinds(16, 256, 40, slot)
+
+
 def test_strided_inputs_and_untouched_rows():
     args = attention_case([300, 70], [1, 1], 8, 2, 128, 16, BF, E4M3, "slot")
     want = _run(args, 0.1)
