@@ -662,8 +662,8 @@ PagedSplit paged8_split(const fp_paged_args* a, int* unit, int* groups) {
     if (wgs * longest >= int64_t(1) << 17) {
       r.many = true;
       r.tiles = tiles;
-      r.nc = static_cast<int>(
-          std::max<int64_t>(1, std::min<int64_t>((256 + wgs / 2) / wgs, longest / 512)));
+      const int64_t nc = std::min<int64_t>((256 + wgs / 2) / wgs, longest / 512);
+      r.nc = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(nc, fp::kPagedMaxChunks)));
       r.bytes = partial_bytes(a, r.nc);
     }
   }

@@ -100,6 +100,32 @@ def test_write_of_every_16_bit_value(fmt, dtype):
             assert _same(c.view(128, 4, 128).cpu(), want), s
 
 
+@pytest.mark.parametrize("slot", [0, 1])
+def test_write_and_read_back_with_scales_of_two_kinds(slot):
+    """K's scales per slot beside fixed ones of V, and the other way round: each as in a
+    call in which both are of its kind."""
+    g = torch.Generator().manual_seed(3)
+    rows = (3 * torch.randn(2, 100, 4, 64, generator=g)).to(BF).to(DEV)
+    slots = torch.randperm(7 * 24, generator=g)[:100].to(DEV)
+    fixed = torch.tensor([0.01, 0.02, 0.5, 0.003], device=DEV)
+    cu = torch.tensor([0, 7 * 24], dtype=torch.int32, device=DEV)
+    table = torch.arange(7, dtype=torch.int32, device=DEV).view(1, -1)
+
+    def run(kinds):
+        c = torch.zeros(2, 7, 24, 4, 64, dtype=torch.uint8, device=DEV).view(E4M3)
+        sc = [torch.ones(7, 4, 24, device=DEV) if k else fixed for k in kinds]
+        vb.reshape_and_cache(*rows, *c, slots, *sc)
+        back = torch.zeros(2, 7 * 24, 4, 64, dtype=BF, device=DEV)
+        vb.gather_cache(*c, *back, cu, table, None, *sc)
+        return c.view(torch.uint8), sc, back
+
+    got = run([slot == 0, slot == 1])
+    for i in range(2):
+        want = run([i == slot] * 2)
+        assert torch.equal(got[0][i], want[0][i]) and torch.equal(got[1][i], want[1][i])
+        assert torch.equal(got[2][i], want[2][i]) and got[2][i].any()
+
+
 def test_write_of_no_tokens_and_index_types():
     cache = torch.zeros(2, 4, 16, 2, 64, dtype=torch.uint8, device=DEV).view(E4M3)
     x = torch.ones(3, 2, 64, dtype=BF, device=DEV)
@@ -386,6 +412,17 @@ def test_many_rows_of_256_with_other_head_counts(roomy):
     for hq, hkv in ((5, 5), (7, 1), (34, 2)):
         _check(attention_case([1900, 70, 700], [150, 30, 141], hq, hkv, 256, 16, BF, E4M3, "head"),
                1 / 16)
+
+
+def test_one_token_of_128_heads_over_every_chunk():
+    # the most chunk slots: one tile of rows, and a table with room for 2^17 keys and more
+    args = attention_case([34000], [1], 128, 1, 256, 16, BF, E4M3, "head", width=9000)
+    q, kc, vc, cu, used, table, ks, vs = args
+    rows = table[0, :34000 // 16].long()
+    k, v = (values(c, s)[rows].reshape(-1, 256)[:34000] for c, s in ((kc, ks), (vc, vs)))
+    p = torch.softmax(q[0].double() @ k.t() / 16, -1)
+    got = _run(args, 1 / 16).double()
+    assert ((got[0] - p @ v).abs() <= bound(p @ v, p @ v.abs(), BF)).all()
 
 
 @pytest.mark.parametrize("page,mode", [(16, "slot"), (16, "head"), (24, "slot")])
