@@ -9,6 +9,16 @@
 // types, s_k multiplies the fp32 score, a fixed s_v the fp32 row at the end and one
 // per slot the fp32 P of its key. P s_v enters P.V as bf16 parts (fp32's exponents,
 // so nothing underflows) beside c_v as bf16, whatever the type of q.
+//
+// Few rows (k_paged8) are bound by HBM where there are many bytes: 32 sequences of 300 ..
+// 15,000 tokens, 32 q / 8 kv heads of 128, 447 MB of codes in 95 us (4.7 TB/s) and 6.5 for
+// the merge; one sequence of 65,000, 137 MB with its scales, 31 and 7; one of 333, 8 us,
+// of which 1.7 are the launch, 1.5 the search for the place of the workgroup and 3.3 the
+// first loads and the end of a segment. Many rows (k_paged8_rows) are bound by MFMA, VALU
+// and LDS alike (about 1,500 cycles each per wave and tile of 64 keys) and by how little
+// the two waves of a SIMD overlap them: 2,048 new tokens of each of 4 sequences of 4,096 ..
+// 6,144 in 728 us, 713 TFLOP/s (1,070 counting both parts of P), MFMA busy 40 % of the
+// time; raised wave priorities around the MFMAs are 0 to 3 % slower.
 #include "fp_float8.h"
 #include "fp_paged_common.h"
 
@@ -636,13 +646,20 @@ __global__ __launch_bounds__(1024) void k_paged8_merge(Paged8Args pa) {
   }
 }
 
-// Many rows (prefill over a cached prefix): k_paged_rows with tiles that are
+// Many rows (prefill over a cached prefix): 128-row tiles as in k_paged_rows, over keys that are
 // widened on their way into LDS. The 64 keys of a tile are loaded into registers
 // (16 keys by each wave, a tile ahead), widened once per workgroup and written as
 // 16-bit tiles, K in q's type and V in bf16; P s_v takes two bf16 parts: 2^-17 of
 // each product, an eighth of what rounding the output to fp16 may lose and a 256th
 // of its cached value's own step, where a third part would add half as many MFMAs
-// to P.V again.
+// to P.V again (one part: a fifth less time).
+//
+// Chunks have the length of the call's longest sequence over its chunk slots. Chunks cut
+// to each sequence, for an equal share of all keys per workgroup, balance the workgroups
+// but split more rows: 118 -> 146 us (512 new of 8,192 tokens), 82 -> 102 (300 new of
+// 5,500 and of 1,200), 157 -> 144 .. 159 (500 new of 6,144, 2,500 and 1,111).
+//
+// D = 256: one workgroup per CU (256 VGPRs and 240 AGPRs, 130 KB of LDS).
 template <typename T, int F, int D, bool P16, bool PS>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged8_rows(Paged8Args pa) {
   constexpr int KT = 64, TT = KT / 32;
