@@ -519,6 +519,11 @@ int scratch_on_current_device(void** out) {
   return FP_OK;
 }
 
+// A stride between n entries: a dimension of one entry may have any.
+bool stride_ok(int64_t stride, int64_t n, int64_t step) {
+  return n == 1 || (stride >= 0 && stride % step == 0);
+}
+
 int paged_valid(const fp_paged_args* a) {
   if (!a) return fail(FP_E_INVALID_ARG, "paged arguments are NULL");
   if (a->dtype != FP_DTYPE_BF16 && a->dtype != FP_DTYPE_F16)
@@ -542,8 +547,11 @@ int paged_valid(const fp_paged_args* a) {
                           a->o_stride_head,   a->kc_stride_block, a->kc_stride_slot,
                           a->kc_stride_head,  a->vc_stride_block, a->vc_stride_slot,
                           a->vc_stride_head};
+  const int64_t n[10] = {a->num_tokens, a->num_q_heads,  a->num_tokens, a->num_q_heads,
+                         a->num_blocks, a->block_size,   a->num_kv_heads, a->num_blocks,
+                         a->block_size, a->num_kv_heads};
   for (int i = 0; i < 10; ++i)
-    if (st[i] < 0 || st[i] % 8)
+    if (!stride_ok(st[i], n[i], 8))
       return fail(FP_E_INVALID_ARG, "paged: strides must be non-negative multiples of 8 elements");
   // a lane's offset inside a page (16 slots) is formed in 32 bits
   if (a->kc_stride_slot >= (int64_t(1) << 24) || a->vc_stride_slot >= (int64_t(1) << 24))
@@ -745,13 +753,15 @@ int paged8_valid(const fp_paged_fp8_args* a) {
   if (rc != FP_OK || a->base.num_tokens == 0) return rc;
   const int64_t st[6] = {a->base.kc_stride_block, a->base.kc_stride_slot, a->base.kc_stride_head,
                          a->base.vc_stride_block, a->base.vc_stride_slot, a->base.vc_stride_head};
+  const int64_t n[3] = {a->base.num_blocks, a->base.block_size, a->base.num_kv_heads};
   for (int i = 0; i < 6; ++i)
-    if (st[i] % 16)
+    if (!stride_ok(st[i], n[i % 3], 16))
       return fail(FP_E_INVALID_ARG, "paged: strides of an 8-bit cache must be multiples of 16");
   for (const fp_kv_scales* s : {&a->k_scale, &a->v_scale}) {
     if ((rc = scales_valid(*s, "paged")) != FP_OK) return rc;
     if (s->per_slot && a->base.block_size % 16 == 0 &&
-        (!aligned16(s->data) || s->stride_block % 4 || s->stride_head % 4))
+        (!aligned16(s->data) || !stride_ok(s->stride_block, n[0], 4) ||
+         !stride_ok(s->stride_head, n[2], 4)))
       return fail(FP_E_INVALID_ARG, "paged: scales per slot must be 16-byte aligned with strides "
                   "of multiples of 4 where block_size is a multiple of 16");
   }
@@ -785,8 +795,11 @@ int cache8_valid(const fp_kv_cache_args* a, const fp_kv_scales& ks, const fp_kv_
   const int64_t strides[10] = {a->k_stride_tok, a->k_stride_head, a->v_stride_tok, a->v_stride_head,
                                a->kc_stride_block, a->kc_stride_slot, a->kc_stride_head,
                                a->vc_stride_block, a->vc_stride_slot, a->vc_stride_head};
+  const int64_t n[10] = {a->num_tokens, a->num_kv_heads, a->num_tokens, a->num_kv_heads,
+                         a->num_blocks, a->block_size,   a->num_kv_heads, a->num_blocks,
+                         a->block_size, a->num_kv_heads};
   for (int i = 0; i < 10; ++i)
-    if (strides[i] < 0 || strides[i] % 8)
+    if (!stride_ok(strides[i], n[i], 8))
       return fail(FP_E_INVALID_ARG, "%s: strides must be non-negative multiples of 8 elements", what);
   const int rc = scales_valid(ks, what);
   return rc != FP_OK ? rc : scales_valid(vs, what);
@@ -974,7 +987,7 @@ int fp_paged_attention_fp8(const fp_paged_fp8_args* a, void* ws, void* stream) {
   r.vs = scales(a->v_scale);
   if (!r.vs.slot) {
     r.a.vscale = r.vs.p;
-    r.a.vscale_head = static_cast<int32_t>(r.vs.sh);
+    r.a.vscale_head = r.vs.sh;
   }
   const hipError_t e = fp::launch_paged8(r, a->base.dtype, a->format, a->base.head_dim, sp.many,
                                          sp.tiles, static_cast<hipStream_t>(stream));

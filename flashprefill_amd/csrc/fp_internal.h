@@ -162,7 +162,7 @@ struct PagedArgs {
   // V scale of KV head h at [h * vscale_head], by which the merges multiply a row's sum
   // (8-bit caches with fixed scales), or null
   const float* vscale;
-  int32_t vscale_head;
+  int64_t vscale_head;
 };
 
 // Scales of an 8-bit cache: one for all (sh 0) or per KV head (sh 1), or one per

@@ -310,13 +310,13 @@ def paged_decode_attention(query: torch.Tensor, key_cache: torch.Tensor,
 _INDEX = (torch.int32, torch.int64)
 
 
-def _rows_ok(t: torch.Tensor) -> bool:
+def _rows_ok(t: torch.Tensor, any_stride_of_one: bool) -> bool:
     step = 16 // t.element_size()
     *rest, last = t.stride()
     if last != 1 or t.data_ptr() % 16:
         return False
-    for s in rest:
-        if s % step or s < 0:
+    for i, s in enumerate(rest):
+        if (s % step or s < 0) and not (any_stride_of_one and t.shape[i] == 1):
             return False
     return True
 
@@ -346,7 +346,7 @@ def _paged_kernel_takes(query, key_cache, value_cache, out, cu, used, table, k_s
     if cdt != dt and cdt not in _FORMATS:
         return False
     for t, want in ((query, dt), (key_cache, cdt), (value_cache, cdt), (out, dt)):
-        if t.dtype != want or t.device != dev or not _rows_ok(t):
+        if t.dtype != want or t.device != dev or not _rows_ok(t, cdt != dt):
             return False
     for s in (k_scale, v_scale):
         if s is not None and s.dim() == 3 and bs % 16 == 0 and \

@@ -506,6 +506,49 @@ def test_one_head_or_one_page_of_any_stride(new, d):
         _check(args, 0.1)
 
 
+def test_rows_and_caches_of_one_entry_and_any_stride():
+    g = torch.Generator().manual_seed(2)
+
+    def odd(x, dim, stride):  # the same memory with another stride of a dimension of one entry
+        st = list(x.stride())
+        assert x.shape[dim] == 1
+        st[dim] = stride
+        return x.as_strided(x.shape, st)
+
+    for page in (16, 1):
+        n = 16 if page == 16 else 1
+        k, v = (odd(odd(torch.randn(1, 1, 64, generator=g).to(BF).to(DEV), 0, 3), 1, 1)
+                for _ in range(2))
+        caches = [torch.full((1, page, 1, 64), NAN_CODE, dtype=torch.uint8, device=DEV).view(E4M3)
+                  for _ in range(2)]
+        caches = [odd(odd(c, 0, 5), 2, 1) for c in caches]
+        if page == 1:
+            caches = [odd(c, 1, 7) for c in caches]
+        sc = [odd(odd(torch.ones(1, 1, page, device=DEV), 0, 3), 1, 1) for _ in range(2)]
+        vb.reshape_and_cache(k, v, *caches, torch.tensor([n - 1], device=DEV), *sc)
+        kw, ks = quantise(k.cpu(), E4M3, None)
+        assert torch.equal(caches[0][0, n - 1].view(torch.uint8).cpu(), kw[0].view(torch.uint8))
+        assert torch.equal(sc[0][0, :, n - 1].cpu(), ks[0])
+        table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+        back = [odd(torch.zeros(1, 1, 64, dtype=BF, device=DEV), 0, 3) for _ in range(2)]
+        vb.gather_cache(*caches, *back, torch.tensor([0, 1], device=DEV), table,
+                        torch.tensor([n - 1], device=DEV), *sc)
+        vw, vs = quantise(v.cpu(), E4M3, None)
+        want = (vw.float() * vs.unsqueeze(-1)).to(BF)
+        assert torch.equal(back[1].cpu(), want)
+        if page == 16:
+            caches = [c[:, n - 1:].contiguous().expand(1, 16, 1, 64).contiguous() for c in
+                      (x.view(torch.uint8) for x in caches)]
+            caches = [odd(c.view(E4M3), 2, 1) for c in caches]
+            sc = [odd(s[:, :, n - 1:].expand(1, 1, 16).contiguous(), 1, 1) for s in sc]
+        q = odd(torch.randn(1, 2, 64, generator=g).to(BF).to(DEV), 0, 1)
+        out = odd(torch.zeros(1, 2, 64, dtype=BF, device=DEV), 0, 1)
+        meta = [torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([0, 1], [1])]
+        assert vb._paged_kernel_takes(q, *caches, out, *meta, table, *sc)
+        vb.paged_decode_attention(q, *caches, out, *meta, table, 0.1, *sc)
+        assert torch.equal(out.cpu(), want.expand(1, 2, 64))  # (one key: its value)
+
+
 def test_offsets_past_32_bits():
     """Pages behind the first 4 GiB of a cache, written, attended and read back."""
     hkv, d, page, n = 8, 128, 16, 200
