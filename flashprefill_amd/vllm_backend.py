@@ -25,7 +25,7 @@ The v1 forward mirrors what the 0.12 patch does to
 * an fp8 ``kv_cache_dtype`` (:151-166) keeps the cache in 8-bit floats with the
   layer's ``_k_scale`` / ``_v_scale``: written by the HIP kernel behind
   ``fp_kv_cache_write_fp8``, attended by ``fp_paged_attention_fp8``. The query
-  stays in 16 bits.
+  stays in 16 bits: one that the layer has quantised is refused.
 
 vLLM is not a dependency: the forward only touches the attributes of the
 impl object and the metadata that the reference's forward reads, and the two
@@ -295,8 +295,8 @@ def paged_decode_attention(query: torch.Tensor, key_cache: torch.Tensor,
 
     Caches of float8_e4m3fn or float8_e5m2 stand for their values times
     ``k_scale`` / ``v_scale``, which are as ``reshape_and_cache`` takes them; query
-    and out stay in 16 bits, and no cached value is rounded on the way
-    (``fp_paged_attention_fp8``)."""
+    and out stay in 16 bits (a query of 8 bits is refused), and no cached value is
+    rounded on the way (``fp_paged_attention_fp8``)."""
     _check_scales(key_cache, k_scale, v_scale)
     if _paged_kernel_takes(query, key_cache, value_cache, out, cu_seqlens_q, seqused_k,
                            block_table, k_scale, v_scale):
@@ -421,6 +421,9 @@ def paged_attention_reference(query: torch.Tensor, key_cache: torch.Tensor,
     """The torch composition of ``paged_decode_attention`` in fp32 (one small
     gather per sequence): the kernels' reference, and the path of the calls
     they do not take."""
+    if key_cache.dtype in _FORMATS and query.element_size() < 2:
+        raise NotImplementedError(f"a query of {query.dtype} over an 8-bit cache: its codes have a "
+                                  f"scale of their own, which this operation does not take")
     cu = cu_seqlens_q.tolist()
     used = seqused_k.tolist()
     _, bs, hkv, d = key_cache.shape
