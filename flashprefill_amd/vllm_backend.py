@@ -156,6 +156,30 @@ def _check_written(*tensors) -> None:
             raise RuntimeError("a tensor to be written requires a gradient: use torch.no_grad()")
 
 
+def _torch_only() -> bool:
+    """Whether a trace or a dispatch mode is on: they see torch operations, not kernels."""
+    return torch._C._get_tracing_state() is not None or torch._C._len_torch_dispatch_stack() > 0
+
+
+def _check_no_tangents(*tensors) -> None:
+    """Refuse forward-mode tangents, which the kernels would drop."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("a tensor has a forward-mode tangent: the cache's write and "
+                                      "read-back have no derivative")
+
+
+def _check_places(what: str, *tensors) -> None:
+    """Refuse tensors to be written that begin at one place. (Tensors without memory, as
+    those of a trace over fake ones, have a storage of their own all the same.)"""
+    at = {t.data_ptr() for t in tensors} if not _torch_only() else \
+        {(t.untyped_storage()._cdata, t.storage_offset()) for t in tensors}
+    if len(at) < len(tensors):
+        raise ValueError(f"{what} must be memory of their own")
+
+
 def _cache_args(key, value, key_cache, value_cache, slots: int, n: int) -> _lib.FpKvCacheArgs:
     nb, bs, hkv, d = key_cache.shape
     return _lib.FpKvCacheArgs(key.data_ptr(), value.data_ptr(), *key.stride()[:2],
@@ -184,32 +208,70 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.T
       for a row of zeros), and written beside it.
 
     Slots named by two tokens hold either row, or parts of both. No derivative is
-    recorded."""
+    recorded (forward-mode tangents are refused by 8-bit caches). Under a trace or a
+    dispatch mode the write is made of torch operations, with the same results."""
     _check_rows(key, value, key_cache, value_cache, "kv-cache write")
     _check_scales(key_cache, k_scale, v_scale)
     n = slot_mapping.numel()
     if key.shape[0] < n or value.shape[0] < n:
         raise ValueError(f"key {tuple(key.shape)} / value {tuple(value.shape)} do not match the "
                          f"cache {tuple(key_cache.shape)} and {n} slots")
-    dev = key.device
+    dev, eight = key.device, key_cache.dtype in _FORMATS
+    if eight:
+        _check_no_tangents(key, value, key_cache, value_cache, k_scale, v_scale)
     for t in (key, value, key_cache, value_cache):
         if not t.is_cuda or t.device != dev:
             raise ValueError("key, value and the caches must be on one GPU")
+    if eight:
+        written = [key_cache, value_cache]
+        written += [s for s in (k_scale, v_scale) if s is not None and s.dim() == 3]
+        _check_written(*written)
+        if n:
+            _check_places("the caches and the scales to be written", *written)
+    if _torch_only():
+        reshape_and_cache_reference(key, value, key_cache, value_cache, slot_mapping, k_scale,
+                                    v_scale)
+        return
     slots = slot_mapping.to(device=dev, dtype=torch.int64).contiguous()
     lib = _lib.load()
     base = _cache_args(key, value, key_cache, value_cache, slots.data_ptr(), n)
-    if key_cache.dtype not in _FORMATS:
+    if not eight:
         _launch(dev, lib.fp_kv_cache_write, ctypes.byref(base))
         return
-    written = [key_cache, value_cache]
-    written += [s for s in (k_scale, v_scale) if s is not None and s.dim() == 3]
-    _check_written(*written)
-    if n and len({t.data_ptr() for t in written}) < len(written):
-        raise ValueError("the caches and the scales to be written must be memory of their own")
     (ks, k_keep), (vs, v_keep) = _scale_args(k_scale, dev), _scale_args(v_scale, dev)
     _launch(dev, lib.fp_kv_cache_write_fp8,
             ctypes.byref(_lib.FpKvCacheFp8Args(base, ks, vs, _FORMATS[key_cache.dtype])))
     torch.autograd.graph.increment_version(written)
+
+
+@torch.no_grad()
+def reshape_and_cache_reference(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
+                                value_cache: torch.Tensor, slot_mapping: torch.Tensor,
+                                k_scale: Optional[torch.Tensor] = None,
+                                v_scale: Optional[torch.Tensor] = None) -> None:
+    """The torch composition of ``reshape_and_cache``, what a trace or a dispatch mode
+    sees of it."""
+    bs, dev = key_cache.shape[1], key_cache.device
+    slots = slot_mapping.reshape(-1).long().to(dev)
+    rows = ((slots >= 0) & (slots < key_cache.shape[0] * bs)).nonzero().view(-1)
+    page, at = slots[rows] // bs, slots[rows] % bs
+    for x, cache, scale in ((key, key_cache, k_scale), (value, value_cache, v_scale)):
+        x = x.to(dev)[rows]
+        if cache.dtype not in _FORMATS:
+            cache[page, at] = x
+            continue
+        x, top = x.float(), torch.finfo(cache.dtype).max
+        s = None
+        if scale is not None and scale.dim() == 3:
+            # (a tensor, by which torch divides: a number's reciprocal it would multiply by)
+            s = x.abs().masked_fill(~x.isfinite(), 0.0).amax(-1) / x.new_full((), top)
+            s = torch.where(s > 0, s, torch.ones_like(s))
+            scale[page, :, at] = s
+        elif scale is not None:
+            s = scale.to(dev).view(1, -1)
+        if s is not None:
+            x = x / s.unsqueeze(-1)
+        cache[page, at] = x.clamp(-top, top).to(cache.dtype)
 
 
 def gather_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.Tensor,
@@ -228,7 +290,8 @@ def gather_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.
     that descend or leave the rows make every row NaN, tokens before the first or
     past the room of the table, and pages outside the cache (a number below 0
     counts from the end, as in an index), their own rows. No derivative is
-    recorded."""
+    recorded (forward-mode tangents are refused). Under a trace or a dispatch mode the
+    read-back is made of torch operations, with the same results."""
     _check_rows(key, value, key_cache, value_cache, "kv-cache read-back")
     _check_scales(key_cache, k_scale, v_scale)
     if value.shape != key.shape:
@@ -243,6 +306,7 @@ def gather_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.
     for name, t in (("cu_seqlens", cu_seqlens), ("block_table", block_table), ("starts", starts)):
         if t is not None and t.dtype not in _INDEX:
             raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
+    _check_no_tangents(key, value, key_cache, value_cache, k_scale, v_scale)
     if not cu_seqlens.is_cuda:  # known without a synchronisation
         at = cu_seqlens.tolist()
         if at[0] < 0 or at[-1] > key.shape[0] or any(x > y for x, y in zip(at, at[1:])):
@@ -251,9 +315,13 @@ def gather_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.
         if not t.is_cuda or t.device != dev:
             raise ValueError("key, value and the caches must be on one GPU")
     _check_written(key, value)
-    if key.numel() and key.data_ptr() == value.data_ptr():
-        raise ValueError("key and value must be memory of their own")
+    if key.numel():
+        _check_places("key and value", key, value)
     if B == 0:
+        return
+    if _torch_only():
+        gather_cache_reference(key_cache, value_cache, key, value, cu_seqlens, block_table, starts,
+                               k_scale, v_scale)
         return
     cu, table = cu_seqlens.to(dev).contiguous(), block_table.to(dev)
     if table.stride(1) != 1:
@@ -269,6 +337,53 @@ def gather_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.
         None if starts is None else starts.data_ptr(), table.stride(0))
     _launch(dev, _lib.load().fp_kv_cache_gather, ctypes.byref(a))
     torch.autograd.graph.increment_version([key, value])
+
+
+@torch.no_grad()
+def gather_cache_reference(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.Tensor,
+                           value: torch.Tensor, cu_seqlens: torch.Tensor, block_table: torch.Tensor,
+                           starts: Optional[torch.Tensor] = None,
+                           k_scale: Optional[torch.Tensor] = None,
+                           v_scale: Optional[torch.Tensor] = None) -> None:
+    """The torch composition of ``gather_cache``, what a trace or a dispatch mode sees
+    of it."""
+    dev, n, B = key.device, key.shape[0], cu_seqlens.numel() - 1
+    nb, bs = key_cache.shape[:2]
+    if key.numel() == 0:
+        return
+    if nb < 1 or bs < 1:
+        raise ValueError("the caches have no pages")
+    room = block_table.shape[1] * bs
+    cu, row = cu_seqlens.long().to(dev), torch.arange(n, device=dev)
+    off = (cu[0] < 0) | (cu[-1] > n) | (cu[1:] < cu[:-1]).any()
+    b = torch.bucketize(row, cu, right=True) - 1
+    written = (b >= 0) & (b < B)
+    b = torch.where(written, b, 0)
+    at = row - cu[b]
+    fits, written = written & ~off, written | off
+    if starts is not None:
+        first = starts.long().to(dev)[b]
+        fits = fits & (first >= 0) & (first < room)
+        at = at + torch.where(fits, first, 0)
+    fits = fits & (at >= 0) & (at < room)
+    at = torch.where(fits, at, 0)
+    if room > 0:
+        page, at = block_table.long().to(dev)[b, at // bs], at % bs
+        page = torch.where(page < 0, page + nb, page)
+        fits = fits & (page >= 0) & (page < nb)
+        page = torch.where(fits, page, 0)
+    else:
+        page = at
+    for y, cache, scale in ((key, key_cache, k_scale), (value, value_cache, v_scale)):
+        x = cache[page, at]
+        if cache.dtype in _FORMATS:
+            x = x.float()
+            if scale is not None:
+                s = scale[page, :, at] if scale.dim() == 3 else scale.to(dev).view(1, -1)
+                x = x * s.unsqueeze(-1)
+            x = x.to(y.dtype)
+        x = x.masked_fill(~fits.view(-1, 1, 1), math.nan)
+        y.copy_(torch.where(written.view(-1, 1, 1), x, y))
 
 
 def paged_decode_attention(query: torch.Tensor, key_cache: torch.Tensor,
@@ -330,8 +445,8 @@ def _paged_kernel_takes(query, key_cache, value_cache, out, cu, used, table, k_s
     trace or dispatch mode to carry along (they see only torch operations)."""
     if not query.is_cuda or query.dtype not in _DTYPES:
         return False
-    if forward_ad._current_level >= 0 or torch._C._functorch.peek_interpreter_stack() is not None \
-            or torch._C._get_tracing_state() is not None or torch._C._len_torch_dispatch_stack() > 0:
+    if forward_ad._current_level >= 0 or _torch_only() or \
+            torch._C._functorch.peek_interpreter_stack() is not None:
         return False
     dev, dt = query.device, query.dtype
     if query.dim() != 3 or out.dim() != 3 or key_cache.dim() != 4 or \
@@ -452,9 +567,7 @@ def paged_attention_reference(query: torch.Tensor, key_cache: torch.Tensor,
 def _pages_fp32(cache: torch.Tensor, blocks: torch.Tensor,
                 scale: Optional[torch.Tensor]) -> torch.Tensor:
     """The pages' values in fp32, (blocks, block_size, Hkv, d)."""
-    if cache.dtype not in _FORMATS:
-        return cache[blocks].float()
-    x = cache.view(torch.uint8)[blocks].view(cache.dtype).float()
+    x = cache[blocks].float()
     if scale is None:
         return x
     if scale.dim() == 3:

@@ -1,0 +1,120 @@
+"""The 8-bit paged KV cache on the GPU where the call is unusual: under traces and dispatch
+modes, in memory of the host, captured where workgroups share the keys."""
+
+import math
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+from torch.utils._python_dispatch import TorchDispatchMode
+
+from tests._kv8 import E4M3, E5M2, MODES, scales
+from flashprefill_amd import vllm_backend as vb
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, HF = torch.bfloat16, torch.float16
+
+
+class _Seen(TorchDispatchMode):
+    def __init__(self):
+        super().__init__()
+        self.ops = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.ops.append(str(func))
+        return func(*args, **(kwargs or {}))
+
+
+def _equal(a, b):
+    """Equal values and signs, NaN (of either sign) where the other has NaN."""
+    if not a.is_floating_point():
+        return torch.equal(a, b)
+    a, b = a.float(), b.float()
+    nan = a.isnan()
+    return torch.equal(nan, b.isnan()) and torch.equal(a[~nan].view(torch.int32),
+                                                       b[~nan].view(torch.int32))
+
+
+def _state(dtype, fmt, mode, page, seed):
+    """Rows (among them zeros, infinities, NaN, the type's largest), slots with padding,
+    caches and scales: what a call of each operator takes."""
+    g = torch.Generator().manual_seed(seed)
+    nb, hkv, d, n = 11, 3, 64, 90
+    k, v = (torch.randn(n, hkv, d, generator=g).to(dtype) for _ in range(2))
+    k[0], k[1, :, 0], k[2, 0, 1], k[3] = 0.0, math.inf, math.nan, torch.finfo(dtype).max
+    slots = torch.randperm(nb * page, generator=g)[:n]
+    slots[5], slots[6] = -1, nb * page
+    c = [torch.zeros(nb, page, hkv, d, dtype=torch.uint8).view(fmt) if fmt in (E4M3, E5M2) else
+         torch.zeros(nb, page, hkv, d, dtype=fmt) for _ in range(2)]
+    sc = [scales(mode, nb, page, hkv, g) for _ in range(2)]
+    cu = torch.tensor([1, 40, 40, 73], dtype=torch.int32)
+    table = torch.randint(-2, nb, (3, 5), generator=g, dtype=torch.int32)
+    table[1, 0] = nb
+    starts = torch.tensor([2, 0, 7], dtype=torch.int32)
+    y = [torch.full((90, hkv, d), 7.0, dtype=dtype) for _ in range(2)]
+    return [None if t is None else t.to(DEV) for t in (k, v, *c, slots, *sc, cu, table, starts, *y)]
+
+
+def _step(k, v, kc, vc, slots, ks, vs, cu, table, starts, y, z):
+    vb.reshape_and_cache(k, v, kc, vc, slots, ks, vs)
+    vb.gather_cache(kc, vc, y, z, cu, table, starts, ks, vs)
+    return y, z
+
+
+def _check_same(mine, other):
+    assert all(a is None or _equal(a, b) for a, b in zip(mine, other))
+
+
+@pytest.mark.parametrize("dtype,fmt,mode", [(t, f, m) for t in (BF, HF) for f in (E4M3, E5M2)
+                                            for m in MODES] + [(BF, BF, "none")])
+def test_a_dispatch_mode_sees_the_write_and_the_read_back(dtype, fmt, mode):
+    for page in (16, 9):
+        kernel, seen = (_state(dtype, fmt, mode, page, 3) for _ in range(2))
+        _step(*kernel)
+        with _Seen() as m:
+            _step(*seen)
+        assert sum("index_put" in o for o in m.ops) >= 2 and sum("copy_" in o for o in m.ops) >= 2
+        _check_same(kernel, seen)
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("fmt,mode", [(E4M3, "slot"), (E5M2, "head"), (E4M3, "none"), (BF, "none")])
+def test_a_trace_replays_the_write_and_the_read_back(fmt, mode):
+    """Both kinds of trace, replayed over other rows, slots and tables."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    none = [i for i, t in enumerate(_state(BF, fmt, mode, 16, 4)) if t is None]
+
+    def step(*args):
+        args = list(args)
+        for i in none:
+            args.insert(i, None)
+        return _step(*args)
+
+    def given(state):
+        return [t for t in state if t is not None]
+
+    traces = [make_fx(step)(*given(_state(BF, fmt, mode, 16, 4)))]
+    traces.append(torch.jit.trace(step, tuple(given(_state(BF, fmt, mode, 16, 4))), check_trace=False))
+    for seed in (5, 6):
+        want = _state(BF, fmt, mode, 16, seed)
+        _step(*want)
+        for trace in traces:
+            mine = _state(BF, fmt, mode, 16, seed)
+            with torch.jit.optimized_execution(False):  # (torch's fuser has no 8-bit floats)
+                trace(*given(mine))
+            _check_same(want, mine)
+
+
+def test_tangents_are_refused():
+    k, v, kc, vc, slots, ks, vs, cu, table, starts, y, z = _state(BF, E4M3, "head", 16, 7)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(ks, torch.ones_like(ks))
+        with pytest.raises(NotImplementedError, match="tangent"):
+            vb.reshape_and_cache(k, v, kc, vc, slots, dual, vs)
+        with pytest.raises(NotImplementedError, match="tangent"):
+            vb.gather_cache(kc, vc, y, z, cu, table, starts, dual, vs)
+        vb.reshape_and_cache(k, v, kc, vc, slots, ks, vs)
+        vb.gather_cache(kc, vc, y, z, cu, table, starts, ks, vs)
+    assert (y[0] == 7.0).all() and not (y[1:40] == 7.0).any()

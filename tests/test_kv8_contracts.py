@@ -1,11 +1,13 @@
 """CPU tests of what the 8-bit KV cache's operators refuse or leave to torch operations."""
 
+import math
 from types import SimpleNamespace
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from tests._kv8 import E4M3, E5M2
+from tests._kv8 import E4M3, E5M2, MODES, quantise, scales, values
 from flashprefill_amd import vllm_backend as vb
 
 BF = torch.bfloat16
@@ -45,3 +47,142 @@ def test_queries_of_8_bits_are_refused_by_an_8_bit_cache(qdtype):
     with pytest.raises(NotImplementedError, match="query"):
         vb.make_forward_v0(cfg, ops)(impl, layer, q, k, k, kv, v0, output=out)
     assert (out == 7.0).all()
+
+
+# ---------------------------------------------------------------------------
+# traces, dispatch modes and forward-mode tangents
+# ---------------------------------------------------------------------------
+
+def _write_case(fmt, mode, seed=0):
+    """Rows with values that a cast can go wrong at, slots of padding, past the cache and
+    none, zeroed caches, scales."""
+    g = torch.Generator().manual_seed(seed)
+    nb, page, hkv, d, n = 5, 6, 3, 24, 22
+    k, v = (torch.randn(n, hkv, d, generator=g).to(BF) for _ in range(2))
+    k[0], k[1, :, 0], k[2, 0, 1], k[3] = 0.0, math.inf, math.nan, torch.finfo(BF).max
+    v[4], v[5, 1], v[6] = -0.0, -math.inf, 2.0 ** -130
+    slots = torch.randperm(nb * page, generator=g)[:n]
+    slots[7], slots[8], slots[9] = -1, nb * page, -100
+    kc, vc = (torch.zeros(nb, page, hkv, d, dtype=torch.uint8).view(fmt) for _ in range(2))
+    ks, vs = (scales(mode, nb, page, hkv, g) for _ in range(2))
+    return k, v, kc, vc, slots, ks, vs
+
+
+@pytest.mark.parametrize("fmt", [E4M3, E5M2])
+@pytest.mark.parametrize("mode", MODES)
+def test_the_composition_of_the_write(fmt, mode):
+    k, v, kc, vc, slots, ks, vs = _write_case(fmt, mode)
+    vb.reshape_and_cache_reference(k, v, kc, vc, slots, ks, vs)
+    for x, c, s in ((k, kc, ks), (v, vc, vs)):
+        fixed = torch.ones(1, 1) if s is None else s.view(1, -1) if mode != "slot" else None
+        codes, found = quantise(x, fmt, fixed)
+        want = torch.zeros(30, 3, 24, dtype=torch.uint8)
+        for t, slot in enumerate(slots.tolist()):
+            if 0 <= slot < 30:
+                want[slot] = codes[t].view(torch.uint8)
+                if mode == "slot":
+                    assert torch.equal(s[slot // 6, :, slot % 6], found[t])
+        assert torch.equal(c.view(torch.uint8).view(30, 3, 24), want)
+
+
+def test_the_composition_of_a_16_bit_write():
+    k, v, kc, vc, slots, _, _ = _write_case(E4M3, "none")
+    kc, vc = torch.zeros(kc.shape, dtype=BF), torch.zeros(kc.shape, dtype=BF)
+    vb.reshape_and_cache_reference(k, v, kc, vc, slots)
+    for x, c in ((k, kc), (v, vc)):
+        want = torch.zeros(30, 3, 24, dtype=BF)
+        for t, slot in enumerate(slots.tolist()):
+            if 0 <= slot < 30:
+                want[slot] = x[t]
+        assert torch.equal(c.view(30, 3, 24).view(torch.int16), want.view(torch.int16))
+
+
+def _read_back_case(fmt, mode, seed=0):
+    """Sequences of none to many tokens, rows before the first and behind the last, a table
+    with pages counted from the end and outside the cache."""
+    g = torch.Generator().manual_seed(seed)
+    nb, page, hkv, d = 9, 4, 2, 16
+    kc, vc = (torch.randn(nb, page, hkv, d, generator=g).to(fmt) for _ in range(2))
+    ks, vs = (None, None) if fmt == BF else (scales(mode, nb, page, hkv, g) for _ in range(2))
+    cu = torch.tensor([2, 9, 9, 12, 13, 15], dtype=torch.int32)
+    table = torch.randint(0, nb, (5, 3), generator=g, dtype=torch.int64)
+    table[0, 1], table[2, 0] = -2, nb
+    starts = torch.tensor([1, 0, 3, -1, 11])  # the fourth before the first token, the last past the room
+    key, value = (torch.full((18, hkv, d), 7.0, dtype=BF) for _ in range(2))
+    return kc, vc, key, value, cu, table, starts, ks, vs
+
+
+def _read_back(cache, scale, rows, cu, table, starts):
+    nb, page = cache.shape[:2]
+    x, want = values(cache, scale), rows.clone()
+    for b in range(cu.numel() - 1):
+        for i in range(int(cu[b + 1]) - int(cu[b])):
+            t = i + (0 if starts is None else int(starts[b]))
+            want[int(cu[b]) + i] = math.nan
+            if t >= 0 and (starts is None or starts[b] >= 0) and t < table.shape[1] * page:
+                p = int(table[b, t // page])
+                if -nb <= p < nb:  # (products of an 8-bit value and a scale in fp32)
+                    want[int(cu[b]) + i] = x[p, t % page].float().to(BF)
+    return want
+
+
+@pytest.mark.parametrize("fmt,mode", [(BF, "none")] + [(f, m) for f in (E4M3, E5M2) for m in MODES])
+@pytest.mark.parametrize("from_first", [True, False])
+def test_the_composition_of_the_read_back(fmt, mode, from_first):
+    kc, vc, key, value, cu, table, starts, ks, vs = _read_back_case(fmt, mode)
+    starts = None if from_first else starts
+    want = [_read_back(c, s, r, cu, table, starts) for c, s, r in ((kc, ks, key), (vc, vs, value))]
+    vb.gather_cache_reference(kc, vc, key, value, cu, table, starts, ks, vs)
+    for got, w in zip((key, value), want):
+        assert torch.equal(got.isnan(), w.isnan()) and torch.equal(got.nan_to_num(), w.nan_to_num())
+    for bad in ([0, 5, 3], [-1, 4, 9], [0, 4, 19]):  # offsets that do not fit: every row
+        vb.gather_cache_reference(kc, vc, key, value, torch.tensor(bad), table, None, ks, vs)
+        assert key.isnan().all() and value.isnan().all()
+    key.fill_(1.0)  # a table without room
+    vb.gather_cache_reference(kc, vc, key, value, torch.tensor([0, 2]), table[:, :0], None, ks, vs)
+    assert key[:2].isnan().all() and (key[2:] == 1.0).all()
+
+
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
+def test_a_trace_holds_the_write_and_the_read_back():
+    """Traced over fake tensors, which have no memory: nothing may reach a kernel."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.fx.experimental.symbolic_shapes import ShapeEnv
+
+    env = ShapeEnv(allow_dynamic_output_shape_ops=True)
+    with FakeTensorMode(shape_env=env, allow_non_fake_inputs=True):
+        x = torch.empty(3, 2, 64, dtype=BF, device="cuda")
+        cache = [torch.empty(4, 16, 2, 64, dtype=torch.uint8, device="cuda").view(E4M3)
+                 for _ in range(2)]
+        sc = [torch.empty(4, 2, 16, device="cuda") for _ in range(2)]
+        slots = torch.empty(3, dtype=torch.int64, device="cuda")
+        cu, table = (torch.empty(s, dtype=torch.int32, device="cuda") for s in ((2,), (1, 4)))
+
+        def step(x, kc, vc, ks, vs, slots, cu, table):
+            y, z = torch.zeros_like(x), torch.zeros_like(x)
+            vb.reshape_and_cache(x, x, kc, vc, slots, ks, vs)
+            vb.gather_cache(kc, vc, y, z, cu, table, None, ks, vs)
+            return y, z
+
+        ops = [str(n.target) for n in make_fx(step)(x, *cache, *sc, slots, cu, table).graph.nodes]
+        with pytest.raises(ValueError, match="of their own"):
+            vb.reshape_and_cache(x, x, cache[0], cache[0], slots, *sc)
+        with pytest.raises(ValueError, match="of their own"):
+            vb.gather_cache(*cache, x, x, cu, table, None, *sc)
+    assert sum("index_put" in o for o in ops) == 4 and sum("copy_" in o for o in ops) == 2
+
+
+def test_tangents_are_refused():
+    # (before anything looks for a GPU)
+    k, v, kc, vc, slots, ks, vs = _write_case(E4M3, "head")
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(k, torch.ones_like(k))
+        with pytest.raises(NotImplementedError, match="tangent"):
+            vb.reshape_and_cache(dual, v, kc, vc, slots, ks, vs)
+        wide = forward_ad.make_dual(vs, torch.ones_like(vs))
+        with pytest.raises(NotImplementedError, match="tangent"):
+            vb.gather_cache(kc, vc, k, v, torch.tensor([0, 3]), torch.zeros(1, 9).int(), None, ks, wide)
+        # tensors without one are taken as ever (and have to be on a GPU)
+        with pytest.raises(ValueError, match="one GPU"):
+            vb.reshape_and_cache(k, v, kc, vc, slots, ks, vs)
