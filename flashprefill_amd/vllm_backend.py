@@ -197,10 +197,10 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.T
     token; the mapping's length is the number of tokens written, negative
     slots are padding and skipped), on the current stream.
 
-    Caches of key's dtype hold the rows as they are. Caches of float8_e4m3fn or
-    float8_e5m2 hold ``x / scale`` rounded to nearest even, what lies beyond the
-    format's largest finite value (infinities too) as that value, NaN as NaN.
-    The fp32 scales are
+    Caches of key's dtype hold the rows as they are, and may lie in pinned memory of
+    the host. Caches of float8_e4m3fn or float8_e5m2 hold ``x / scale`` rounded to
+    nearest even, what lies beyond the format's largest finite value (infinities too)
+    as that value, NaN as NaN. The fp32 scales are
 
     * fixed, and read: one value, or one per KV head (None: 1);
     * one per slot and KV head, ``(num_blocks, Hkv, block_size)``: found from each
@@ -220,7 +220,9 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.T
     if eight:
         _check_no_tangents(key, value, key_cache, value_cache, k_scale, v_scale)
     for t in (key, value, key_cache, value_cache):
-        if not t.is_cuda or t.device != dev:
+        if t.device != dev and not eight and t.device.type == "cpu" and t.is_pinned():
+            continue  # the GPU reads and writes it in place
+        if not key.is_cuda or t.device != dev:
             raise ValueError("key, value and the caches must be on one GPU")
     if eight:
         written = [key_cache, value_cache]

@@ -118,3 +118,23 @@ def test_tangents_are_refused():
         vb.reshape_and_cache(k, v, kc, vc, slots, ks, vs)
         vb.gather_cache(kc, vc, y, z, cu, table, starts, ks, vs)
     assert (y[0] == 7.0).all() and not (y[1:40] == 7.0).any()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_16_bit_caches_in_pinned_memory_of_the_host(dtype):
+    k, v, kc, vc, slots, *_ = _state(dtype, dtype, "none", 16, 8)
+    vb.reshape_and_cache(k, v, kc, vc, slots)
+    host = [torch.zeros(kc.shape, dtype=dtype, pin_memory=True) for _ in range(2)]
+    vb.reshape_and_cache(k, v, *host, slots)
+    torch.cuda.synchronize()
+    assert _equal(host[0], kc.cpu()) and _equal(host[1], vc.cpu()) and kc.any()
+    rows = v.cpu().pin_memory()
+    host[1].zero_()
+    vb.reshape_and_cache(k, rows, *host, slots)
+    torch.cuda.synchronize()
+    assert _equal(host[1], vc.cpu())
+    # memory that the GPU cannot reach, and 8-bit caches, stay refused
+    for c in (torch.zeros(kc.shape, dtype=dtype),
+              torch.zeros(kc.shape, dtype=torch.uint8, pin_memory=True).view(E4M3)):
+        with pytest.raises(ValueError, match="one GPU"):
+            vb.reshape_and_cache(k, v, c, c.clone(), slots)
