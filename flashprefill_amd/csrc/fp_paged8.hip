@@ -712,9 +712,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged8_rows(Paged8Arg
   // (fixed scales: one factor, its sign in q, so that the largest score is that of the
   // largest product)
   const float signed_scale = a.scale_log2 * fixed_scale(pa.ks, h);
-  // (not 0, by which a masked score would be NaN)
+  // (not 0, by which a masked score would be NaN: by 2^-149 no score reaches 2^-21)
   const float scale = kScaled ? signed_scale
-                              : signed_scale == 0.0f ? 0x1p-126f : fabsf(signed_scale);
+                              : signed_scale == 0.0f ? 0x1p-149f : fabsf(signed_scale);
   const uint32_t flip = !kScaled && signed_scale < 0.0f ? 0x80008000u : 0u;
   typename T::vec8 qb[KS];
   {

@@ -8,7 +8,7 @@ import torch
 from torch.autograd import forward_ad
 from torch.utils._python_dispatch import TorchDispatchMode
 
-from tests._kv8 import E4M3, E5M2, MODES, scales
+from tests._kv8 import E4M3, E5M2, MODES, attention, attention_case, bound, scales
 from flashprefill_amd import vllm_backend as vb
 
 pytestmark = pytest.mark.gpu
@@ -138,3 +138,28 @@ def test_16_bit_caches_in_pinned_memory_of_the_host(dtype):
               torch.zeros(kc.shape, dtype=torch.uint8, pin_memory=True).view(E4M3)):
         with pytest.raises(ValueError, match="one GPU"):
             vb.reshape_and_cache(k, v, c, c.clone(), slots)
+
+
+@pytest.mark.parametrize("news", [1, 40, 130])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("zero", ["softmax", "key"])
+def test_a_scale_of_zero_under_scores_near_the_largest(zero, d, news):
+    """Products of up to 2^127 times a scale of 0: every visible key counts alike."""
+    n, hq, hkv = 700, 8, 2
+    args = attention_case([n], [news], hq, hkv, d, 16, BF, E4M3, "tensor", seed=15, width=90)
+    q, kc, _, _, _, _, ks, vs = args
+    q.zero_()
+    q[..., 0] = 2.0 ** 126
+    codes = torch.zeros(kc.shape)
+    codes[..., 0] = torch.tensor([1.5, -1.5])[torch.randint(0, 2, kc.shape[:3])]
+    kc.view(torch.uint8).copy_(codes.to(E4M3).view(torch.uint8))
+    ks.fill_(0.0 if zero == "key" else 1.0)
+    scale = 0.0 if zero == "softmax" else 0.1
+    want, size = attention(*args, scale)
+    dev = [t.to(DEV) for t in args]
+    out = torch.empty(q.shape, dtype=BF, device=DEV)
+    assert vb._paged_kernel_takes(*dev[:3], out, *dev[3:])
+    vb.paged_decode_attention(*dev[:3], out, *dev[3:6], scale, *dev[6:])
+    # (P is off by 2^127 x 2^-149 in its exponent at most: inside bound's fp32 share)
+    off = ((out.cpu().double() - want).abs() / bound(want, size, BF)).max().item()
+    assert off <= 1.0
