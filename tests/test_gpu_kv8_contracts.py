@@ -9,6 +9,7 @@ from torch.autograd import forward_ad
 from torch.utils._python_dispatch import TorchDispatchMode
 
 from tests._kv8 import E4M3, E5M2, MODES, attention, attention_case, bound, scales
+from tests._kv8_paths import path
 from flashprefill_amd import vllm_backend as vb
 
 pytestmark = pytest.mark.gpu
@@ -163,3 +164,63 @@ def test_a_scale_of_zero_under_scores_near_the_largest(zero, d, news):
     # (P is off by 2^127 x 2^-149 in its exponent at most: inside bound's fp32 share)
     off = ((out.cpu().double() - want).abs() / bound(want, size, BF)).max().item()
     assert off <= 1.0
+
+
+@pytest.mark.parametrize("news,d,width,want", [([1, 1, 1], 128, 200, "shared"), ([4, 1, 2], 64, 200, "shared"),
+                                               ([1, 2, 1], 256, 200, "shared"),
+                                               ([40, 33, 60], 128, 200, "rows merged"),
+                                               ([140, 90, 101], 256, 1200, "rows merged")])
+@pytest.mark.parametrize("mode", ["slot", "head"])
+def test_capture_and_replay_where_keys_are_shared(news, d, width, want, mode):
+    """A graph whose call needs a workspace, replayed over lengths that change which
+    workgroups (or chunks) share a row, with the same calls made eagerly in between. Two
+    graphs of one pool, so that their workspaces may be one memory."""
+    hq, hkv, page = 8, 2, 16
+    assert path(sum(news), len(news), hq, hkv, d, page, width) == want
+    lens = [3000, 700, 1500]
+    args = [t.to(DEV) for t in attention_case(lens, news, hq, hkv, d, page, BF, E4M3, mode, seed=21,
+                                              width=width)]
+    q, kc, vc, cu, used, table, ks, vs = args
+    others = [[3000, 700, 1500], [300, 161, 170], [2900, 150, 130], [201, 699, 1499], [1, 0, 1],
+              [2048, 160, 1025]]
+
+    def step(out):
+        vb.paged_decode_attention(q, kc, vc, out, cu, used, table, 1 / math.sqrt(d), ks, vs)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(torch.empty_like(q))
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = [torch.zeros_like(q) for _ in range(2)]
+    for i in range(2):
+        with torch.cuda.graph(graphs[i], pool=None if i == 0 else graphs[0].pool()):
+            step(outs[i])
+    for n in others + others[:2]:
+        used.copy_(torch.tensor(n))
+        q.normal_()
+        mine = torch.zeros_like(q)
+        step(mine)
+        for i in range(2):
+            outs[i].zero_()
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert _equal(outs[i], mine), (n, i)
+    assert mine.isfinite().all() and mine.any()
+
+
+def test_many_rows_of_256_of_one_query_head_each():
+    news, width = [200, 90, 141], 2500
+    assert path(sum(news), 3, 5, 5, 256, 16, width) == "rows merged"
+    for mode in ("head", "slot"):
+        args = attention_case([1900, 120, 700], news, 5, 5, 256, 16, BF, E4M3, mode, seed=22,
+                              width=width)
+        want, size = attention(*args, 1 / 16)
+        dev = [t.to(DEV) for t in args]
+        out = torch.empty(args[0].shape, dtype=BF, device=DEV)
+        assert vb._paged_kernel_takes(*dev[:3], out, *dev[3:])
+        vb.paged_decode_attention(*dev[:3], out, *dev[3:6], 1 / 16, *dev[6:])
+        off = ((out.cpu().double() - want).abs() / bound(want, size, BF)).max().item()
+        assert off <= 1.0

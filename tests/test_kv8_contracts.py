@@ -8,6 +8,7 @@ import torch
 from torch.autograd import forward_ad
 
 from tests._kv8 import E4M3, E5M2, MODES, quantise, scales, values
+from tests._kv8_paths import path
 from flashprefill_amd import vllm_backend as vb
 
 BF = torch.bfloat16
@@ -186,3 +187,22 @@ def test_tangents_are_refused():
         # tensors without one are taken as ever (and have to be on a GPU)
         with pytest.raises(ValueError, match="one GPU"):
             vb.reshape_and_cache(k, v, kc, vc, slots, ks, vs)
+
+
+# ---------------------------------------------------------------------------
+# which kernels the GPU tests' calls take
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("news,hq,hkv,d,page,width,want", [
+    # one query each: short tables, long ones
+    ([1, 1], 8, 2, 128, 16, 57, "whole"), ([1, 1], 8, 2, 128, 16, 64, "whole"),
+    ([1, 1], 8, 2, 128, 16, 65, "shared"), ([1, 1, 1], 8, 2, 64, 16, 200, "shared"),
+    # many rows
+    ([40, 40], 8, 2, 128, 16, 200, "rows merged"), ([40, 40], 8, 2, 64, 16, 200, "rows merged"),
+    ([150, 30, 141], 7, 1, 256, 16, 2500, "rows merged"), ([150, 30, 141], 34, 2, 256, 16, 2500, "rows merged"),
+    ([130, 70], 8, 2, 256, 16, 1200, "rows merged"), ([700], 8, 2, 256, 16, 1200, "rows merged"),
+    # head_dim 256 below 128 rows per sequence, and with so many
+    ([150, 30, 141], 5, 5, 256, 16, 2500, "shared"), ([200, 90, 141], 5, 5, 256, 16, 2500, "rows merged"),
+])
+def test_which_kernels_a_call_takes(news, hq, hkv, d, page, width, want):
+    assert path(sum(news), len(news), hq, hkv, d, page, width) == want
