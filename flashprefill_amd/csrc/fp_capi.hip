@@ -651,12 +651,17 @@ fp::KvCacheArgs cache_args(const fp_kv_cache_args* a) {
 // 300, 32 / 8, 82 and 180; one of 2,000 with 500, 8 / 2 (2^16 triples), 49 and 40; 8 of
 // 3,000 with 16, 32 / 8 (64 rows each), 85 and 77.
 //
-// Few rows: kPaged8Groups workgroups, as many as the card holds at a time, share the keys
-// in units of 128 (more where the units would not count in 31 bits); where the table has
-// room for kWhole keys at most, each segment (16 rows of a KV head's queries) is a
-// workgroup's as a whole. Shared and whole, 32 q / 8 kv heads, d = 128: 1, 32 and 128
-// sequences of 333 tokens 13.8, 18.5 and 37 us and 8.2, 10.5 and 27; of 1,000 tokens 12.3,
-// 23 and 71, and 12.0, 17 and 65; of 2,000 tokens 12.7, 39 and 117, and 18, 32 and 114.
+// Few rows: kPaged8Groups workgroups share the keys in units of 128 (more where the units
+// would not count in 31 bits): two for each CU, what it holds at head_dim 256, and at 128
+// with scales per slot (128 with fixed scales: three, 64: three to four). Where the table
+// has room for kWhole keys at most, each segment (16 rows of a KV head's queries) is a
+// workgroup's as a whole. The host sees the room of the table, not the lengths: short
+// sequences under a table as wide as a model's maximum are shared and merged like long
+// ones, and the rule above takes them for long ones too (the one of 2,000 tokens 48 us
+// under a table of 131,072, 41 under its own). Shared and whole, 32 q / 8 kv heads,
+// d = 128: 1, 32 and 128 sequences of 333 tokens 13.8, 18.5 and 37 us and 8.2, 10.5 and
+// 27; of 1,000 tokens 12.3, 23 and 71, and 12.0, 17 and 65; of 2,000 tokens 12.7, 39 and
+// 117, and 18, 32 and 114.
 PagedSplit paged8_split(const fp_paged_args* a, int* unit, int* groups) {
   constexpr int kWhole = 1024;
   PagedSplit r = paged_split(a);

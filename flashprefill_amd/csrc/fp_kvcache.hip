@@ -17,13 +17,16 @@
 // values (1 where that is 0), written beside the row. x / s is the correctly
 // rounded fp32 quotient, so a code differs from that of the exact quotient only
 // where both lie within 2^-24 of a tie. 2 bytes read and 1 written per element:
-// HBM-bound like the copy (131,072 tokens of 8 heads of 128, 797 MB: 155 us in a row of
-// calls, 5.1 TB/s, where a 1 GiB copy reaches 4.8; 14,500 of 4 heads, 45 MB, 17 us: four
-// rounds of loads per workgroup do not hide each other's latency).
+// HBM-bound like the copy (131,072 tokens of 8 heads of 128, 798 MB: 159 us in a row of
+// calls, 5.0 TB/s, where a plain stream of two reads to a write reaches 6.4). 14,500 tokens
+// of 4 heads, 45 MB: 16 us (7 at that rate). There a workgroup makes one pass, its four
+// loads per thread in flight together, but only once the slots' lookup has passed the
+// barrier, and with 104 registers 1,024 of the 1,821 workgroups run at a time.
 //
 // Read-back (k_kv_cache_gather): row cu[b] + i of key / value is cached token
 // starts[b] + i of sequence b, c * s in fp32 rounded once (a 16-bit cache: its
-// bits). 218,000 tokens of 8 heads of 128, 1.34 GB: 239 us, 5.6 TB/s.
+// bits). 218,000 tokens of 8 heads of 128, 1.34 GB: 239 us, 5.6 TB/s (a plain stream of
+// one read to two writes: 6.0); from a 16-bit cache, 1.78 GB, 326 us, 5.5 TB/s.
 #include "fp_float8.h"
 #include "fp_paged_common.h"
 

@@ -10,15 +10,17 @@
 // per slot the fp32 P of its key. P s_v enters P.V as bf16 parts (fp32's exponents,
 // so nothing underflows) beside c_v as bf16, whatever the type of q.
 //
-// Few rows (k_paged8) are bound by HBM where there are many bytes: 32 sequences of 300 ..
-// 15,000 tokens, 32 q / 8 kv heads of 128, 447 MB of codes in 95 us (4.7 TB/s) and 6.5 for
+// Few rows (k_paged8) are bound by the loads that eight waves per CU have in flight where
+// there are many bytes: 32 sequences of 300 .. 15,000 tokens, 32 q / 8 kv heads of 128,
+// 447 MB of codes in 96 us (4.7 TB/s, where a stream that only reads reaches 7.2) and 7 for
 // the merge; one sequence of 65,000, 137 MB with its scales, 31 and 7; one of 333, 8 us,
 // of which 1.7 are the launch, 1.5 the search for the place of the workgroup and 3.3 the
-// first loads and the end of a segment. Many rows (k_paged8_rows) are bound by MFMA, VALU
-// and LDS alike (about 1,500 cycles each per wave and tile of 64 keys) and by how little
-// the two waves of a SIMD overlap them: 2,048 new tokens of each of 4 sequences of 4,096 ..
-// 6,144 in 728 us, 713 TFLOP/s (1,070 counting both parts of P), MFMA busy 40 % of the
-// time; raised wave priorities around the MFMAs are 0 to 3 % slower.
+// first loads and the end of a segment. Many rows (k_paged8_rows) are bound by MFMA and
+// VALU and by how little the two waves of a SIMD overlap them: 2,048 new tokens of each of
+// 4 sequences of 4,096 .. 6,144 in 730 .. 760 us in a row of calls, about 700 TFLOP/s
+// (1,050 counting both parts of P); of the kernel's cycles MFMA is busy in 49 %, vector
+// instructions issue in 53 % and LDS is busy in 33 %, a quarter of them bank conflicts.
+// Raised wave priorities around the MFMAs are 0 to 3 % slower.
 #include "fp_float8.h"
 #include "fp_paged_common.h"
 
@@ -43,7 +45,9 @@ __device__ __forceinline__ void bf16_parts(float x0, float x1, uint32_t (&u)[N])
 // (sequence, heads, row tile) and every workgroup takes an equal share of the units, whatever segments
 // they belong to: a decode step reads each cached byte once, so equal bytes take equal
 // times, and no workgroup starts for keys that are not there (the host cannot see the
-// lengths without a synchronisation). A segment that is one workgroup's is written out,
+// lengths without a synchronisation). A share is a whole number of units, so that a call of
+// few leaves workgroups without any: 1,620 units are four for each of 405 workgroups of 512,
+// 2,152 five for each of 431, 13,728 twenty-seven for each of 509. A segment that is one workgroup's is written out,
 // the others as partials (O, m, l), the first and the last of a workgroup at most, which
 // k_paged8_merge combines. Where the table has room for few keys, a unit is a whole
 // sequence and a segment a workgroup's: no merge.
@@ -159,7 +163,13 @@ __device__ __forceinline__ Work find_work(const Paged8Args& pa, int wg, int64_t 
 // P16: the page size is a multiple of 16, so a 16-key tile lies in one page: a wave
 // looks up 64 of them at a time, one per lane, and reads a tile's place from its lane.
 // PS: all scales are per slot. Other pages, and scales of which only K's or only V's are
-// per slot, take the general form (neither).
+// per slot, take the general form (neither), which looks up every key's page and scale for
+// itself: the 32 sequences above in pages of 24 take 237 us (354 with scales per slot), in
+// pages of 16 with K's scales per slot and V's fixed 336, where the other forms take 100 to
+// 102 (whole calls).
+//
+// Registers: 119 to 139 at head_dim 64, 161 to 177 at 128, 229 to 256 at 256; 65 to 101
+// scalar ones are kept in lanes of vector registers.
 template <typename T, int F, int D, bool P16, bool PS, int HP>
 __global__ __launch_bounds__(256, 2) void k_paged8(Paged8Args pa) {
   constexpr int KS = D / 32;  // MFMA k-steps over the head dim
@@ -649,17 +659,21 @@ __global__ __launch_bounds__(1024) void k_paged8_merge(Paged8Args pa) {
 // Many rows (prefill over a cached prefix): 128-row tiles as in k_paged_rows, over keys that are
 // widened on their way into LDS. The 64 keys of a tile are loaded into registers
 // (16 keys by each wave, a tile ahead), widened once per workgroup and written as
-// 16-bit tiles, K in q's type and V in bf16; P s_v takes two bf16 parts: 2^-17 of
-// each product, an eighth of what rounding the output to fp16 may lose and a 256th
-// of its cached value's own step, where a third part would add half as many MFMAs
-// to P.V again (one part: a fifth less time).
+// 16-bit tiles, K in q's type and V in bf16; P s_v takes two bf16 parts, 2^-17 of
+// each product: a 64th of what rounding the output to fp16 may lose of its value
+// (2^-11; to bf16 2^-8) and an 8,192nd of what rounding to e4m3 may have lost of the
+// cached one (2^-4; to e5m2 2^-3). A third part, as k_paged8 has it, would add half as
+// many MFMAs to P.V again for errors below these; one part would save a fifth of the
+// time and lose 2^-8 of each product, as much as a bf16 output's rounding.
 //
 // Chunks have the length of the call's longest sequence over its chunk slots. Chunks cut
 // to each sequence, for an equal share of all keys per workgroup, balance the workgroups
 // but split more rows: 118 -> 146 us (512 new of 8,192 tokens), 82 -> 102 (300 new of
 // 5,500 and of 1,200), 157 -> 144 .. 159 (500 new of 6,144, 2,500 and 1,111).
 //
-// D = 256: one workgroup per CU (256 VGPRs and 240 AGPRs, 130 KB of LDS).
+// D = 256: one workgroup per CU (256 VGPRs and 240 AGPRs, 130 KB of LDS), one wave per
+// SIMD: nothing runs beside its softmax. 3 sequences of 5,000 tokens with 600 new ones,
+// 32 q / 4 kv heads: 570 us, 486 TFLOP/s (729 counting both parts of P).
 template <typename T, int F, int D, bool P16, bool PS>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged8_rows(Paged8Args pa) {
   constexpr int KT = 64, TT = KT / 32;
