@@ -156,28 +156,26 @@ def _check_written(*tensors) -> None:
             raise RuntimeError("a tensor to be written requires a gradient: use torch.no_grad()")
 
 
+_tracing_state, _dispatch_modes = torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack
+
+
 def _torch_only() -> bool:
     """Whether a trace or a dispatch mode is on: they see torch operations, not kernels."""
-    return torch._C._get_tracing_state() is not None or torch._C._len_torch_dispatch_stack() > 0
+    return _dispatch_modes() > 0 or _tracing_state() is not None
 
 
 def _check_no_tangents(*tensors) -> None:
     """Refuse forward-mode tangents, which the kernels would drop."""
-    if forward_ad._current_level < 0:
-        return
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise NotImplementedError("a tensor has a forward-mode tangent: the cache's write and "
                                       "read-back have no derivative")
 
 
-def _check_places(what: str, *tensors) -> None:
-    """Refuse tensors to be written that begin at one place. (Tensors without memory, as
-    those of a trace over fake ones, have a storage of their own all the same.)"""
-    at = {t.data_ptr() for t in tensors} if not _torch_only() else \
-        {(t.untyped_storage()._cdata, t.storage_offset()) for t in tensors}
-    if len(at) < len(tensors):
-        raise ValueError(f"{what} must be memory of their own")
+def _place(t: torch.Tensor, torch_only: bool):
+    """Where a tensor begins. (Those without memory, as in a trace over fake tensors, have
+    a storage of their own all the same.)"""
+    return (t.untyped_storage()._cdata, t.storage_offset()) if torch_only else t.data_ptr()
 
 
 def _cache_args(key, value, key_cache, value_cache, slots: int, n: int) -> _lib.FpKvCacheArgs:
@@ -217,20 +215,22 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.T
         raise ValueError(f"key {tuple(key.shape)} / value {tuple(value.shape)} do not match the "
                          f"cache {tuple(key_cache.shape)} and {n} slots")
     dev, eight = key.device, key_cache.dtype in _FORMATS
-    if eight:
+    if eight and forward_ad._current_level >= 0:
         _check_no_tangents(key, value, key_cache, value_cache, k_scale, v_scale)
     for t in (key, value, key_cache, value_cache):
-        if t.device != dev and not eight and t.device.type == "cpu" and t.is_pinned():
-            continue  # the GPU reads and writes it in place
-        if not key.is_cuda or t.device != dev:
+        if t.is_cuda and t.device == dev:
+            continue
+        # (pinned memory of the host the GPU reads and writes in place)
+        if t is key or t.is_cuda or eight or not t.is_pinned():
             raise ValueError("key, value and the caches must be on one GPU")
+    torch_only = _torch_only()
     if eight:
         written = [key_cache, value_cache]
         written += [s for s in (k_scale, v_scale) if s is not None and s.dim() == 3]
         _check_written(*written)
-        if n:
-            _check_places("the caches and the scales to be written", *written)
-    if _torch_only():
+        if n and len({_place(t, torch_only) for t in written}) < len(written):
+            raise ValueError("the caches and the scales to be written must be memory of their own")
+    if torch_only:
         reshape_and_cache_reference(key, value, key_cache, value_cache, slot_mapping, k_scale,
                                     v_scale)
         return
@@ -253,11 +253,12 @@ def reshape_and_cache_reference(key: torch.Tensor, value: torch.Tensor, key_cach
                                 v_scale: Optional[torch.Tensor] = None) -> None:
     """The torch composition of ``reshape_and_cache``, what a trace or a dispatch mode
     sees of it."""
-    bs, dev = key_cache.shape[1], key_cache.device
-    slots = slot_mapping.reshape(-1).long().to(dev)
-    rows = ((slots >= 0) & (slots < key_cache.shape[0] * bs)).nonzero().view(-1)
-    page, at = slots[rows] // bs, slots[rows] % bs
+    bs = key_cache.shape[1]
     for x, cache, scale in ((key, key_cache, k_scale), (value, value_cache, v_scale)):
+        dev = cache.device
+        slots = slot_mapping.reshape(-1).long().to(dev)
+        rows = ((slots >= 0) & (slots < cache.shape[0] * bs)).nonzero().view(-1)
+        page, at = slots[rows] // bs, slots[rows] % bs
         x = x.to(dev)[rows]
         if cache.dtype not in _FORMATS:
             cache[page, at] = x
@@ -308,7 +309,8 @@ def gather_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.
     for name, t in (("cu_seqlens", cu_seqlens), ("block_table", block_table), ("starts", starts)):
         if t is not None and t.dtype not in _INDEX:
             raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
-    _check_no_tangents(key, value, key_cache, value_cache, k_scale, v_scale)
+    if forward_ad._current_level >= 0:
+        _check_no_tangents(key, value, key_cache, value_cache, k_scale, v_scale)
     if not cu_seqlens.is_cuda:  # known without a synchronisation
         at = cu_seqlens.tolist()
         if at[0] < 0 or at[-1] > key.shape[0] or any(x > y for x, y in zip(at, at[1:])):
@@ -317,11 +319,12 @@ def gather_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.
         if not t.is_cuda or t.device != dev:
             raise ValueError("key, value and the caches must be on one GPU")
     _check_written(key, value)
-    if key.numel():
-        _check_places("key and value", key, value)
+    torch_only = _torch_only()
+    if key.numel() and _place(key, torch_only) == _place(value, torch_only):
+        raise ValueError("key and value must be memory of their own")
     if B == 0:
         return
-    if _torch_only():
+    if torch_only:
         gather_cache_reference(key_cache, value_cache, key, value, cu_seqlens, block_table, starts,
                                k_scale, v_scale)
         return
