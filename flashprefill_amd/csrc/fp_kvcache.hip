@@ -28,7 +28,7 @@
 // bits). 218,000 tokens of 8 heads of 128, 1.34 GB: 239 us, 5.6 TB/s (a plain stream of
 // one read to two writes: 6.0); from a 16-bit cache, 1.78 GB, 326 us, 5.5 TB/s.
 #include "fp_float8.h"
-#include "fp_paged_common.h"
+#include "fp_kvcache_common.h"
 
 namespace fp {
 
@@ -60,28 +60,6 @@ hipError_t launch_kv_cache_write(const KvCacheArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(k_kv_cache_write, dim3(static_cast<unsigned>(a.num_tokens)), dim3(256), 0, s,
                      a);
   return hipGetLastError();
-}
-
-// Rows and codes pass once: nontemporal moves (131072 tokens of 8 heads of 128 written:
-// 177 us without them, 169 with them; 218,000 tokens read back 344 and 325). Addresses
-// are of global memory, also where the compiler cannot see it.
-template <typename X>
-__device__ __forceinline__ __attribute__((address_space(1))) X* global_ptr(const void* p) {
-  return (__attribute__((address_space(1))) X*)(p);
-}
-__device__ __forceinline__ uint4 ld16_once(const void* p) {
-  const u32x4 v = __builtin_nontemporal_load(global_ptr<const u32x4>(p));
-  return make_uint4(v[0], v[1], v[2], v[3]);
-}
-__device__ __forceinline__ uint2 ld8_once(const void* p) {
-  const uint64_t v = __builtin_nontemporal_load(global_ptr<const uint64_t>(p));
-  return make_uint2(static_cast<uint32_t>(v), static_cast<uint32_t>(v >> 32));
-}
-__device__ __forceinline__ void st16_once(void* p, uint4 v) {
-  __builtin_nontemporal_store(u32x4{v.x, v.y, v.z, v.w}, global_ptr<u32x4>(p));
-}
-__device__ __forceinline__ void st8_once(void* p, uint2 v) {
-  __builtin_nontemporal_store(static_cast<uint64_t>(v.y) << 32 | v.x, global_ptr<uint64_t>(p));
 }
 
 // A row's quotient x / s, rounded once, without a division per element: with r the
@@ -165,19 +143,6 @@ __device__ __forceinline__ Side choose(bool v, const Side& a, const Side& b) {
               v ? b.scale_head : a.scale_head,
               v ? b.per_slot : a.per_slot,
               v ? b.one : a.one};
-}
-
-// Block and place in it of a slot: a 64-bit division only where the slot needs one
-__device__ __forceinline__ void split_slot(int64_t slot, int32_t block_size, int64_t& blk,
-                                           int64_t& off) {
-  if (slot >> 32) {
-    blk = slot / block_size;
-    off = slot % block_size;
-  } else {
-    const uint32_t q = static_cast<uint32_t>(slot) / static_cast<uint32_t>(block_size);
-    blk = q;
-    off = static_cast<uint32_t>(slot) - q * static_cast<uint32_t>(block_size);
-  }
 }
 
 // U rows of a thread are loaded before the first is used. Their loads have no branch
@@ -321,60 +286,22 @@ hipError_t launch_kv_cache_write8(const Cache8Args& a, int dtype, int format, hi
 }
 
 // F: the cache's format (FP_CACHE_16BIT: T itself). The first wave of a workgroup finds
-// its tokens' sequences (64 at a time, a search over the lanes: a token belongs to the
-// last sequence b with cu[b] <= token, if token < cu[b + 1]) and places, then all
-// waves move their heads.
+// its tokens' places, then all waves move their heads.
 template <typename T, int F, int U>
 __global__ __launch_bounds__(256) void k_kv_cache_gather(GatherArgs a, Sides sides, RowWalk w) {
-  constexpr int64_t kSkip = -1, kNaN = -2;  // rows of no sequence; rows that cannot be read
   __shared__ int64_t s_at[kRowTokens][2], s_sc[kRowTokens][2];
   const KvCacheArgs& c = a.g.c;
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * w.tokens;
   const int n = static_cast<int>(min(static_cast<int64_t>(w.tokens), c.num_tokens - t0));
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x;
-    const int64_t tok = t0 + lane;
-    int64_t b = -1, seq0 = 0;
-    bool off = false;
-    for (int base = 0; base < a.B; base += 64) {
-      int64_t c0 = INT64_MAX, c1 = 0;
-      const bool in = base + lane < a.B;
-      if (in) {
-        c0 = ld_int(a.cu, a.cu64, base + lane);
-        c1 = ld_int(a.cu, a.cu64, base + lane + 1);
-      }
-      off = off || __ballot(in && (c0 < 0 || c1 > c.num_tokens || c1 < c0)) != 0;
-      int last = 0;  // the last of these that begins at or before the token
-#pragma unroll
-      for (int step = 32; step > 0; step >>= 1)
-        if (shfl64(c0, last + step) <= tok) last += step;
-      const int64_t f = shfl64(c0, last), e = shfl64(c1, last);
-      if (f <= tok && tok < e) {
-        b = base + last;
-        seq0 = f;
-      }
-    }
-    int64_t at[2] = {kSkip, kSkip}, sc[2] = {0, 0};
-    if (off) {
-      at[0] = at[1] = kNaN;
-    } else if (b >= 0) {
-      int64_t pos = tok - seq0;
-      const int64_t start = a.starts ? ld_int(a.starts, a.starts64, b) : 0;
-      const int64_t room = static_cast<int64_t>(a.width) * c.block_size;
-      at[0] = at[1] = kNaN;
-      if (start >= 0 && start < room && pos + start < room) {
-        pos += start;
-        int64_t blk, in;
-        split_slot(pos, c.block_size, blk, in);
-        int64_t page = ld_int(a.table, a.table64, b * a.table_stride + blk);
-        if (page < 0) page += a.num_blocks;
-        if (page >= 0 && page < a.num_blocks) {
-          at[0] = page * c.kc_stride_block + in * c.kc_stride_slot;
-          at[1] = page * c.vc_stride_block + in * c.vc_stride_slot;
-          sc[0] = scale_place(a.g.ks, page, in);
-          sc[1] = scale_place(a.g.vs, page, in);
-        }
-      }
+    const CachedToken f = find_cached_token(a, t0 + lane);
+    int64_t at[2] = {f.page, f.page}, sc[2] = {0, 0};
+    if (f.page >= 0) {
+      at[0] = f.page * c.kc_stride_block + f.in * c.kc_stride_slot;
+      at[1] = f.page * c.vc_stride_block + f.in * c.vc_stride_slot;
+      sc[0] = scale_place(a.g.ks, f.page, f.in);
+      sc[1] = scale_place(a.g.vs, f.page, f.in);
     }
     if (lane < n) {
 #pragma unroll
