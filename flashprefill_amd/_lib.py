@@ -36,6 +36,8 @@ EXPORTS = (
     "fp_abi_version", "fp_flashprefill_noalloc", "fp_kv_cache_write", "fp_rope_qk",
     "fp_paged_attention", "fp_paged_workspace_bytes", "fp_kv_cache_write_fp8",
     "fp_kv_cache_gather", "fp_paged_attention_fp8", "fp_paged_fp8_workspace_bytes",
+    "fp_kv_cache_write_int4", "fp_kv_cache_gather_int4", "fp_paged_attention_int4",
+    "fp_paged_int4_workspace_bytes",
 )
 NOALLOC_SCRATCH_BYTES = 96 * 1024 * 1024
 
@@ -160,6 +162,35 @@ class FpPagedFp8Args(ctypes.Structure):
     ]
 
 
+class FpKvGroups(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride_block", ctypes.c_int64),
+                ("stride_head", ctypes.c_int64)]
+
+
+class FpKvCacheInt4Args(ctypes.Structure):
+    _fields_ = [
+        ("base", FpKvCacheArgs), ("k_groups", FpKvGroups), ("v_groups", FpKvGroups),
+        ("k_scale", FpKvScales), ("v_scale", FpKvScales),
+    ]
+
+
+class FpKvGatherInt4Args(ctypes.Structure):
+    _fields_ = [
+        ("cache", FpKvCacheInt4Args), ("batch", ctypes.c_int32), ("table_width", ctypes.c_int32),
+        ("cu_is64", ctypes.c_int32), ("table_is64", ctypes.c_int32),
+        ("starts_is64", ctypes.c_int32),
+        ("cu_seqlens", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+    ]
+
+
+class FpPagedInt4Args(ctypes.Structure):
+    _fields_ = [
+        ("base", FpPagedArgs), ("k_groups", FpKvGroups), ("v_groups", FpKvGroups),
+        ("k_scale", FpKvScales), ("v_scale", FpKvScales),
+    ]
+
+
 _LIB = None
 
 
@@ -192,6 +223,11 @@ def load(path: Path = LIB_PATH) -> ctypes.CDLL:
     lib.fp_paged_attention_fp8.argtypes = [ctypes.POINTER(FpPagedFp8Args), vp, vp]
     lib.fp_paged_fp8_workspace_bytes.argtypes = [ctypes.POINTER(FpPagedFp8Args)]
     lib.fp_paged_fp8_workspace_bytes.restype = ctypes.c_size_t
+    lib.fp_kv_cache_write_int4.argtypes = [ctypes.POINTER(FpKvCacheInt4Args), vp]
+    lib.fp_kv_cache_gather_int4.argtypes = [ctypes.POINTER(FpKvGatherInt4Args), vp]
+    lib.fp_paged_attention_int4.argtypes = [ctypes.POINTER(FpPagedInt4Args), vp, vp]
+    lib.fp_paged_int4_workspace_bytes.argtypes = [ctypes.POINTER(FpPagedInt4Args)]
+    lib.fp_paged_int4_workspace_bytes.restype = ctypes.c_size_t
     lib.fp_search.argtypes = [P, vp, vp, vp, vp]
     lib.fp_select.argtypes = [P, vp, vp, vp, vp]
     lib.fp_read_status.argtypes = [P, vp, vp, ctypes.POINTER(ctypes.c_uint32)]

@@ -662,12 +662,15 @@ fp::KvCacheArgs cache_args(const fp_kv_cache_args* a) {
 // d = 128: 1, 32 and 128 sequences of 333 tokens 13.8, 18.5 and 37 us and 8.2, 10.5 and
 // 27; of 1,000 tokens 12.3, 23 and 71, and 12.0, 17 and 65; of 2,000 tokens 12.7, 39 and
 // 117, and 18, 32 and 114.
-PagedSplit paged8_split(const fp_paged_args* a, int* unit, int* groups) {
+// heads: KV heads of a segment.
+int paged8_heads(const fp_paged_args* a) {
+  return a->head_dim == 64 && a->num_kv_heads % 2 == 0 ? 2 : 1;
+}
+PagedSplit paged8_split(const fp_paged_args* a, int heads, int* unit) {
   constexpr int kWhole = 1024;
   PagedSplit r = paged_split(a);
   *unit = 128;
-  const int pair = a->head_dim == 64 && a->num_kv_heads % 2 == 0 ? 2 : 1;
-  *groups = a->num_kv_heads / pair;
+  const int64_t groups = a->num_kv_heads / heads;
   const int64_t longest = static_cast<int64_t>(a->table_width) * a->block_size;
   const int64_t rows = a->num_tokens * (a->num_q_heads / a->num_kv_heads);
   if (a->head_dim == 256 && rows >= int64_t(128) * a->batch) {
@@ -681,14 +684,14 @@ PagedSplit paged8_split(const fp_paged_args* a, int* unit, int* groups) {
     }
   }
   if (r.many) return r;
-  const int64_t segs = std::max<int64_t>(1, r.tiles * *groups);
+  const int64_t segs = std::max<int64_t>(1, r.tiles * groups);
   const auto units = [&] { return segs * std::max<int64_t>(1, (longest + *unit - 1) / *unit); };
   r.bytes = 0;
   if (longest <= kWhole) *unit = 1 << 30;
   while (*unit < 1 << 30 && units() >= int64_t(1) << 31) *unit *= 2;
   r.nc = static_cast<int>(longest <= kWhole ? segs
                                             : std::min<int64_t>(fp::kPaged8Groups, units()));
-  if (longest > kWhole) r.bytes = static_cast<size_t>(r.nc) * 2 * 16 * pair * (a->head_dim + 2) * 4;
+  if (longest > kWhole) r.bytes = static_cast<size_t>(r.nc) * 2 * 16 * heads * (a->head_dim + 2) * 4;
   return r;
 }
 
@@ -746,6 +749,25 @@ int scales_valid(const fp_kv_scales& s, const char* what) {
     return fail(FP_E_INVALID_ARG, "%s: scales must be 4-byte aligned", what);
   if (s.stride_head < 0 || (s.per_slot && s.stride_block < 0))
     return fail(FP_E_INVALID_ARG, "%s: negative scale strides", what);
+  return FP_OK;
+}
+
+// The split and the argument block of a call over an 8- or 4-bit cache.
+int paged8_args(const fp_paged_args* a, int heads, const fp_kv_scales& ks, const fp_kv_scales& vs,
+                void* ws, fp::Paged8Args* r, PagedSplit* sp) {
+  *sp = paged8_split(a, heads, &r->unit);
+  // (the merge's launch holds fewer than 2^32 threads, 1024 for each head of a segment)
+  if (!sp->many && sp->tiles * a->num_kv_heads >= int64_t(1) << 22)
+    return fail(FP_E_UNSUPPORTED, "paged: %lld tiles of query rows in one call",
+                static_cast<long long>(sp->tiles));
+  if (sp->bytes > 0 && !ws) return fail(FP_E_INVALID_ARG, "paged: workspace is NULL");
+  if (!aligned16(ws)) return fail(FP_E_INVALID_ARG, "paged: workspace must be 16-byte aligned");
+  r->min_share = r->unit == 128 ? 2 : 1;  // (1 and 4 within 1 us of 2, either way)
+  r->groups = a->num_kv_heads / heads;
+  r->segs = sp->tiles * r->groups;
+  r->a = paged_args(a, *sp, ws);
+  r->ks = scales(ks);
+  r->vs = scales(vs);
   return FP_OK;
 }
 
@@ -819,6 +841,124 @@ fp::Cache8Args cache8_args(const fp_kv_cache_args* a, const fp_kv_scales& ks,
   r.ks = scales(ks);
   r.vs = scales(vs);
   return r;
+}
+
+// Which cached tokens a read-back's rows are (A: fp_kv_gather_args or its 4-bit form).
+template <typename A>
+int gather_args(const A* a, int64_t block_size, int64_t num_blocks, fp::GatherArgs* r) {
+  if (a->batch < 1 || a->table_width < 0 || a->table_stride < 0)
+    return fail(FP_E_INVALID_ARG, "kv-gather: sizes out of range");
+  if (!a->cu_seqlens || (!a->block_table && a->table_width > 0))
+    return fail(FP_E_INVALID_ARG, "kv-gather: NULL pointer");
+  if (a->table_width * block_size >= (int64_t(1) << 30))
+    return fail(FP_E_UNSUPPORTED, "kv-gather: 2^30 or more tokens per sequence");
+  r->cu = a->cu_seqlens;
+  r->table = a->block_table;
+  r->starts = a->starts;
+  r->cu64 = a->cu_is64 != 0;
+  r->table64 = a->table_is64 != 0;
+  r->starts64 = a->starts_is64 != 0;
+  r->table_stride = a->table_stride;
+  r->num_blocks = num_blocks;
+  r->B = a->batch;
+  r->width = a->table_width;
+  return FP_OK;
+}
+
+// A 4-bit cache's groups, of which the kernels read pieces of `words` words.
+int groups_valid(const fp_kv_groups& g, const fp_kv_cache_args* a, int words, const char* what) {
+  if (!g.data) return fail(FP_E_INVALID_ARG, "%s: groups are NULL", what);
+  if (reinterpret_cast<uintptr_t>(g.data) % (2 * words) ||
+      !stride_ok(g.stride_block, a->num_blocks, words) ||
+      !stride_ok(g.stride_head, a->num_kv_heads, words))
+    return fail(FP_E_INVALID_ARG, "%s: groups must be aligned to %d words, with strides of "
+                "multiples of %d", what, words, words);
+  return FP_OK;
+}
+
+int fixed_valid(const fp_kv_scales& s, const char* what) {
+  if (s.per_slot) return fail(FP_E_UNSUPPORTED, "%s: a 4-bit cache has fixed scales", what);
+  return scales_valid(s, what);
+}
+
+// The arguments that the 4-bit write and the read-back share.
+int cache4_valid(const fp_kv_cache_int4_args* c, const char* what) {
+  const fp_kv_cache_args* a = &c->base;
+  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256)
+    return fail(FP_E_UNSUPPORTED, "%s: head_dim %d unsupported (64, 128 or 256)", what, a->head_dim);
+  int rc = cache8_valid(a, c->k_scale, c->v_scale, what, 1);
+  if (rc != FP_OK || a->num_tokens == 0) return rc;
+  // (a launch holds fewer than 2^32 threads, four for each row)
+  if (a->num_tokens * a->num_kv_heads >= int64_t(1) << 29)
+    return fail(FP_E_UNSUPPORTED, "%s: %lld tokens of %d heads in one call", what,
+                static_cast<long long>(a->num_tokens), a->num_kv_heads);
+  const int64_t st[6] = {a->kc_stride_block, a->kc_stride_slot, a->kc_stride_head,
+                         a->vc_stride_block, a->vc_stride_slot, a->vc_stride_head};
+  const int64_t n[3] = {a->num_blocks, a->block_size, a->num_kv_heads};
+  for (int i = 0; i < 6; ++i)
+    if (!stride_ok(st[i], n[i % 3], 16))
+      return fail(FP_E_INVALID_ARG, "%s: strides of a 4-bit cache must be multiples of 16", what);
+  if (!aligned16(a->key_cache) || !aligned16(a->value_cache))
+    return fail(FP_E_INVALID_ARG, "%s: the caches must be 16-byte aligned", what);
+  for (const fp_kv_groups* g : {&c->k_groups, &c->v_groups})
+    if ((rc = groups_valid(*g, a, a->head_dim / 32, what)) != FP_OK) return rc;
+  if ((rc = fixed_valid(c->k_scale, what)) != FP_OK) return rc;
+  return fixed_valid(c->v_scale, what);
+}
+
+fp::CacheGroups groups(const fp_kv_groups& g) {
+  return fp::CacheGroups{g.data, g.stride_block, g.stride_head};
+}
+
+fp::Cache4Args cache4_args(const fp_kv_cache_int4_args* c) {
+  const fp_kv_cache_args& a = c->base;
+  const auto side = [](const void* rows, int64_t tok, int64_t head, void* cache, int64_t cb,
+                       int64_t cs, int64_t ch, const fp_kv_groups& g, const fp_kv_scales& s) {
+    return fp::Cache4Side{static_cast<uint16_t*>(const_cast<void*>(rows)), tok, head,
+                          static_cast<uint8_t*>(cache), cb, cs, ch, groups(g), s.data,
+                          s.data ? s.stride_head : 0};
+  };
+  fp::Cache4Args r;
+  r.side[0] = side(a.key, a.k_stride_tok, a.k_stride_head, a.key_cache, a.kc_stride_block,
+                   a.kc_stride_slot, a.kc_stride_head, c->k_groups, c->k_scale);
+  r.side[1] = side(a.value, a.v_stride_tok, a.v_stride_head, a.value_cache, a.vc_stride_block,
+                   a.vc_stride_slot, a.vc_stride_head, c->v_groups, c->v_scale);
+  r.slot_mapping = a.slot_mapping;
+  r.num_slots = a.num_blocks * a.block_size;
+  r.num_tokens = static_cast<int32_t>(a.num_tokens);
+  r.block_size = a.block_size;
+  r.num_kv_heads = a.num_kv_heads;
+  r.head_dim = a.head_dim;
+  return r;
+}
+
+int paged4_valid(const fp_paged_int4_args* a) {
+  if (!a) return fail(FP_E_INVALID_ARG, "paged arguments are NULL");
+  int rc = paged_valid(&a->base);
+  if (rc != FP_OK || a->base.num_tokens == 0) return rc;
+  const fp_paged_args& b = a->base;
+  const int64_t st[6] = {b.kc_stride_block, b.kc_stride_slot, b.kc_stride_head,
+                         b.vc_stride_block, b.vc_stride_slot, b.vc_stride_head};
+  const int64_t n[3] = {b.num_blocks, b.block_size, b.num_kv_heads};
+  for (int i = 0; i < 6; ++i)
+    if (!stride_ok(st[i], n[i % 3], 16))
+      return fail(FP_E_INVALID_ARG, "paged: strides of a 4-bit cache must be multiples of 16");
+  fp_kv_cache_args c{};
+  c.num_blocks = b.num_blocks;
+  c.num_kv_heads = b.num_kv_heads;
+  const int words = b.block_size % 16 == 0 ? 8 : b.head_dim / 32;
+  for (const fp_kv_groups* g : {&a->k_groups, &a->v_groups})
+    if ((rc = groups_valid(*g, &c, words, "paged")) != FP_OK) return rc;
+  if ((rc = fixed_valid(a->k_scale, "paged")) != FP_OK) return rc;
+  return fixed_valid(a->v_scale, "paged");
+}
+
+// A 4-bit call is split as an 8-bit one, but that a segment of few rows serves as many KV
+// heads as make up a cache line of 128 bytes.
+int paged4_heads(const fp_paged_args* a) {
+  int heads = 1;
+  while (heads < 256 / a->head_dim && a->num_kv_heads % (2 * heads) == 0) heads *= 2;
+  return heads;
 }
 
 }  // namespace
@@ -969,8 +1109,8 @@ int fp_paged_attention(const fp_paged_args* a, void* ws, void* stream) {
 }
 
 size_t fp_paged_fp8_workspace_bytes(const fp_paged_fp8_args* a) {
-  int unit, groups;
-  return paged8_valid(a) == FP_OK ? paged8_split(&a->base, &unit, &groups).bytes : 0;
+  int unit;
+  return paged8_valid(a) == FP_OK ? paged8_split(&a->base, paged8_heads(&a->base), &unit).bytes : 0;
 }
 
 int fp_paged_attention_fp8(const fp_paged_fp8_args* a, void* ws, void* stream) {
@@ -978,18 +1118,9 @@ int fp_paged_attention_fp8(const fp_paged_fp8_args* a, void* ws, void* stream) {
   if (rc != FP_OK) return rc;
   if (a->base.num_tokens == 0) return FP_OK;
   fp::Paged8Args r;
-  const PagedSplit sp = paged8_split(&a->base, &r.unit, &r.groups);
-  // (the merge's launch holds fewer than 2^32 threads, 1024 for each head of a segment)
-  if (!sp.many && sp.tiles * a->base.num_kv_heads >= int64_t(1) << 22)
-    return fail(FP_E_UNSUPPORTED, "paged: %lld tiles of query rows in one call",
-                static_cast<long long>(sp.tiles));
-  if (sp.bytes > 0 && !ws) return fail(FP_E_INVALID_ARG, "paged: workspace is NULL");
-  if (!aligned16(ws)) return fail(FP_E_INVALID_ARG, "paged: workspace must be 16-byte aligned");
-  r.min_share = r.unit == 128 ? 2 : 1;  // (1 and 4 within 1 us of 2, either way)
-  r.segs = sp.tiles * r.groups;
-  r.a = paged_args(&a->base, sp, ws);
-  r.ks = scales(a->k_scale);
-  r.vs = scales(a->v_scale);
+  PagedSplit sp;
+  const int prc = paged8_args(&a->base, paged8_heads(&a->base), a->k_scale, a->v_scale, ws, &r, &sp);
+  if (prc != FP_OK) return prc;
   if (!r.vs.slot) {
     r.a.vscale = r.vs.p;
     r.a.vscale_head = r.vs.sh;
@@ -1036,6 +1167,16 @@ int fp_kv_cache_write_fp8(const fp_kv_cache_fp8_args* a, void* stream) {
   return e == hipSuccess ? FP_OK : hip_fail(e, "kv-cache write launch");
 }
 
+int fp_kv_cache_write_int4(const fp_kv_cache_int4_args* a, void* stream) {
+  if (!a) return fail(FP_E_INVALID_ARG, "kv-cache arguments are NULL");
+  const int rc = cache4_valid(a, "kv-cache");
+  if (rc != FP_OK || a->base.num_tokens == 0) return rc;
+  if (!a->base.slot_mapping) return fail(FP_E_INVALID_ARG, "kv-cache: NULL pointer");
+  const hipError_t e = fp::launch_kv_cache_write4(cache4_args(a), a->base.dtype,
+                                                  static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? FP_OK : hip_fail(e, "kv-cache write launch");
+}
+
 int fp_kv_cache_gather(const fp_kv_gather_args* a, void* stream) {
   if (!a) return fail(FP_E_INVALID_ARG, "kv-gather arguments are NULL");
   if (!is_fp8(a->format) && a->format != FP_CACHE_16BIT)
@@ -1043,27 +1184,49 @@ int fp_kv_cache_gather(const fp_kv_gather_args* a, void* stream) {
   const int rc = cache8_valid(&a->base, a->k_scale, a->v_scale, "kv-gather",
                               a->format == FP_CACHE_16BIT ? 2 : 1);
   if (rc != FP_OK || a->base.num_tokens == 0) return rc;
-  if (a->batch < 1 || a->table_width < 0 || a->table_stride < 0)
-    return fail(FP_E_INVALID_ARG, "kv-gather: sizes out of range");
-  if (!a->cu_seqlens || (!a->block_table && a->table_width > 0))
-    return fail(FP_E_INVALID_ARG, "kv-gather: NULL pointer");
-  if (static_cast<int64_t>(a->table_width) * a->base.block_size >= (int64_t(1) << 30))
-    return fail(FP_E_UNSUPPORTED, "kv-gather: 2^30 or more tokens per sequence");
   fp::GatherArgs r;
+  const int grc = gather_args(a, a->base.block_size, a->base.num_blocks, &r);
+  if (grc != FP_OK) return grc;
   r.g = cache8_args(&a->base, a->k_scale, a->v_scale);
-  r.cu = a->cu_seqlens;
-  r.table = a->block_table;
-  r.starts = a->starts;
-  r.cu64 = a->cu_is64 != 0;
-  r.table64 = a->table_is64 != 0;
-  r.starts64 = a->starts_is64 != 0;
-  r.table_stride = a->table_stride;
-  r.num_blocks = a->base.num_blocks;
-  r.B = a->batch;
-  r.width = a->table_width;
   const hipError_t e =
       fp::launch_kv_cache_gather(r, a->base.dtype, a->format, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? FP_OK : hip_fail(e, "kv-gather launch");
+}
+
+int fp_kv_cache_gather_int4(const fp_kv_gather_int4_args* a, void* stream) {
+  if (!a) return fail(FP_E_INVALID_ARG, "kv-gather arguments are NULL");
+  const int rc = cache4_valid(&a->cache, "kv-gather");
+  const fp_kv_cache_args& b = a->cache.base;
+  if (rc != FP_OK || b.num_tokens == 0) return rc;
+  fp::GatherArgs r;
+  const int grc = gather_args(a, b.block_size, b.num_blocks, &r);
+  if (grc != FP_OK) return grc;
+  r.g = cache8_args(&b, a->cache.k_scale, a->cache.v_scale);
+  const hipError_t e = fp::launch_kv_cache_gather4(cache4_args(&a->cache), r, b.dtype,
+                                                   static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? FP_OK : hip_fail(e, "kv-gather launch");
+}
+
+size_t fp_paged_int4_workspace_bytes(const fp_paged_int4_args* a) {
+  int unit;
+  return paged4_valid(a) == FP_OK ? paged8_split(&a->base, paged4_heads(&a->base), &unit).bytes : 0;
+}
+
+int fp_paged_attention_int4(const fp_paged_int4_args* a, void* ws, void* stream) {
+  int rc = paged4_valid(a);
+  if (rc != FP_OK || a->base.num_tokens == 0) return rc;
+  const int heads = paged4_heads(&a->base);
+  fp::Paged4Args r;
+  PagedSplit sp;
+  if ((rc = paged8_args(&a->base, heads, a->k_scale, a->v_scale, ws, &r.p, &sp)) != FP_OK) return rc;
+  r.p.a.vscale = r.p.vs.p;
+  r.p.a.vscale_head = r.p.vs.sh;
+  r.kg = groups(a->k_groups);
+  r.vg = groups(a->v_groups);
+  r.dtype = a->base.dtype;
+  const hipError_t e = fp::launch_paged4(r, a->base.head_dim, heads, sp.many, sp.tiles,
+                                         static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? FP_OK : hip_fail(e, "paged attention launch");
 }
 
 int fp_read_status(const fp_problem* p, void* ws, void* stream, uint32_t* status) {

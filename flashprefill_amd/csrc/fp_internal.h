@@ -226,6 +226,37 @@ struct GatherArgs {
   int32_t B, width;
 };
 
+// Words of a 4-bit cache's groups: head_dim / 32 of a slot at p[block * sb + head * sh +
+// slot * (head_dim / 32)].
+struct CacheGroups {
+  uint16_t* p;
+  int64_t sb, sh;
+};
+
+// Attention over a paged 4-bit cache (fp_paged4.hip)
+struct Paged4Args {
+  Paged8Args p;  // (ks, vs: fixed)
+  CacheGroups kg, vg;
+  int32_t dtype;
+};
+
+// Write of a 4-bit cache and its read-back (fp_kvcache4.hip), K in side[0], V in side[1].
+struct Cache4Side {
+  uint16_t* rows;  // 16-bit rows, read by the write, written by the read-back
+  int64_t row_tok, row_head;
+  uint8_t* cache;
+  int64_t block, slot, head;
+  CacheGroups g;
+  const float* t;  // nullable
+  int64_t t_head;
+};
+struct Cache4Args {
+  Cache4Side side[2];
+  const int64_t* slot_mapping;
+  int64_t num_slots;
+  int32_t num_tokens, block_size, num_kv_heads, head_dim;
+};
+
 constexpr int kRopeMaxBatch = 64;  // sequences whose offsets k_rope takes
 
 struct RopeArgs {
@@ -269,6 +300,13 @@ hipError_t launch_paged8(const Paged8Args& a, int dtype, int format, int head_di
 hipError_t launch_kv_cache_write8(const Cache8Args& a, int dtype, int format, hipStream_t s);
 hipError_t launch_kv_cache_gather(const GatherArgs& a, int dtype, int format, hipStream_t s);
 hipError_t launch_kv_cache_write(const KvCacheArgs& a, hipStream_t s);
+hipError_t launch_kv_cache_write4(const Cache4Args& a, int dtype, hipStream_t s);
+// (find: the call's sequences and pages)
+hipError_t launch_kv_cache_gather4(const Cache4Args& a, const GatherArgs& find, int dtype,
+                                   hipStream_t s);
+// hp: KV heads of a segment
+hipError_t launch_paged4(const Paged4Args& a, int head_dim, int hp, bool rows, int64_t tiles,
+                         hipStream_t s);
 hipError_t launch_pool(const PoolArgs& a, int dtype, int head_dim, int64_t grid, hipStream_t s);
 // k_plan then k_pool as one launch (batch <= kSmallPlanBatch)
 hipError_t launch_plan_pool(const PlanArgs& pa, const PoolArgs& a, const FullRowsArgs& f, int dtype,

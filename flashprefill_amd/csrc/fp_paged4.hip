@@ -1,0 +1,834 @@
+// Attention over a paged KV cache of 4-bit integers: the 4-bit form of fp_paged8.hip (the
+// same rows, shares, partials and merges). Cached element x of a key or value is
+// s (c + z) t: exactly an fp16 number u = s (c + z) (fp_int4.h) times the KV head's scale.
+//
+//   S = scale t_k (q . u_k),  P = exp2(S - m),  O = t_v sum P u_v / sum P
+//
+// No cached value is rounded on the way: u enters v_mfma_f32_*_f16 as it is, whatever the
+// type of q. bf16 queries become fp16 ones times a power of two f that takes their row's
+// largest finite element to 2^13 .. 2^14: exactly, but for elements below 2^-39 of it,
+// whose last bits fp16's subnormals lose. P enters as P 2^15 (few rows: two fp16 parts, the
+// second of what the first lost), of which fp16 holds all above 2^-39 of m's exponent.
+#include "fp_int4.h"
+#include "fp_paged_segments.h"
+
+namespace fp {
+
+constexpr float kPScale = 15.0f;  // few rows: log2 of the factor of P
+
+// 8 elements of a query row, dims 0 .. 7 as fp16 numbers in the order {0, 2, 1, 3, 4, 6, 5,
+// 7} of a key's piece (piece_group), times f
+__device__ __forceinline__ uint4 query8(uint4 x, bool bf, float f) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  if (!bf && f > 0.0f) {
+    return make_uint4(halves<0>(w[0], w[1]), halves<1>(w[0], w[1]), halves<0>(w[2], w[3]),
+                      halves<1>(w[2], w[3]));
+  }
+  float y[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    y[2 * e] = f * (bf ? __uint_as_float(w[e] << 16) : F16::to_f32(static_cast<uint16_t>(w[e])));
+    y[2 * e + 1] = f * (bf ? __uint_as_float(w[e] & 0xffff0000u)
+                           : F16::to_f32(static_cast<uint16_t>(w[e] >> 16)));
+  }
+  return make_uint4(pack2<F16>(y[0], y[2]), pack2<F16>(y[1], y[3]), pack2<F16>(y[4], y[6]),
+                    pack2<F16>(y[5], y[7]));
+}
+// largest finite magnitude of 8 bf16 elements and m
+__device__ __forceinline__ float most8(uint4 x, float m) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float a = fabsf(__uint_as_float(w[e] << 16));
+    const float b = fabsf(__uint_as_float(w[e] & 0xffff0000u));
+    m = fmaxf(m, a < INFINITY ? a : 0.0f);
+    m = fmaxf(m, b < INFINITY ? b : 0.0f);
+  }
+  return m;
+}
+// log2 of a bf16 row's factor; rows below 2^-106 keep that of 2^-106
+__device__ __forceinline__ int row_exponent(float most) {
+  return 13 - max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -106);
+}
+__device__ __forceinline__ uint16_t round16(float x, bool bf) {
+  return bf ? BF16::from_f32(x) : F16::from_f32(x);
+}
+__device__ __forceinline__ uint32_t round2(float a, float b, bool bf) {
+  return bf ? pack2<BF16>(a, b) : pack2<F16>(a, b);
+}
+
+// a key's dot product with a lane's share of a query row: groups of a piece, in fp32
+template <int NB>
+__device__ __forceinline__ float piece_dot(const uint32_t (&w)[NB], const uint32_t (&gw)[NB / 2],
+                                           const f16x8 (&q)[NB], const Int4Consts& k) {
+  float d = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const f16x8 u = as_vec8<F16>(piece_group<NB>(w, gw, j, k));
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      d = fmaf(static_cast<float>(q[j][e]), static_cast<float>(u[e]), d);
+  }
+  return d;
+}
+
+// ---------------------------------------------------------------------------
+// Few rows
+// ---------------------------------------------------------------------------
+// As k_paged8: four waves take 32 keys in turn, a round ahead of their use, straight from
+// the pages into registers.
+//
+//   S^T (keys x rows) = K . Q^T on v_mfma_f32_16x16x32_f16: lane (r = l % 16, g = l / 16)
+//     loads piece g of key r, whose group j is the operand of k-step j
+//   O^T (dims x rows) += V^T . P^T: k index 8 g + 4 t + v is key 16 t + 4 g + v, row m of
+//     MFMA 2 j + p is dim 32 j + 2 m + p, nibble p of byte j of the D / 32 that lane m
+//     loads of each of its 8 keys
+//
+// HP: KV heads of a segment, each served by 4 / HP waves, so that whole cache lines are
+// one segment's.
+//
+// P16: the page size is a multiple of 16, so a 16-key tile lies in one page: a wave looks
+// up 64 of them at a time, one per lane, and reads a tile's place from its lane. Other
+// pages look up every key's.
+template <int D, bool P16, int HP>
+__global__ __launch_bounds__(256, 2) void k_paged4(Paged4Args pa4) {
+  constexpr int NB = D / 32;  // groups, MFMA k-steps over the head dim
+  constexpr int GW = NB / 2;  // words of 32 bits of a key's groups
+  constexpr int E = D / 16;
+  constexpr int VW = NB < 4 ? 1 : NB / 4;  // words of 32 bits of V's bytes per lane and key
+  constexpr int OS = D + 4;   // padded row of the merge buffer (floats)
+  constexpr int NW = 4 / HP;  // waves of a head
+  constexpr int RK = 32 * NW;  // keys of a round, all waves of a head
+  __shared__ float sm[4][16][OS];
+  __shared__ float sml[4][16][2];
+  const Paged8Args& pa = pa4.p;
+  const PagedArgs& a = pa.a;
+  const Work work = find_work(pa, static_cast<int>(blockIdx.x), -1);
+  if (work.b < 0) return;
+  const Int4Consts k4;
+  const bool bf = pa4.dtype == FP_DTYPE_BF16;
+  const int t = threadIdx.x, lane = t & 63;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int hw = w / NW, kw = w % NW;  // the wave's head of the segment, and its turn
+  const int r16 = lane & 15, g = lane >> 4;
+  int b = work.b;
+  PagedSeq sq = work.s;
+  const int start = static_cast<int>(blockIdx.x) * work.share;
+  int left = min(work.share, work.total - start);
+  int tiles = seq_tiles(a, sq), units = seq_units(pa.unit, sq);
+  int seg = __builtin_amdgcn_readfirstlane((start - work.units) / units);
+  int u = start - work.units - seg * units;
+  for (bool first = true;; first = false) {
+    const int hg = __builtin_amdgcn_readfirstlane(seg / tiles), tl = seg - hg * tiles;
+    const int h = hg * HP + hw;
+    const int take = min(units - u, left);
+    const bool single = take == units;
+    const int nk = static_cast<int>(sq.nk), nq = sq.nq;
+    const int k0 = u * pa.unit;
+    const int k1 = single ? nk : min(k0 + take * pa.unit, nk);
+
+    // this lane's query row (B operand column), its factor and its last visible key
+    const int rr = tl * 16 + r16;
+    const bool rvalid = rr < nq * a.G;
+    const int qi = rvalid ? rr / a.G : 0;
+    const int lim = rvalid ? nk - nq + qi : nk - 1;
+    f16x8 qb[NB];
+    float scale = a.scale_log2 * fixed_scale(pa.ks, h);
+    {
+      const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (sq.q0 + qi) * a.qst +
+                           static_cast<int64_t>(h * a.G + (rvalid ? rr % a.G : 0)) * a.qhs + 8 * g;
+      uint4 x[NB];
+      float most = 0.0f;
+#pragma unroll
+      for (int j = 0; j < NB; ++j) x[j] = rvalid ? ld16(qp + 32 * j) : zero4();
+      float f = 1.0f;
+      if (bf) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) most = most8(x[j], most);
+        const int e = row_exponent(row4_max(most));
+        f = __builtin_amdgcn_ldexpf(1.0f, e);
+        scale *= __builtin_amdgcn_ldexpf(1.0f, -e);
+      }
+#pragma unroll
+      for (int j = 0; j < NB; ++j) qb[j] = as_vec8<F16>(query8(x[j], bf, f));
+    }
+
+    f32x4 acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = f32x4{};
+    float m_run = -INFINITY, l_part = 0.0f;
+    bool bad = false;
+    const int64_t row = static_cast<int64_t>(b) * a.table_stride;
+    const uint8_t* kc = static_cast<const uint8_t*>(a.kc) + static_cast<int64_t>(h) * a.kch;
+    const uint8_t* vc = static_cast<const uint8_t*>(a.vc) + static_cast<int64_t>(h) * a.vch;
+    const uint16_t* kg = pa4.kg.p + h * pa4.kg.sh;
+    const uint16_t* vg = pa4.vg.p + h * pa4.vg.sh;
+
+    // what a round loads: 32 keys, lanes as above
+    struct {
+      uint32_t k[2][NB], kg[2][GW];
+      uint32_t v[2][4][VW], vg[2][4 * GW];
+    } r;
+    // places of the 64 16-key tiles from key `win`, one per lane (P16; tiles past the
+    // sequence repeat the last one, their scores are masked)
+    int win = k0;
+    int64_t kat = 0, vat = 0, kgat = 0, vgat = 0;
+    const int last16 = (nk - 1) & ~15;
+    auto look = [&](int from) {
+      win = from;
+      const int key = min(from + 16 * lane, last16);
+      const int64_t pg = paged_page<false>(a, row, key, bad);
+      const int in = a.bs_shift >= 0 ? key & (a.bs - 1) : key % a.bs;
+      kat = pg * a.kcb + in * a.kcs;
+      vat = pg * a.vcb + in * a.vcs;
+      kgat = pg * pa4.kg.sb + in * NB;
+      vgat = pg * pa4.vg.sb + in * NB;
+    };
+    auto place = [&](int64_t x, int tile) {
+      return static_cast<int64_t>(
+          static_cast<uint64_t>(static_cast<uint32_t>(
+              __builtin_amdgcn_readlane(static_cast<int>(x >> 32), tile))) << 32 |
+          static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), tile)));
+    };
+    // a lane's offsets in a tile
+    const uint32_t koff = static_cast<uint32_t>(r16 * static_cast<int>(a.kcs) + 4 * NB * g);
+    uint32_t voff[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      voff[v] = static_cast<uint32_t>((4 * g + v) * static_cast<int>(a.vcs) + NB * r16);
+    auto load_k = [&](int base) {
+      if constexpr (P16) {
+        if (base >= win + 1024) look(k0 + ((base - k0) & ~1023));
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if constexpr (P16) {
+          const int tile = ((base - win) >> 4) + j;
+          load_piece<NB>(kc + place(kat, tile) + koff, r.k[j]);
+          load_words<NB>(kg + place(kgat, tile) + r16 * NB, r.kg[j]);
+        } else {
+          const int key = min(base + 16 * j + r16, nk - 1);
+          const int64_t pg = paged_page<false>(a, row, key, bad);
+          const int in = key % a.bs;
+          load_piece<NB>(kc + pg * a.kcb + static_cast<int64_t>(in) * a.kcs + 4 * NB * g, r.k[j]);
+          load_words<NB>(kg + pg * pa4.kg.sb + static_cast<int64_t>(in) * NB, r.kg[j]);
+        }
+      }
+    };
+    auto load_v = [&](int base) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int tile = ((base - win) >> 4) + j;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const uint8_t* p;
+          if constexpr (P16) {
+            p = vc + place(vat, tile) + voff[v];
+          } else {
+            const int key = min(base + 16 * j + 4 * g + v, nk - 1);
+            const int64_t pg = paged_page<false>(a, row, key, bad);
+            const int in = key % a.bs;
+            p = vc + pg * a.vcb + static_cast<int64_t>(in) * a.vcs + NB * r16;
+            uint32_t x[GW];
+            load_words<NB>(vg + pg * pa4.vg.sb + static_cast<int64_t>(in) * NB, x);
+#pragma unroll
+            for (int q = 0; q < GW; ++q) r.vg[j][GW * v + q] = x[q];
+          }
+          if constexpr (NB == 2) {
+            r.v[j][v][0] = *reinterpret_cast<const uint16_t*>(p);
+          } else if constexpr (NB == 4) {
+            r.v[j][v][0] = *reinterpret_cast<const uint32_t*>(p);
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(p);
+            r.v[j][v][0] = x.x; r.v[j][v][1] = x.y;
+          }
+        }
+        if constexpr (P16) load_words<4 * NB>(vg + place(vgat, tile) + 4 * g * NB, r.vg[j]);
+      }
+    };
+    f32x4 s[2];
+    auto scores = [&]() {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        s[j] = f32x4{};
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+          s[j] = mfma16(as_vec8<F16>(piece_group<NB>(r.k[j], r.kg[j], i, k4)), qb[i], s[j]);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s[j][v] *= scale;
+      }
+    };
+    auto softmax_pv = [&](int base) {
+      if (base + 31 > nk - nq) {  // some row's causal limit or the end lies in this round
+        asm volatile("");  // (a branch: as selects they would be in every round)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int key = base + 16 * j + 4 * g + v;
+            if (key > lim) s[j][v] = -INFINITY;
+            if (key >= nk) {  // slots past the end may hold anything: a step of 0
+#pragma unroll
+              for (int q = 0; q < GW; ++q) r.vg[j][GW * v + q] = 0u;
+            }
+          }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) mx = fmaxf(mx, s[j][v]);
+      const float m_new = fmaxf(m_run, row4_max(mx));
+      if (__ballot(m_new > m_run) != 0) {
+        // rows with no visible key yet keep m = -inf: their factors are 0
+        const float ms = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m_run - ms);
+        m_run = m_new;
+        l_part *= alpha;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) acc[e][v] *= alpha;
+      }
+      const float ms = m_run == -INFINITY ? 0.0f : m_run - kPScale;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          s[j][v] = __builtin_amdgcn_exp2f(s[j][v] - ms);
+          l_part += s[j][v];
+        }
+      uint32_t hi[4], lo[4];  // keys 2 i, 2 i + 1 of this lane
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x0 = s[i >> 1][2 * (i & 1)], x1 = s[i >> 1][2 * (i & 1) + 1];
+        hi[i] = pack2<F16>(x0, x1);
+        lo[i] = pack2<F16>(x0 - F16::to_f32(static_cast<uint16_t>(hi[i])),
+                           x1 - F16::to_f32(static_cast<uint16_t>(hi[i] >> 16)));
+      }
+      const f16x8 ph = as_vec8<F16>(make_uint4(hi[0], hi[1], hi[2], hi[3]));
+      const f16x8 pl = as_vec8<F16>(make_uint4(lo[0], lo[1], lo[2], lo[3]));
+#pragma unroll
+      for (int q = 0; q < GW; ++q) {  // groups 2 q and 2 q + 1
+        uint32_t hv[4];
+        Step2 st[2][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // a pair of keys
+          const int jt = i >> 1, va = 2 * (i & 1);
+          const uint32_t xa = r.v[jt][va][q >> 1], xb = r.v[jt][va + 1][q >> 1];
+          hv[i] = q & 1 ? halves<1>(xa, xb) : halves<0>(xa, xb);
+          const uint32_t ga = r.vg[jt][GW * va + q], gb = r.vg[jt][GW * (va + 1) + q];
+          st[0][i] = steps(halves<0>(ga, gb), k4);
+          st[1][i] = steps(halves<1>(ga, gb), k4);
+        }
+        auto pv = [&](auto nc) {
+          constexpr int N = decltype(nc)::value;
+          uint32_t x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = values2<N>(hv[i], st[N >> 1][i], k4);
+          const f16x8 va = as_vec8<F16>(make_uint4(x[0], x[1], x[2], x[3]));
+          acc[4 * q + N] = mfma16(va, pl, acc[4 * q + N]);
+          acc[4 * q + N] = mfma16(va, ph, acc[4 * q + N]);
+        };
+        pv(IntC<0>{});
+        pv(IntC<1>{});
+        pv(IntC<2>{});
+        pv(IntC<3>{});
+      }
+    };
+
+    // A round's keys are loaded while the one before is used, its values after that: the
+    // last round, which loads nothing, stands apart, since with the loads under a branch
+    // the compiler waits for all of them at the next use. The steps are kept in order.
+    int base = k0 + 32 * kw;
+    if (base < k1) {
+      if constexpr (P16) look(k0);
+      load_k(base);
+      load_v(base);
+      for (; base + RK < k1; base += RK) {
+        scores();
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(base + RK);
+        __builtin_amdgcn_sched_barrier(0);
+        softmax_pv(base);
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(base + RK);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      scores();
+      softmax_pv(base);
+    }
+
+    // O not finite (a group of NaN; finite values cannot overflow: P 2^15 times 2^15 times
+    // 2^30 keys): P.V again over the keys that each row sees, since a masked key's NaN
+    // times P = 0 is NaN
+    {
+      float nf = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) nf = fmaf(acc[e][v], 0.0f, nf);
+      if (__ballot(nf != 0.0f) != 0) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = f32x4{};
+        const float ms = m_run == -INFINITY ? 0.0f : m_run - kPScale;
+        int lane2 = static_cast<int>(threadIdx.x);  // (formed here, not kept across the loop)
+        asm volatile("" : "+v"(lane2));
+        const int g2 = (lane2 >> 4) & 3;
+#pragma unroll 1
+        for (int i = 0; i < 32 * ((k1 - k0 + RK - 1) / RK); ++i) {
+          const int key = k0 + 32 * kw + RK * (i >> 5) + (i & 31);
+          if (key >= k1) break;
+          const int64_t pg = paged_page<true>(a, row, key, bad);
+          const int64_t in = key % a.bs;
+          uint32_t x[NB], gw[GW];
+          load_piece<NB>(kc + pg * a.kcb + in * a.kcs + 4 * NB * g2, x);
+          load_words<NB>(kg + pg * pa4.kg.sb + in * NB, gw);
+          const float d = row4_sum(piece_dot<NB>(x, gw, qb, k4)) * scale;
+          if (key > lim) continue;
+          const float p = __builtin_amdgcn_exp2f(d - ms);
+          load_piece<NB>(vc + pg * a.vcb + in * a.vcs + 4 * NB * g2, x);
+          load_words<NB>(vg + pg * pa4.vg.sb + in * NB, gw);
+#pragma unroll
+          for (int j = 0; j < NB; ++j) {
+            // dims 32 j + 8 g + {0, 2, 1, 3, 4, 6, 5, 7}: dim 2 v + p of the eight is
+            // acc[2 j + p][v]
+            const f16x8 y = as_vec8<F16>(piece_group<NB>(x, gw, j, k4));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int v = 2 * (e >> 2) + (e & 1), pp = (e >> 1) & 1;
+              acc[2 * j + pp][v] = fmaf(p, static_cast<float>(y[e]), acc[2 * j + pp][v]);
+            }
+          }
+        }
+      }
+    }
+
+    // acc[2 j + p][v] is dim 32 j + 8 g + 2 v + p of row r16
+    float l = row4_sum(l_part);
+    if (__ballot(bad) != 0) l = __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int v = 0; v < 4; v += 2)
+        *reinterpret_cast<float4*>(&sm[w][r16][32 * j + 8 * g + 2 * v]) =
+            make_float4(acc[2 * j][v], acc[2 * j + 1][v], acc[2 * j][v + 1], acc[2 * j + 1][v + 1]);
+    if (g == 0) {
+      sml[w][r16][0] = m_run;
+      sml[w][r16][1] = l;
+    }
+    __syncthreads();
+    const int orow = t >> 4, od = E * (t & 15);
+    const int orr = tl * 16 + orow;
+    if (orr < nq * a.G) {
+#pragma unroll
+      for (int x = 0; x < HP; ++x) {
+        float M = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < NW; ++k) M = fmaxf(M, sml[x * NW + k][orow][0]);
+        float L = 0.0f, o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NW; ++k) {
+          const float mk = sml[x * NW + k][orow][0], lk = sml[x * NW + k][orow][1];
+          // (a quarter each: as k_paged8 leaves them to the merge)
+          const float f = mk == -INFINITY ? 0.0f : 0.25f * __builtin_amdgcn_exp2f(mk - M);
+          // (a wave without keys has m = -inf and l = 0; NaN scores leave m = -inf
+          // with l = NaN, which the sum keeps)
+          L += mk == -INFINITY ? lk : f * lk;
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] += f * sm[x * NW + k][orow][od + e];
+        }
+        if (single) {
+          const int ho = hg * HP + x;
+          const int64_t tok = sq.q0 + orr / a.G;
+          const int hq = ho * a.G + orr % a.G;
+          uint16_t* op =
+              static_cast<uint16_t*>(a.o) + tok * a.ost + static_cast<int64_t>(hq) * a.ohs + od;
+          const float rcp = 1.0f / L, vs = fixed_scale(pa.vs, ho);
+          uint32_t pk[E / 2];
+#pragma unroll
+          for (int q = 0; q < E / 2; ++q) {
+            float lo = o[2 * q] * rcp * vs, hi = o[2 * q + 1] * rcp * vs;
+            if (nk == 0) lo = hi = sq.bad ? __uint_as_float(0x7fc00000u) : 0.0f;
+            pk[q] = round2(lo, hi, bf);
+          }
+#pragma unroll
+          for (int q = 0; q < E / 2; q += 2)
+            *reinterpret_cast<uint2*>(op + 2 * q) = make_uint2(pk[q], pk[q + 1]);
+        } else {
+          const int64_t part =
+              ((2 * static_cast<int64_t>(blockIdx.x) + !first) * HP + x) * 16 + orow;
+          float* pp = a.part + part * D + od;
+#pragma unroll
+          for (int e = 0; e < E; e += 4)
+            *reinterpret_cast<float4*>(pp + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          if ((t & 15) == 0) {
+            a.ml[2 * part] = M;
+            a.ml[2 * part + 1] = L;
+          }
+        }
+      }
+    }
+    left -= take;
+    if (left <= 0) return;
+    u = 0;
+    if (++seg == tiles * pa.groups) {  // the next sequence with rows (there are units left)
+      seg = 0;
+      do sq = uniform_seq(paged_seq(a, ++b));
+      while (sq.nq == 0);
+      tiles = seq_tiles(a, sq);
+      units = seq_units(pa.unit, sq);
+    }
+    __syncthreads();  // (the merge buffer)
+  }
+}
+
+template <typename T, int D, int HP>
+__global__ __launch_bounds__(1024) void k_paged4_merge(Paged8Args pa) {
+  merge_segments<T, D, HP>(pa);
+}
+
+// Many rows (prefill over a cached prefix): 128-row tiles as in k_paged8_rows. The 64 keys
+// of a tile are loaded into registers (16 keys by each wave, four lanes to a key, a tile
+// ahead), made fp16 numbers once per workgroup and written to LDS, in which the dims of
+// every eight lie in the order of a piece ({0, 2, 1, 3, 4, 6, 5, 7}); so do the queries',
+// and O's come out in it. P 2^7 (at most 2^15, see kStep) is rounded to fp16 once: 2^-11 of
+// each product, as much as rounding the output to fp16 may lose (to bf16 2^-8) and less than
+// a fiftieth of what rounding to 4 bits lost of the cached value; a second part would add
+// half as many MFMAs to P.V again.
+template <int D, bool P16>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged4_rows(Paged4Args pa4) {
+  constexpr int KT = 64, TT = KT / 32;
+  constexpr int KS = D / 16, DT = D / 32, CH = D / 8;
+  constexpr int NB = D / 32, GW = NB / 2;
+  constexpr float kStep = 8.0f, kPScaleRows = 7.0f;
+  __shared__ uint4 sk[2][KT * CH];
+  __shared__ uint4 sv[2][KT * CH];
+  __shared__ int s_bad;  // some wave looked up a page outside the cache
+  const Paged8Args& pa = pa4.p;
+  const PagedArgs& a = pa.a;
+  const int h = static_cast<int>(blockIdx.x % a.Hkv);
+  const int64_t x = blockIdx.x / a.Hkv;
+  const int c = static_cast<int>(blockIdx.y);
+  const PagedTile tile = paged_find(a, 128, x, -1);
+  if (tile.b < 0) return;
+  const PagedSeq& sq = tile.s;
+  const int nk = static_cast<int>(sq.nk), nq = sq.nq;
+  const int k0 = c * tile.chunk;
+  if (k0 >= nk && c > 0) return;
+  const Int4Consts k4;
+  const bool bf = pa4.dtype == FP_DTYPE_BF16;
+  const bool single = nk <= tile.chunk;
+  const int t = threadIdx.x, lane = t & 63;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int half = lane >> 5, l32 = lane & 31;
+  const int rows = nq * a.G;
+  // (a sequence's last rows see most keys and start first)
+  const int tl = (rows + 127) / 128 - 1 - tile.tl;
+
+  // this lane's query row and its last visible key
+  const int rr = tl * 128 + 32 * w + l32;
+  const bool rvalid = rr < rows;
+  const int qi = (rvalid ? rr : rows - 1) / a.G;
+  const int64_t tok = sq.q0 + qi;
+  const int hq = h * a.G + (rvalid ? rr : rows - 1) % a.G;
+  const int lim = nk - nq + qi;
+  // the wave's first and last visible keys' bounds (wave-uniform)
+  const int r0 = min(tl * 128 + 32 * w, rows - 1);
+  const int r1 = min(tl * 128 + 32 * w + 31, rows - 1);
+  const int lim_lo = __builtin_amdgcn_readfirstlane(nk - nq + r0 / a.G);
+  const int lim_hi = __builtin_amdgcn_readfirstlane(nk - nq + r1 / a.G);
+  // keys past the last row of the tile are visible to none of its rows
+  const int last_row = min(tl * 128 + 127, rows - 1);
+  const int k1 = __builtin_amdgcn_readfirstlane(
+      min(min(k0 + tile.chunk, nk), max(nk - nq + last_row / a.G + 1, 0)));
+
+  // (the factor of a row's scores: its sign in q, so that the largest score is that of the
+  // largest product)
+  const float signed_scale = a.scale_log2 * fixed_scale(pa.ks, h);
+  float scale = fabsf(signed_scale), f = signed_scale < 0.0f ? -1.0f : 1.0f;
+  f16x8 qb[KS];
+  {
+    const uint16_t* qp = static_cast<const uint16_t*>(a.q) + tok * a.qst +
+                         static_cast<int64_t>(hq) * a.qhs + 8 * half;
+    uint4 y[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) y[s] = rvalid ? ld16(qp + 16 * s) : zero4();
+    if (bf) {
+      float most = 0.0f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) most = most8(y[s], most);
+      const int e = row_exponent(pair32_max(most));
+      f = __builtin_amdgcn_ldexpf(f, e);
+      scale *= __builtin_amdgcn_ldexpf(1.0f, -e);
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qb[s] = as_vec8<F16>(query8(y[s], bf, f));
+  }
+  // (not 0, by which a masked score would be NaN: by 2^-149 no score reaches 2^-100)
+  if (scale == 0.0f) scale = 0x1p-149f;
+  f32x16 o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
+  float m_run = -INFINITY, l_part = 0.0f;
+  bool bad = false;
+
+  const int64_t row = static_cast<int64_t>(tile.b) * a.table_stride;
+  const uint8_t* kc = static_cast<const uint8_t*>(a.kc) + static_cast<int64_t>(h) * a.kch;
+  const uint8_t* vc = static_cast<const uint8_t*>(a.vc) + static_cast<int64_t>(h) * a.vch;
+  const uint16_t* kg = pa4.kg.p + h * pa4.kg.sh;
+  const uint16_t* vg = pa4.vg.p + h * pa4.vg.sh;
+
+  const int lkey = lane >> 2, lp = lane & 3;  // the lane's key of a load, and its piece
+  uint32_t kr[NB], vr[NB], kgr[GW], vgr[GW];
+  const int last16 = (nk - 1) & ~15;
+  // tile of keys base .. base + 63; keys past the sequence read its last 16-key
+  // group (P16) or its last key
+  auto load = [&](int base) {
+    int64_t pg, in;
+    if constexpr (P16) {
+      const int tb = min(base + 16 * w, last16);
+      pg = paged_page<true>(a, row, tb, bad);
+      in = (a.bs_shift >= 0 ? tb & (a.bs - 1) : tb % a.bs) + lkey;
+    } else {
+      const int key = min(base + 16 * w + lkey, nk - 1);
+      pg = paged_page<false>(a, row, key, bad);
+      in = key % a.bs;
+    }
+    load_piece<NB>(kc + pg * a.kcb + in * a.kcs + 4 * NB * lp, kr);
+    load_piece<NB>(vc + pg * a.vcb + in * a.vcs + 4 * NB * lp, vr);
+    load_words<NB>(kg + pg * pa4.kg.sb + in * NB, kgr);
+    load_words<NB>(vg + pg * pa4.vg.sb + in * NB, vgr);
+  };
+  // as fp16 numbers into buffer `buf`; V of slots past the sequence is 0 (they may hold
+  // anything)
+  auto store = [&](int base, int buf) {
+    const int r = 16 * w + lkey;
+    if (base + r >= nk) {
+#pragma unroll
+      for (int q = 0; q < GW; ++q) vgr[q] = 0u;
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int at = r * CH + ((4 * j + lp) ^ swz<D>(r));
+      sk[buf][at] = piece_group<NB>(kr, kgr, j, k4);
+      sv[buf][at] = piece_group<NB>(vr, vgr, j, k4);
+    }
+  };
+  const int g16 = lane >> 4, i16 = lane & 15;
+  const int tr_row = 4 * (g16 >> 1) + (i16 >> 2);
+  const int tr_col = 16 * (g16 & 1) + 4 * (i16 & 3);
+
+  // (ordered before the flag by the barrier after the loop)
+  if (t == 0) s_bad = 0;
+  if (k0 < k1) {
+    load(k0);
+    store(k0, 0);
+  }
+  int buf = 0;
+  for (int base = k0; base < k1; base += KT, buf ^= 1) {
+    // this tile is in LDS for every wave, and every wave is done with the other buffer
+    lds_barrier();
+    const bool more = base + KT < k1;
+    if (more) load(base + KT);
+    if (base <= lim_hi) {  // (else no key of this tile is visible to the wave)
+      f32x16 s[TT];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int t4 = 0; t4 < TT; ++t4) {
+          const int r = 32 * t4 + l32;
+          const uint4 kop = sk[buf][r * CH + ((2 * ks + half) ^ swz<D>(r))];
+          s[t4] = F16::mfma32(as_vec8<F16>(kop), qb[ks], ks == 0 ? f32x16{} : s[t4]);
+        }
+      if (base + KT - 1 > lim_lo) {
+        asm volatile("");  // (a branch: as selects they would be in every tile)
+#pragma unroll
+        for (int t4 = 0; t4 < TT; ++t4)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            if (base + 32 * t4 + 8 * (v >> 2) + 4 * half + (v & 3) > lim) s[t4][v] = -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t4 = 0; t4 < TT; ++t4)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[t4][v]);
+      mx = pair32_max(mx) * scale;
+      // m moves only where it must, so that P stays below 2^kStep: not in every tile that
+      // has a new largest score for one of the wave's rows
+      if (__ballot(mx > m_run + kStep) != 0) {
+        const float m_new = fmaxf(m_run, mx);
+        const float ms = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m_run - ms);
+        m_run = m_new;
+        l_part *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[dt][v] *= alpha;
+      }
+      // rows with no visible key yet keep m = -inf: their P is 0
+      const float ms = m_run == -INFINITY ? 0.0f : m_run - kPScaleRows;
+#pragma unroll
+      for (int t4 = 0; t4 < TT; ++t4) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          s[t4][v] = __builtin_amdgcn_exp2f(fmaf(s[t4][v], scale, -ms));
+          l_part += s[t4][v];
+        }
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          uint32_t u[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            u[e] = pack2<F16>(s[t4][8 * hh + 2 * e], s[t4][8 * hh + 2 * e + 1]);
+          const f16x8 pb = as_vec8<F16>(make_uint4(u[0], u[1], u[2], u[3]));
+          const uint16_t* sv16 = reinterpret_cast<const uint16_t*>(sv[buf]);
+          const int r = 32 * t4 + 16 * hh + tr_row;
+          __builtin_amdgcn_sched_barrier(0);
+          f16x8 va[DT];
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) va[dt] = read_vt<F16, D>(sv16, r, 32 * dt + tr_col);
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[dt] = F16::mfma32(va[dt], pb, o[dt]);
+        }
+      }
+    }
+    if (more) store(base + KT, buf ^ 1);
+  }
+
+  // Rows whose O is not finite (a group of NaN) take P.V again over the keys that each row
+  // sees: a masked key's NaN times P = 0 is NaN.
+  float nf = 0.0f;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) nf = fmaf(o[dt][v], 0.0f, nf);
+  if (__ballot(nf != 0.0f) != 0) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
+    const float ms = m_run == -INFINITY ? 0.0f : m_run - kPScaleRows;
+    int half2 = static_cast<int>(threadIdx.x);  // (formed here, not kept across the loop)
+    asm volatile("" : "+v"(half2));
+    half2 = (half2 >> 5) & 1;
+#pragma unroll 1
+    for (int key = k0; key < k1; ++key) {
+      const int64_t pg = paged_page<true>(a, row, key, bad);
+      const int64_t in = key % a.bs;
+      float d = 0.0f;  // the lane's eight of every 16 dims of q . u_k: pieces half, 2 + half
+      uint32_t y[2][NB], gw[GW];
+      load_words<NB>(kg + pg * pa4.kg.sb + in * NB, gw);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        load_piece<NB>(kc + pg * a.kcb + in * a.kcs + 4 * NB * (2 * i + half2), y[i]);
+        f16x8 q[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) q[j] = qb[2 * j + i];
+        d += piece_dot<NB>(y[i], gw, q, k4);
+      }
+      d = pair32_sum(d) * scale;
+      if (key > lim) continue;
+      const float p = __builtin_amdgcn_exp2f(d - ms);
+      load_words<NB>(vg + pg * pa4.vg.sb + in * NB, gw);
+#pragma unroll
+      for (int pc = 0; pc < 4; ++pc) {  // o[dt][4 pc + e]: place 4 half + e of piece pc
+        load_piece<NB>(vc + pg * a.vcb + in * a.vcs + 4 * NB * pc, y[0]);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const uint4 g8 = piece_group<NB>(y[0], gw, dt, k4);
+          const uint32_t g2[2] = {half2 ? g8.z : g8.x, half2 ? g8.w : g8.y};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o[dt][4 * pc + e] =
+                fmaf(p, F16::to_f32(static_cast<uint16_t>(g2[e >> 1] >> (16 * (e & 1)))),
+                     o[dt][4 * pc + e]);
+        }
+      }
+    }
+  }
+
+  // A wave looks up the pages of its 16 keys of a tile only, and all four use the
+  // tile: a bad page found by one makes the rows of all four NaN.
+  float l = pair32_sum(l_part);
+  lds_barrier();
+  if (bad) s_bad = 1;
+  lds_barrier();
+  if (s_bad != 0) l = __uint_as_float(0x7fc00000u);
+  if (!rvalid) return;
+  // (dims 0, 2, 1, 3 of four)
+  if (single) {
+    const float rcp = 1.0f / l, vs = fixed_scale(pa.vs, h);
+    uint16_t* op = static_cast<uint16_t*>(a.o) + tok * a.ost + static_cast<int64_t>(hq) * a.ohs;
+    const float nan = __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[e] = o[dt][4 * g4 + e] * rcp * vs;
+          if (nk == 0) y[e] = sq.bad ? nan : 0.0f;
+        }
+        *reinterpret_cast<uint2*>(op + 32 * dt + 8 * g4 + 4 * half) =
+            make_uint2(round2(y[0], y[2], bf), round2(y[1], y[3], bf));
+      }
+  } else {
+    const int64_t slot = (tok * a.Hq + hq) * a.nc + c;
+    float* pp = a.part + slot * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4)
+        *reinterpret_cast<float4*>(pp + 32 * dt + 8 * g4 + 4 * half) =
+            make_float4(o[dt][4 * g4], o[dt][4 * g4 + 2], o[dt][4 * g4 + 1], o[dt][4 * g4 + 3]);
+    if (half == 0) {
+      a.ml[2 * slot] = m_run;
+      a.ml[2 * slot + 1] = l;
+    }
+  }
+}
+
+template <int D, int HP>
+hipError_t launch_few4(const Paged4Args& p, hipStream_t s) {
+  const PagedArgs& a = p.p.a;
+  const dim3 grid(static_cast<unsigned>(a.nc)), b(256);
+  if (a.bs % 16 != 0) hipLaunchKernelGGL((k_paged4<D, false, HP>), grid, b, 0, s, p);
+  else hipLaunchKernelGGL((k_paged4<D, true, HP>), grid, b, 0, s, p);
+  if (a.part != nullptr) {
+    const dim3 mg(static_cast<unsigned>(p.p.segs * HP)), mb(1024);
+    if (p.dtype == FP_DTYPE_BF16)
+      hipLaunchKernelGGL((k_paged4_merge<BF16, D, HP>), mg, mb, 0, s, p.p);
+    else
+      hipLaunchKernelGGL((k_paged4_merge<F16, D, HP>), mg, mb, 0, s, p.p);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_paged4(const Paged4Args& p, int head_dim, int hp, bool rows, int64_t tiles,
+                         hipStream_t s) {
+  const PagedArgs& a = p.p.a;
+  return with_head_dim(head_dim, [&](auto dc) -> hipError_t {
+    constexpr int D = decltype(dc)::value;
+    if (!rows) {
+      if constexpr (D == 64) {
+        if (hp == 4) return launch_few4<D, 4>(p, s);
+      }
+      if constexpr (D <= 128) {
+        if (hp == 2) return launch_few4<D, 2>(p, s);
+      }
+      return launch_few4<D, 1>(p, s);
+    }
+    const dim3 grid(static_cast<unsigned>(tiles * a.Hkv), static_cast<unsigned>(a.nc)), b(256);
+    if (a.bs % 16 != 0) hipLaunchKernelGGL((k_paged4_rows<D, false>), grid, b, 0, s, p);
+    else hipLaunchKernelGGL((k_paged4_rows<D, true>), grid, b, 0, s, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.nc <= 1) return e;
+    return launch_paged_merge8(a, p.dtype, D, s);
+  });
+}
+
+}  // namespace fp

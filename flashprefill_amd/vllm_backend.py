@@ -25,7 +25,8 @@ The v1 forward mirrors what the 0.12 patch does to
 * an fp8 ``kv_cache_dtype`` (:151-166) keeps the cache in 8-bit floats with the
   layer's ``_k_scale`` / ``_v_scale``: written by the HIP kernel behind
   ``fp_kv_cache_write_fp8``, attended by ``fp_paged_attention_fp8``. The query
-  stays in 16 bits: one that the layer has quantised is refused.
+  stays in 16 bits: one that the layer has quantised is refused. ``int4`` keeps it
+  in 4-bit integers (``int4_cache``), 9/16 of a byte for each element.
 
 vLLM is not a dependency: the forward only touches the attributes of the
 impl object and the metadata that the reference's forward reads, and the two
@@ -66,6 +67,7 @@ _DTYPES = {torch.bfloat16: _lib.FP_DTYPE_BF16, torch.float16: _lib.FP_DTYPE_F16}
 
 # 8-bit cache types and their names in vLLM's kv_cache_dtype
 _FORMATS = {torch.float8_e4m3fn: _lib.FP_CACHE_E4M3, torch.float8_e5m2: _lib.FP_CACHE_E5M2}
+_INT4_NAME = "int4"
 _FP8_NAMES = {"fp8": torch.float8_e4m3fn, "fp8_e4m3": torch.float8_e4m3fn,
               "fp8_e5m2": torch.float8_e5m2}
 
@@ -277,6 +279,37 @@ def reshape_and_cache_reference(key: torch.Tensor, value: torch.Tensor, key_cach
         cache[page, at] = x.clamp(-top, top).to(cache.dtype)
 
 
+def _check_sequences(cu_seqlens, block_table, starts, rows: int) -> int:
+    """Refuse sequences of a read-back that do not fit; how many there are."""
+    if cu_seqlens.dim() != 1 or block_table.dim() != 2 or \
+            (starts is not None and starts.dim() != 1):
+        raise ValueError("cu_seqlens and starts must have one dimension, block_table two")
+    B = cu_seqlens.numel() - 1
+    if B < 0 or block_table.shape[0] < B or (starts is not None and starts.numel() < B):
+        raise ValueError(f"block_table {tuple(block_table.shape)} or starts do not match "
+                         f"{B} sequences")
+    for name, t in (("cu_seqlens", cu_seqlens), ("block_table", block_table), ("starts", starts)):
+        if t is not None and t.dtype not in _INDEX:
+            raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
+    if not cu_seqlens.is_cuda:  # known without a synchronisation
+        at = cu_seqlens.tolist()
+        if at[0] < 0 or at[-1] > rows or any(x > y for x, y in zip(at, at[1:])):
+            raise ValueError(f"cu_seqlens {at} do not ascend within {rows} rows")
+    return B
+
+
+def _sequence_args(cu_seqlens, block_table, starts, device):
+    """The trailing fields of the read-backs' arguments, and the tensors they name."""
+    cu, table = cu_seqlens.to(device).contiguous(), block_table.to(device)
+    if table.stride(1) != 1:
+        table = table.contiguous()
+    if starts is not None:
+        starts = starts.to(device).contiguous()
+    return (cu.numel() - 1, table.shape[1], cu.dtype == torch.int64, table.dtype == torch.int64,
+            starts is not None and starts.dtype == torch.int64, cu.data_ptr(), table.data_ptr(),
+            None if starts is None else starts.data_ptr(), table.stride(0)), (cu, table, starts)
+
+
 def gather_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.Tensor,
                  value: torch.Tensor, cu_seqlens: torch.Tensor, block_table: torch.Tensor,
                  starts: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
@@ -299,22 +332,9 @@ def gather_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.
     _check_scales(key_cache, k_scale, v_scale)
     if value.shape != key.shape:
         raise ValueError(f"key {tuple(key.shape)} and value {tuple(value.shape)} differ")
-    if cu_seqlens.dim() != 1 or block_table.dim() != 2 or \
-            (starts is not None and starts.dim() != 1):
-        raise ValueError("cu_seqlens and starts must have one dimension, block_table two")
-    B, dev = cu_seqlens.numel() - 1, key.device
-    if B < 0 or block_table.shape[0] < B or (starts is not None and starts.numel() < B):
-        raise ValueError(f"block_table {tuple(block_table.shape)} or starts do not match "
-                         f"{B} sequences")
-    for name, t in (("cu_seqlens", cu_seqlens), ("block_table", block_table), ("starts", starts)):
-        if t is not None and t.dtype not in _INDEX:
-            raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
+    B, dev = _check_sequences(cu_seqlens, block_table, starts, key.shape[0]), key.device
     if forward_ad._current_level >= 0:
         _check_no_tangents(key, value, key_cache, value_cache, k_scale, v_scale)
-    if not cu_seqlens.is_cuda:  # known without a synchronisation
-        at = cu_seqlens.tolist()
-        if at[0] < 0 or at[-1] > key.shape[0] or any(x > y for x, y in zip(at, at[1:])):
-            raise ValueError(f"cu_seqlens {at} do not ascend within {key.shape[0]} rows")
     for t in (key, value, key_cache, value_cache):
         if not t.is_cuda or t.device != dev:
             raise ValueError("key, value and the caches must be on one GPU")
@@ -328,34 +348,20 @@ def gather_cache(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.
         gather_cache_reference(key_cache, value_cache, key, value, cu_seqlens, block_table, starts,
                                k_scale, v_scale)
         return
-    cu, table = cu_seqlens.to(dev).contiguous(), block_table.to(dev)
-    if table.stride(1) != 1:
-        table = table.contiguous()
-    if starts is not None:
-        starts = starts.to(dev).contiguous()
     (ks, k_keep), (vs, v_keep) = _scale_args(k_scale, dev), _scale_args(v_scale, dev)
+    sequences, keep = _sequence_args(cu_seqlens, block_table, starts, dev)
     a = _lib.FpKvGatherArgs(
         _cache_args(key, value, key_cache, value_cache, 0, key.shape[0]), ks, vs,
-        _FORMATS.get(key_cache.dtype, _lib.FP_CACHE_16BIT), B, table.shape[1],
-        cu.dtype == torch.int64, table.dtype == torch.int64,
-        starts is not None and starts.dtype == torch.int64, cu.data_ptr(), table.data_ptr(),
-        None if starts is None else starts.data_ptr(), table.stride(0))
+        _FORMATS.get(key_cache.dtype, _lib.FP_CACHE_16BIT), *sequences)
     _launch(dev, _lib.load().fp_kv_cache_gather, ctypes.byref(a))
     torch.autograd.graph.increment_version([key, value])
 
 
-@torch.no_grad()
-def gather_cache_reference(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.Tensor,
-                           value: torch.Tensor, cu_seqlens: torch.Tensor, block_table: torch.Tensor,
-                           starts: Optional[torch.Tensor] = None,
-                           k_scale: Optional[torch.Tensor] = None,
-                           v_scale: Optional[torch.Tensor] = None) -> None:
-    """The torch composition of ``gather_cache``, what a trace or a dispatch mode sees
-    of it."""
-    dev, n, B = key.device, key.shape[0], cu_seqlens.numel() - 1
-    nb, bs = key_cache.shape[:2]
-    if key.numel() == 0:
-        return
+def _cached_places(dev, n, shape, cu_seqlens, block_table, starts):
+    """Where a read-back's n rows lie in a cache of ``shape``: page and slot of each,
+    whether it can be read, and whether it is written (as NaN where it cannot be read)."""
+    nb, bs = shape[:2]
+    B = cu_seqlens.numel() - 1
     if nb < 1 or bs < 1:
         raise ValueError("the caches have no pages")
     room = block_table.shape[1] * bs
@@ -379,12 +385,27 @@ def gather_cache_reference(key_cache: torch.Tensor, value_cache: torch.Tensor, k
         page = torch.where(fits, page, 0)
     else:
         page = at
+    return page, at, fits, written
+
+
+@torch.no_grad()
+def gather_cache_reference(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch.Tensor,
+                           value: torch.Tensor, cu_seqlens: torch.Tensor, block_table: torch.Tensor,
+                           starts: Optional[torch.Tensor] = None,
+                           k_scale: Optional[torch.Tensor] = None,
+                           v_scale: Optional[torch.Tensor] = None) -> None:
+    """The torch composition of ``gather_cache``, what a trace or a dispatch mode sees
+    of it."""
+    if key.numel() == 0:
+        return
+    page, at, fits, written = _cached_places(key.device, key.shape[0], key_cache.shape, cu_seqlens,
+                                             block_table, starts)
     for y, cache, scale in ((key, key_cache, k_scale), (value, value_cache, v_scale)):
         x = cache[page, at]
         if cache.dtype in _FORMATS:
             x = x.float()
             if scale is not None:
-                s = scale[page, :, at] if scale.dim() == 3 else scale.to(dev).view(1, -1)
+                s = scale[page, :, at] if scale.dim() == 3 else scale.to(y.device).view(1, -1)
                 x = x * s.unsqueeze(-1)
             x = x.to(y.dtype)
         x = x.masked_fill(~fits.view(-1, 1, 1), math.nan)
@@ -441,42 +462,27 @@ def _rows_ok(t: torch.Tensor, any_stride_of_one: bool) -> bool:
     return True
 
 
-def _paged_kernel_takes(query, key_cache, value_cache, out, cu, used, table, k_scale=None,
-                        v_scale=None) -> bool:
-    """Whether the HIP kernels take this call as it is: 16-bit tensors of one
-    type on one GPU (or caches of one 8-bit type with scales that the kernels can
-    read in 16-byte pieces), head_dim 64 / 128 / 256, 16-byte aligned rows, int32
-    / int64 metadata of matching shapes, no derivative, functional transform,
-    trace or dispatch mode to carry along (they see only torch operations)."""
-    if not query.is_cuda or query.dtype not in _DTYPES:
+def _call_fits(query, out, shape, cu, used, table) -> bool:
+    """What every paged kernel asks of a call besides its caches, whose pages, slots, KV
+    heads and head_dim are ``shape``: 16-bit queries and outputs on one GPU, head_dim 64 /
+    128 / 256, int32 / int64 metadata of matching shapes, no forward-mode tangent, functional
+    transform, trace or dispatch mode to carry along (they see only torch operations)."""
+    if not query.is_cuda or query.dtype not in _DTYPES or out.dtype != query.dtype or \
+            out.device != query.device:
         return False
     if forward_ad._current_level >= 0 or _torch_only() or \
             torch._C._functorch.peek_interpreter_stack() is not None:
         return False
-    dev, dt = query.device, query.dtype
-    if query.dim() != 3 or out.dim() != 3 or key_cache.dim() != 4 or \
-            value_cache.shape != key_cache.shape:
+    if query.dim() != 3 or out.dim() != 3:
         return False
-    nb, bs, hkv, d = key_cache.shape
+    nb, bs, hkv, d = shape
     T, hq, dq = query.shape
     if d not in (64, 128, 256) or dq != d or nb < 1 or bs < 1 or hkv < 1 or hq < 1 or hq % hkv or \
             out.shape[0] < T or out.shape[1:] != query.shape[1:]:
         return False
-    cdt = key_cache.dtype
-    if cdt != dt and cdt not in _FORMATS:
-        return False
-    for t, want in ((query, dt), (key_cache, cdt), (value_cache, cdt), (out, dt)):
-        if t.dtype != want or t.device != dev or not _rows_ok(t, cdt != dt):
-            return False
-    for s in (k_scale, v_scale):
-        if s is not None and s.dim() == 3 and bs % 16 == 0 and \
-                (s.data_ptr() % 16 or any(st % 4 for st in _slot_scale_strides(s))):
-            return False
     # torch refuses to write these, and so does the composition
     if (0 in out.stride() and any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride()))) or \
             (out.is_inference() and not torch.is_inference_mode_enabled()):
-        return False
-    if key_cache.stride(1) >= 1 << 24 or value_cache.stride(1) >= 1 << 24:
         return False
     if cu.dim() != 1 or used.dim() != 1 or table.dim() != 2 or cu.numel() < 2:
         return False
@@ -490,46 +496,82 @@ def _paged_kernel_takes(query, key_cache, value_cache, out, cu, used, table, k_s
         at = cu.tolist()
         if at[0] < 0 or at[-1] > T or any(x > y for x, y in zip(at, at[1:])):
             return False
-    if not used.is_cuda and any(n > table.shape[1] * bs for n in used[:B].tolist()):
-        return False
+    return used.is_cuda or not any(n > table.shape[1] * bs for n in used[:B].tolist())
+
+
+def _none_requires_grad(*tensors) -> bool:
     if not torch.is_grad_enabled():
         return True
-    for t in (query, key_cache, value_cache, out, k_scale, v_scale):
+    for t in tensors:
         if t is not None and t.requires_grad:
             return False
     return True
 
 
-def _paged_attention_kernel(query, key_cache, value_cache, out, cu, used, table, scale,
-                            k_scale=None, v_scale=None) -> None:
+def _paged_kernel_takes(query, key_cache, value_cache, out, cu, used, table, k_scale=None,
+                        v_scale=None) -> bool:
+    """Whether the HIP kernels take this call as it is: caches of the query's type (or of
+    one 8-bit type with scales that the kernels can read in 16-byte pieces), 16-byte aligned
+    rows, no derivative, and what every paged kernel asks."""
+    if key_cache.dim() != 4 or value_cache.shape != key_cache.shape or \
+            not _call_fits(query, out, key_cache.shape, cu, used, table):
+        return False
+    dev, dt, cdt = query.device, query.dtype, key_cache.dtype
+    if cdt != dt and cdt not in _FORMATS:
+        return False
+    for t, want in ((query, dt), (key_cache, cdt), (value_cache, cdt), (out, dt)):
+        if t.dtype != want or t.device != dev or not _rows_ok(t, cdt != dt):
+            return False
+    bs = key_cache.shape[1]
+    for s in (k_scale, v_scale):
+        if s is not None and s.dim() == 3 and bs % 16 == 0 and \
+                (s.data_ptr() % 16 or any(st % 4 for st in _slot_scale_strides(s))):
+            return False
+    if key_cache.stride(1) >= 1 << 24 or value_cache.stride(1) >= 1 << 24:
+        return False
+    return _none_requires_grad(query, key_cache, value_cache, out, k_scale, v_scale)
+
+
+def _paged_args(query, key_cache, value_cache, out, cu, used, table, scale, d):
+    """``fp_paged_args`` of a call, and the tensors whose memory it names."""
     dev = query.device
-    nb, bs, hkv, d = key_cache.shape
+    nb, bs, hkv, _ = key_cache.shape
     T, hq = query.shape[:2]
     cu, used = cu.to(dev).contiguous(), used.to(dev).contiguous()
     table = table.to(dev)
     if table.stride(1) != 1:
         table = table.contiguous()
-    lib = _lib.load()
-    call = _lib.FpPagedArgs(
+    return _lib.FpPagedArgs(
         query.data_ptr(), *query.stride()[:2], out.data_ptr(), *out.stride()[:2],
         key_cache.data_ptr(), value_cache.data_ptr(), *key_cache.stride()[:3],
         *value_cache.stride()[:3], cu.data_ptr(), used.data_ptr(), table.data_ptr(),
         table.stride(0), T, nb, cu.numel() - 1, table.shape[1], bs, hq, hkv, d,
         _DTYPES[query.dtype], cu.dtype == torch.int64, used.dtype == torch.int64,
-        table.dtype == torch.int64, float(scale))
-    ws_bytes, launch = lib.fp_paged_workspace_bytes, lib.fp_paged_attention
-    if key_cache.dtype in _FORMATS:
-        (ks, k_keep), (vs, v_keep) = _scale_args(k_scale, dev), _scale_args(v_scale, dev)
-        call = _lib.FpPagedFp8Args(call, ks, vs, _FORMATS[key_cache.dtype])
-        ws_bytes, launch = lib.fp_paged_fp8_workspace_bytes, lib.fp_paged_attention_fp8
+        table.dtype == torch.int64, float(scale)), (cu, used, table)
+
+
+def _attend(device, call, ws_bytes, launch, out) -> None:
     # A buffer of this call's own: threads that share a stream may interleave
     # their launches, and a shared one would be written between the chunks and
     # their merge. The caching allocator hands it on in stream order.
     n = ws_bytes(ctypes.byref(call))
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    _launch(dev, launch, ctypes.byref(call), None if ws is None else ws.data_ptr())
+    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    _launch(device, launch, ctypes.byref(call), None if ws is None else ws.data_ptr())
     # a graph that saved `out` finds it changed, as after any in-place operation
     torch.autograd.graph.increment_version(out)
+
+
+def _paged_attention_kernel(query, key_cache, value_cache, out, cu, used, table, scale,
+                            k_scale=None, v_scale=None) -> None:
+    dev, lib = query.device, _lib.load()
+    call, keep = _paged_args(query, key_cache, value_cache, out, cu, used, table, scale,
+                             key_cache.shape[3])
+    if key_cache.dtype not in _FORMATS:
+        _attend(dev, call, lib.fp_paged_workspace_bytes, lib.fp_paged_attention, out)
+        return
+    (ks, k_keep), (vs, v_keep) = _scale_args(k_scale, dev), _scale_args(v_scale, dev)
+    call = _lib.FpPagedFp8Args(call, ks, vs, _FORMATS[key_cache.dtype])
+    _attend(dev, call, lib.fp_paged_fp8_workspace_bytes, lib.fp_paged_attention_fp8, out)
 
 
 def paged_attention_reference(query: torch.Tensor, key_cache: torch.Tensor,
@@ -544,20 +586,30 @@ def paged_attention_reference(query: torch.Tensor, key_cache: torch.Tensor,
     if key_cache.dtype in _FORMATS and query.element_size() < 2:
         raise NotImplementedError(f"a query of {query.dtype} over an 8-bit cache: its codes have a "
                                   f"scale of their own, which this operation does not take")
+    _, bs, hkv, d = key_cache.shape
+    _attend_composed(query, out, cu_seqlens_q, seqused_k, block_table, softmax_scale, bs,
+                     lambda blocks: (_pages_fp32(key_cache, blocks, k_scale),
+                                     _pages_fp32(value_cache, blocks, v_scale)))
+
+
+def _attend_composed(query, out, cu_seqlens_q, seqused_k, block_table, softmax_scale, bs,
+                     pages) -> None:
+    """Attention over pages of ``bs`` tokens whose keys and values ``pages(blocks)`` gives in
+    fp32, (blocks, bs, Hkv, d) each, a sequence at a time."""
     cu = cu_seqlens_q.tolist()
     used = seqused_k.tolist()
-    _, bs, hkv, d = key_cache.shape
-    hq = query.shape[1]
-    g = hq // hkv
+    hq, d = query.shape[1:]
     for b in range(len(cu) - 1):
         q0, q1 = cu[b], cu[b + 1]
         nq, nk = q1 - q0, int(used[b])
         if nq == 0:
             continue
         nblk = (nk + bs - 1) // bs
-        blocks = block_table[b, :nblk].long()
-        k = _pages_fp32(key_cache, blocks, k_scale).reshape(nblk * bs, hkv, d)[:nk]
-        v = _pages_fp32(value_cache, blocks, v_scale).reshape(nblk * bs, hkv, d)[:nk]
+        k, v = pages(block_table[b, :nblk].long())
+        hkv = k.shape[2]
+        g = hq // hkv
+        k = k.reshape(nblk * bs, hkv, d)[:nk]
+        v = v.reshape(nblk * bs, hkv, d)[:nk]
         q = query[q0:q1].float()  # (nq, hq, d)
         k = k.repeat_interleave(g, dim=1).permute(1, 2, 0).contiguous()  # (hq, d, nk)
         v = v.repeat_interleave(g, dim=1).permute(1, 0, 2).contiguous()  # (hq, nk, d)
@@ -587,7 +639,9 @@ class HookOps:
     ``encoder`` and ``cascade`` take the impl and the reference's arguments
     and default to raising: they stay vLLM's. ``cache_write_fp8`` and
     ``decode_fp8`` serve layers with an fp8 cache: the operations above with the
-    scales as two more arguments."""
+    scales as two more arguments. ``cache_write_int4`` and ``decode_int4`` serve layers
+    with a 4-bit cache, the caches' group words as two more behind them (None: those of
+    ``int4_cache``)."""
     cache_write: Callable[..., None] = reshape_and_cache
     prefill: Callable[..., None] = flash_prefill_varlen_func
     decode: Callable[..., None] = paged_decode_attention
@@ -595,14 +649,19 @@ class HookOps:
     cascade: Optional[Callable[..., torch.Tensor]] = None
     cache_write_fp8: Callable[..., None] = reshape_and_cache
     decode_fp8: Callable[..., None] = paged_decode_attention
+    cache_write_int4: Optional[Callable[..., None]] = None
+    decode_int4: Optional[Callable[..., None]] = None
 
 
 def _cache_ops(impl, layer, ops: HookOps, key_cache, value_cache):
     """The layer's caches, its cache write and its attention over them: those of
     ``ops``, or for an fp8 ``kv_cache_dtype`` the 8-bit forms with the layer's
     ``_k_scale`` / ``_v_scale`` (1 where it has none) over the caches, which vLLM
-    allocates as bytes, in their type."""
+    allocates as bytes, in their type; for int4 the 4-bit forms over the codes and
+    group words in those bytes (``int4_cache.int4_cache_views``)."""
     name = str(getattr(impl, "kv_cache_dtype", "auto"))
+    if name == _INT4_NAME:
+        return _int4_ops(layer, ops, key_cache, value_cache)
     if not name.startswith("fp8"):
         return key_cache, value_cache, ops.cache_write, ops.decode
     dtype = _FP8_NAMES.get(name)
@@ -618,6 +677,23 @@ def _cache_ops(impl, layer, ops: HookOps, key_cache, value_cache):
         ops.decode_fp8(q, kc, vc, out, cu, used, table, scale, *scales)
 
     return key_cache.view(dtype), value_cache.view(dtype), write, decode
+
+
+def _int4_ops(layer, ops: HookOps, key_cache, value_cache):
+    from . import int4_cache as i4  # (which builds on this module)
+
+    (kc, kg), (vc, vg) = i4.int4_cache_views(key_cache), i4.int4_cache_views(value_cache)
+    scales = getattr(layer, "_k_scale", None), getattr(layer, "_v_scale", None)
+    write_op = ops.cache_write_int4 or i4.reshape_and_cache_int4
+    decode_op = ops.decode_int4 or i4.paged_decode_attention_int4
+
+    def write(key, value, kc, vc, slots):
+        write_op(key, value, kc, vc, kg, vg, slots, *scales)
+
+    def decode(q, kc, vc, out, cu, used, table, scale):
+        decode_op(q, kc, vc, kg, vg, out, cu, used, table, scale, *scales)
+
+    return kc, vc, write, decode
 
 
 def _is_encoder(attn_type) -> bool:

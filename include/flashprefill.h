@@ -30,7 +30,8 @@
  *                          ops/flashprefill_native_forward.py:227-344, ops/flashprefill_varlen_func.py:449-575
  *   fp_kv_cache_write      the paged KV-cache write the vLLM patch makes before attention
  *                          (reshape_and_cache_flash, patches/patch_loader_vllm_0_12_0.py:140-149);
- *                          fp_kv_cache_write_fp8: into a cache of 8-bit floats
+ *                          fp_kv_cache_write_fp8: into a cache of 8-bit floats,
+ *                          fp_kv_cache_write_int4: of 4-bit integers
  */
 #ifndef FLASHPREFILL_H
 #define FLASHPREFILL_H
@@ -306,6 +307,61 @@ typedef struct fp_paged_fp8_args {
 } fp_paged_fp8_args;
 size_t fp_paged_fp8_workspace_bytes(const fp_paged_fp8_args* a); /* 0: none needed, or invalid */
 int fp_paged_attention_fp8(const fp_paged_fp8_args* a, void* workspace, void* stream);
+
+/* Caches of 4-bit integers. A row of head_dim (64, 128 or 256) elements is head_dim / 2
+ * bytes: byte m (head_dim / 32) + j, m < 16, holds the codes of dims 32 j + 2 m (low half)
+ * and 32 j + 2 m + 1. The 32 dims of group j share a 16-bit word w: code c stands for
+ *   s (c + z) t,  s the fp16 number of bits w & 0x7f80 (4 significant bits, NaN: the group
+ *   is NaN),  z = (w & 0x7f) - 64,  t the fixed scale of the KV head.
+ * s (c + z) is exactly an fp16 number. The words of a slot are head_dim / 32 contiguous ones:
+ * data[block * stride_block + head * stride_head + slot * (head_dim / 32) + j]. */
+typedef struct fp_kv_groups {
+  uint16_t* data;
+  int64_t stride_block, stride_head; /* in words */
+} fp_kv_groups;
+
+/* fp_kv_cache_write into a 4-bit cache. The cache strides count bytes (multiples of 16;
+ * bases 16-byte aligned); the groups are aligned to head_dim / 16 bytes, with strides of
+ * whole slots; scales are fixed. With x' = x / t clamped to +-16384, lo and hi the group's
+ * smallest and largest x', rounding to nearest even throughout:
+ *   s = max((hi - lo) / 15, hi / 56, -lo / 56) rounded to 4 significant bits (to a multiple
+ *   of 2^-17 below 2^-14),  z = lo / s rounded, within -64 .. 63,
+ *   c = (x' / s rounded) - z, within 0 .. 15.
+ * s = 0: c = z = 0. A NaN makes its group NaN. Slots that two tokens name hold either
+ * row, or parts of both. */
+typedef struct fp_kv_cache_int4_args {
+  fp_kv_cache_args base;
+  fp_kv_groups k_groups, v_groups;
+  fp_kv_scales k_scale, v_scale;
+} fp_kv_cache_int4_args;
+int fp_kv_cache_write_int4(const fp_kv_cache_int4_args* a, void* stream);
+
+/* fp_kv_cache_gather from a 4-bit cache: s (c + z) t in fp32 rounded once. */
+typedef struct fp_kv_gather_int4_args {
+  fp_kv_cache_int4_args cache;
+  int32_t batch, table_width;
+  int32_t cu_is64, table_is64, starts_is64;
+  const void* cu_seqlens;
+  const void* block_table;
+  const void* starts;
+  int64_t table_stride;
+} fp_kv_gather_int4_args;
+int fp_kv_cache_gather_int4(const fp_kv_gather_int4_args* a, void* stream);
+
+/* fp_paged_attention over a 4-bit cache. base.dtype: the type of q and o; cache strides
+ * count bytes, as above; where block_size is a multiple of 16 the groups are 16-byte
+ * aligned, with strides of multiples of 8 words. No cached value is rounded: keys and
+ * values enter the products as fp16 numbers, t multiplies fp32 scores and rows. bf16
+ * queries enter them as fp16 numbers times a power of two of their row: what lies below
+ * 2^-39 of the row's largest element is lost. Probabilities are held to 2^-22; a call of
+ * many rows holds them to 2^-11, the rounding of an fp16 output. */
+typedef struct fp_paged_int4_args {
+  fp_paged_args base;
+  fp_kv_groups k_groups, v_groups;
+  fp_kv_scales k_scale, v_scale;
+} fp_paged_int4_args;
+size_t fp_paged_int4_workspace_bytes(const fp_paged_int4_args* a); /* 0: none needed, or invalid */
+int fp_paged_attention_int4(const fp_paged_int4_args* a, void* workspace, void* stream);
 
 /* Rotary position embedding (rotate-half) with optional per-head RMSNorm, in
  * place on the query and key heads of a decoder-layer attention block. No
