@@ -37,7 +37,8 @@ EXPORTS = (
     "fp_paged_attention", "fp_paged_workspace_bytes", "fp_kv_cache_write_fp8",
     "fp_kv_cache_gather", "fp_paged_attention_fp8", "fp_paged_fp8_workspace_bytes",
     "fp_kv_cache_write_int4", "fp_kv_cache_gather_int4", "fp_paged_attention_int4",
-    "fp_paged_int4_workspace_bytes",
+    "fp_paged_int4_workspace_bytes", "fp_rotary", "fp_build_step_tables",
+    "fp_steps_workspace_bytes",
 )
 NOALLOC_SCRATCH_BYTES = 96 * 1024 * 1024
 
@@ -191,6 +192,39 @@ class FpPagedInt4Args(ctypes.Structure):
     ]
 
 
+class FpRotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("q_out", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p),
+        ("q_stride_tok", ctypes.c_int64), ("q_stride_head", ctypes.c_int64),
+        ("k_stride_tok", ctypes.c_int64), ("k_stride_head", ctypes.c_int64),
+        ("q_out_stride_tok", ctypes.c_int64), ("q_out_stride_head", ctypes.c_int64),
+        ("k_out_stride_tok", ctypes.c_int64), ("k_out_stride_head", ctypes.c_int64),
+        ("positions", ctypes.c_void_p), ("frequencies", ctypes.c_void_p),
+        ("num_tokens", ctypes.c_int64),
+        ("positions_is64", ctypes.c_int32), ("num_pairs", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32), ("inverse", ctypes.c_int32),
+        ("amplitude", ctypes.c_float),
+    ]
+
+
+class FpStepsArgs(ctypes.Structure):
+    _fields_ = [
+        ("seq_lens", ctypes.c_void_p), ("new_lens", ctypes.c_void_p),
+        ("finished", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+        ("free_pages", ctypes.c_void_p), ("num_free", ctypes.c_void_p),
+        ("seq_lens_out", ctypes.c_void_p), ("num_free_out", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p), ("granted", ctypes.c_void_p),
+        ("num_tokens", ctypes.c_int64),
+        ("requests", ctypes.c_int32), ("table_width", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32), ("block_size", ctypes.c_int32),
+    ]
+
+
 _LIB = None
 
 
@@ -228,6 +262,10 @@ def load(path: Path = LIB_PATH) -> ctypes.CDLL:
     lib.fp_paged_attention_int4.argtypes = [ctypes.POINTER(FpPagedInt4Args), vp, vp]
     lib.fp_paged_int4_workspace_bytes.argtypes = [ctypes.POINTER(FpPagedInt4Args)]
     lib.fp_paged_int4_workspace_bytes.restype = ctypes.c_size_t
+    lib.fp_rotary.argtypes = [ctypes.POINTER(FpRotaryArgs), vp]
+    lib.fp_build_step_tables.argtypes = [ctypes.POINTER(FpStepsArgs), vp, vp]
+    lib.fp_steps_workspace_bytes.argtypes = [ctypes.POINTER(FpStepsArgs)]
+    lib.fp_steps_workspace_bytes.restype = ctypes.c_size_t
     lib.fp_search.argtypes = [P, vp, vp, vp, vp]
     lib.fp_select.argtypes = [P, vp, vp, vp, vp]
     lib.fp_read_status.argtypes = [P, vp, vp, ctypes.POINTER(ctypes.c_uint32)]

@@ -25,6 +25,7 @@ import torch
 
 from . import _lib
 from .flashprefill_varlen_func import flash_prefill_varlen_func
+from .rotary import Rotary, apply_rotary, apply_rotary_reference
 
 
 def positions_from_cu_seqlens(cu_seqlens: torch.Tensor, total: int) -> torch.Tensor:
@@ -122,8 +123,14 @@ class PrefillAttention(torch.nn.Module):
                  rope_theta: float = 1e6, qk_norm: bool = False, rms_eps: float = 1e-6,
                  alpha: float = 0.12, block_size: int = 128, attention_sink: int = 2,
                  window_size: int = 4, last_n_block: int = 2,
-                 dtype: torch.dtype = torch.bfloat16, device=None, seed: Optional[int] = None):
+                 dtype: torch.dtype = torch.bfloat16, device=None, seed: Optional[int] = None,
+                 rotary: Optional[Rotary] = None):
+        """``rotary``: positions of another layout or scaling than whole heads turned by
+        halves at ``rope_theta`` (which it replaces)."""
         super().__init__()
+        if rotary is not None and rotary.rotary_dim > head_dim:
+            raise ValueError(f"rotary_dim {rotary.rotary_dim} above head_dim {head_dim}")
+        self.rotary = rotary
         self.hidden, self.Hq, self.Hkv, self.d = hidden, num_q_heads, num_kv_heads, head_dim
         self.rope_theta, self.qk_norm, self.rms_eps = rope_theta, qk_norm, rms_eps
         self.alpha, self.block_size = alpha, block_size
@@ -152,6 +159,8 @@ class PrefillAttention(torch.nn.Module):
         q = qkv[:, :self.Hq]
         k = qkv[:, self.Hq:self.Hq + self.Hkv]
         v = qkv[:, self.Hq + self.Hkv:]
+        if self.rotary is not None:
+            return self.project_qkv_rotary(q, k, v, positions_from_cu_seqlens(cu_seqlens, T))
         if qkv.is_cuda and qkv.dtype in (torch.bfloat16, torch.float16):
             # one kernel, in place on the projection (q and k stay views of it);
             # it takes the offsets of up to 64 sequences as they are
@@ -165,6 +174,18 @@ class PrefillAttention(torch.nn.Module):
                           max_position=T, cu_seqlens=cu_seqlens if direct else None)
             return q, k, v
         return self.project_qkv_reference(q, k, v, positions_from_cu_seqlens(cu_seqlens, T))
+
+    def project_qkv_rotary(self, q, k, v, pos):
+        """The norms, where there are any, in torch, then ``self.rotary``: one kernel, in
+        place on the projection or its norms, on the GPU."""
+        if self.qk_norm:
+            q = rms_norm_heads(q, self.q_norm, self.rms_eps)
+            k = rms_norm_heads(k, self.k_norm, self.rms_eps)
+        on_gpu = q.is_cuda and q.dtype in (torch.bfloat16, torch.float16)
+        rotate = apply_rotary if on_gpu else apply_rotary_reference
+        rotate(q, k, pos.to(q.device), self.rotary.on(q.device),
+               interleaved=self.rotary.interleaved, amplitude=self.rotary.amplitude)
+        return q, k, v
 
     def project_qkv_reference(self, q, k, v, pos):
         """The torch composition of the same steps (the fused kernel's

@@ -961,6 +961,71 @@ int paged4_heads(const fp_paged_args* a) {
   return heads;
 }
 
+// Pairs of a thread of k_rotary: the most, up to 8, that divide the pairs and the rest of a
+// row, and that strides and addresses allow to move as one.
+int rotary_pairs(const fp_rotary_args* a) {
+  const int64_t st[8] = {a->q_stride_tok,     a->q_stride_head,     a->k_stride_tok,
+                         a->k_stride_head,    a->q_out_stride_tok,  a->q_out_stride_head,
+                         a->k_out_stride_tok, a->k_out_stride_head};
+  uintptr_t bits = 0;
+  const int H[2] = {a->num_q_heads, a->num_kv_heads};
+  const void* p[2][2] = {{a->q, a->q_out}, {a->k, a->k_out}};
+  for (int i = 0; i < 2; ++i) {
+    if (H[i] == 0) continue;
+    bits |= reinterpret_cast<uintptr_t>(p[i][0]) | reinterpret_cast<uintptr_t>(p[i][1]);
+    for (int s = 0; s < 4; ++s) {
+      const int64_t stride = st[2 * i + (s & 1) + 4 * (s >> 1)];
+      if ((s & 1 ? H[i] : a->num_tokens) > 1) bits |= static_cast<uintptr_t>(stride) * 2;
+    }
+  }
+  int v = 8;
+  while (v > 1 && (bits % (2 * v) || a->num_pairs % v || a->head_dim % (2 * v))) v /= 2;
+  return v;
+}
+
+int rotary_valid(const fp_rotary_args* a) {
+  if (!a) return fail(FP_E_INVALID_ARG, "rotary arguments are NULL");
+  if (a->dtype != FP_DTYPE_BF16 && a->dtype != FP_DTYPE_F16)
+    return fail(FP_E_UNSUPPORTED, "rotary: dtype %d unsupported (bf16 or fp16)", a->dtype);
+  if (a->num_tokens < 0 || a->num_q_heads < 0 || a->num_kv_heads < 0 || a->num_pairs < 0 ||
+      a->head_dim < 2 || a->head_dim % 2 || 2 * static_cast<int64_t>(a->num_pairs) > a->head_dim)
+    return fail(FP_E_INVALID_ARG, "rotary: sizes out of range (head_dim even, 2 num_pairs within)");
+  if (a->head_dim > 1024) return fail(FP_E_UNSUPPORTED, "rotary: head_dim %d above 1024", a->head_dim);
+  if (a->num_tokens == 0) return FP_OK;
+  if ((a->num_q_heads > 0 && (!a->q || !a->q_out)) || (a->num_kv_heads > 0 && (!a->k || !a->k_out)) ||
+      !a->positions || (!a->frequencies && a->num_pairs > 0))
+    return fail(FP_E_INVALID_ARG, "rotary: NULL pointer");
+  // (a launch holds fewer than 2^32 threads; a workgroup's work is counted in 16 bits)
+  if (a->num_tokens >= int64_t(1) << 24)
+    return fail(FP_E_UNSUPPORTED, "rotary: %lld tokens in one call",
+                static_cast<long long>(a->num_tokens));
+  const int64_t heads = static_cast<int64_t>(a->num_q_heads) + a->num_kv_heads;
+  if (heads * (a->head_dim / (2 * rotary_pairs(a))) >= 1 << 16)
+    return fail(FP_E_UNSUPPORTED, "rotary: %lld heads of %d", static_cast<long long>(heads),
+                a->head_dim);
+  return FP_OK;
+}
+
+// A step that one workgroup makes: few requests and tokens. 256 requests with a token each
+// take one launch instead of three.
+bool one_step(const fp_steps_args* a) { return a->requests <= 1024 && a->num_tokens <= 8192; }
+
+int steps_valid(const fp_steps_args* a) {
+  if (!a) return fail(FP_E_INVALID_ARG, "step arguments are NULL");
+  if (a->requests < 0 || a->table_width < 0 || a->num_pages < 0 || a->block_size < 1 ||
+      a->num_tokens < 0 || a->table_stride < 0)
+    return fail(FP_E_INVALID_ARG, "steps: sizes out of range");
+  if (a->num_tokens > INT32_MAX || int64_t(a->table_width) * a->block_size > INT32_MAX ||
+      int64_t(a->requests) * a->table_width > INT32_MAX)
+    return fail(FP_E_UNSUPPORTED, "steps: tokens, a row's room and the table must count in 31 bits");
+  if ((a->requests > 0 && (!a->seq_lens || !a->new_lens || !a->seq_lens_out || !a->granted ||
+                           (a->table_width > 0 && !a->block_table))) ||
+      (a->num_pages > 0 && !a->free_pages) || !a->num_free || !a->num_free_out ||
+      !a->cu_seqlens || (a->num_tokens > 0 && (!a->positions || !a->slots)))
+    return fail(FP_E_INVALID_ARG, "steps: NULL pointer");
+  return FP_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1227,6 +1292,72 @@ int fp_paged_attention_int4(const fp_paged_int4_args* a, void* ws, void* stream)
   const hipError_t e = fp::launch_paged4(r, a->base.head_dim, heads, sp.many, sp.tiles,
                                          static_cast<hipStream_t>(stream));
   return e == hipSuccess ? FP_OK : hip_fail(e, "paged attention launch");
+}
+
+int fp_rotary(const fp_rotary_args* a, void* stream) {
+  const int rc = rotary_valid(a);
+  if (rc != FP_OK || a->num_tokens == 0) return rc;
+  fp::RotaryArgs r{};
+  r.q = a->q;
+  r.k = a->k;
+  r.q_out = a->q_out;
+  r.k_out = a->k_out;
+  r.q_stride_tok = a->q_stride_tok;
+  r.q_stride_head = a->q_stride_head;
+  r.k_stride_tok = a->k_stride_tok;
+  r.k_stride_head = a->k_stride_head;
+  r.qo_stride_tok = a->q_out_stride_tok;
+  r.qo_stride_head = a->q_out_stride_head;
+  r.ko_stride_tok = a->k_out_stride_tok;
+  r.ko_stride_head = a->k_out_stride_head;
+  r.positions = a->positions;
+  r.frequencies = a->frequencies;
+  r.num_tokens = a->num_tokens;
+  r.pos64 = a->positions_is64 != 0;
+  r.pairs = a->num_pairs;
+  r.num_q_heads = a->num_q_heads;
+  r.num_kv_heads = a->num_kv_heads;
+  r.head_dim = a->head_dim;
+  r.interleaved = a->interleaved != 0;
+  r.inverse = a->inverse != 0;
+  r.amplitude = a->amplitude;
+  const hipError_t e = fp::launch_rotary(r, a->dtype, rotary_pairs(a), static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? FP_OK : hip_fail(e, "rotary launch");
+}
+
+size_t fp_steps_workspace_bytes(const fp_steps_args* a) {
+  if (steps_valid(a) != FP_OK || one_step(a)) return 0;
+  return 16 + 12 * static_cast<size_t>(a->requests);
+}
+
+int fp_build_step_tables(const fp_steps_args* a, void* ws, void* stream) {
+  const int rc = steps_valid(a);
+  if (rc != FP_OK) return rc;
+  const bool one = one_step(a);
+  if (!one && (!ws || reinterpret_cast<uintptr_t>(ws) % 4))
+    return fail(FP_E_INVALID_ARG, "steps: workspace is NULL or not 4-byte aligned");
+  fp::StepArgs r;
+  r.seq_lens = a->seq_lens;
+  r.new_lens = a->new_lens;
+  r.finished = a->finished;
+  r.block_table = a->block_table;
+  r.table_stride = a->table_stride;
+  r.free_pages = a->free_pages;
+  r.num_free = a->num_free;
+  r.seq_lens_out = a->seq_lens_out;
+  r.num_free_out = a->num_free_out;
+  r.cu_seqlens = a->cu_seqlens;
+  r.positions = a->positions;
+  r.slots = a->slots;
+  r.granted = a->granted;
+  r.ws = static_cast<int32_t*>(ws);
+  r.R = a->requests;
+  r.W = a->table_width;
+  r.P = a->num_pages;
+  r.block_size = a->block_size;
+  r.N = a->num_tokens;
+  const hipError_t e = fp::launch_steps(r, one, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? FP_OK : hip_fail(e, "steps launch");
 }
 
 int fp_read_status(const fp_problem* p, void* ws, void* stream, uint32_t* status) {

@@ -277,6 +277,45 @@ struct RopeArgs {
   float eps;
 };
 
+// Rotary positions (fp_rotary.hip); strides in elements.
+struct RotaryArgs {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  int64_t q_stride_tok, q_stride_head, k_stride_tok, k_stride_head;
+  int64_t qo_stride_tok, qo_stride_head, ko_stride_tok, ko_stride_head;
+  const void* positions;
+  const double* frequencies;
+  int64_t num_tokens;
+  int32_t pos64, pairs, num_q_heads, num_kv_heads, head_dim, interleaved, inverse;
+  float amplitude;
+  // set by the launch: tokens of a workgroup, tasks of a row, and ceil(2^32 / tasks),
+  // ceil(2^32 / heads)
+  int32_t tokens, row_tasks;
+  uint32_t div_tasks, div_heads;
+};
+
+// Tables of a serving step (fp_steps.hip)
+struct StepArgs {
+  const int32_t* seq_lens;
+  const int32_t* new_lens;
+  const uint8_t* finished;  // nullable
+  int32_t* block_table;
+  int64_t table_stride;
+  int32_t* free_pages;
+  const int32_t* num_free;
+  int32_t* seq_lens_out;
+  int32_t* num_free_out;
+  int32_t* cu_seqlens;
+  int64_t* positions;
+  int64_t* slots;
+  int32_t* granted;
+  int32_t* ws;  // records of the requests, where several launches share the work
+  int32_t R, W, P, block_size;
+  int64_t N;
+};
+
 // f(std::integral_constant<int, D>{}) for the head dim D of the 16-bit
 // kernels' instantiations (64, 128, 256; the C ABI rejects any other)
 template <typename F>
@@ -287,6 +326,9 @@ auto with_head_dim(int head_dim, F&& f) {
 }
 
 hipError_t launch_plan(const PlanArgs& a, hipStream_t s);
+// v: pairs of a thread, 8, 4, 2 or 1
+hipError_t launch_rotary(RotaryArgs a, int dtype, int v, hipStream_t s);
+hipError_t launch_steps(const StepArgs& a, bool one, hipStream_t s);
 hipError_t launch_rope(const RopeArgs& a, int dtype, hipStream_t s);
 hipError_t launch_paged_rows(const PagedArgs& a, int dtype, int head_dim, int64_t tiles,
                              hipStream_t s);

@@ -399,6 +399,69 @@ typedef struct fp_rope_args {
 } fp_rope_args;
 int fp_rope_qk(const fp_rope_args* a, void* stream);
 
+/* Rotary positions of any layout. The first 2 num_pairs dims of each head are pairs (x, y):
+ * dims j and num_pairs + j, interleaved 2 j and 2 j + 1. With c, s = amplitude times cosine
+ * and sine of positions[t] * frequencies[j], formed in 64 bits and rounded to fp32,
+ *   (x, y) <- (round(x c - y s), round(y c + x s)),  s negated by `inverse`;
+ * the other dims are copied. q_out / k_out are q / k themselves or memory of their own.
+ * Elements of 16 bits, strides in elements (any), head dim contiguous; k may have no heads.
+ * Positions are 32- or 64-bit integers of any sign. */
+typedef struct fp_rotary_args {
+    const void* q;            /* (tokens, num_q_heads, head_dim) */
+    const void* k;
+    void* q_out;
+    void* k_out;
+    int64_t q_stride_tok, q_stride_head, k_stride_tok, k_stride_head;
+    int64_t q_out_stride_tok, q_out_stride_head, k_out_stride_tok, k_out_stride_head;
+    const void* positions;    /* device, num_tokens entries */
+    const double* frequencies; /* device, num_pairs entries */
+    int64_t num_tokens;
+    int32_t positions_is64, num_pairs;
+    int32_t num_q_heads, num_kv_heads;
+    int32_t head_dim;         /* even, at most 1024 */
+    int32_t dtype;            /* FP_DTYPE_BF16 or FP_DTYPE_F16 */
+    int32_t interleaved, inverse;
+    float amplitude;
+} fp_rotary_args;
+int fp_rotary(const fp_rotary_args* a, void* stream);
+
+/* The tables of a serving step over a paged cache, from the lengths of its `requests`
+ * (rows of block_table, whose first ceil(seq_lens / block_size) entries are pages) and the
+ * step's new tokens, on the device. All integers are 32-bit but positions and slots.
+ *  - finished[r] != 0 (finished may be NULL): row r's pages go behind the free ones,
+ *    free_pages[num_free ..], in the order of the rows, and its length becomes 0. A row
+ *    whose pages would pass num_pages stays, and is granted nothing.
+ *  - cu_seqlens (requests + 1): where the rows' new tokens begin, clamped to num_tokens.
+ *  - granted[r] = 1: the tokens fit num_tokens and the table's width, and either need no new
+ *    page or are among the first rows that do whose needs the free pages serve together.
+ *    Pages are taken from the free ones' end: the first from free_pages[n - 1], n free
+ *    pages; they are written behind the row's. seq_lens_out[r] grows by the new tokens.
+ *  - positions, slots (num_tokens): of every token; slot -1 where nothing was granted, position
+ *    0 and slot -1 behind the last token.
+ *  - num_free_out: the free pages left.
+ * Negative lengths, and those past the table's width, are granted nothing. seq_lens_out and
+ * num_free_out may be seq_lens and num_free; no other arrays overlap. The workspace is
+ * fp_steps_workspace_bytes() bytes, 4-byte aligned. */
+typedef struct fp_steps_args {
+    const int32_t* seq_lens;
+    const int32_t* new_lens;
+    const uint8_t* finished;
+    int32_t* block_table;
+    int64_t table_stride;     /* entries between rows */
+    int32_t* free_pages;      /* room for num_pages */
+    const int32_t* num_free;  /* one entry */
+    int32_t* seq_lens_out;
+    int32_t* num_free_out;
+    int32_t* cu_seqlens;
+    int64_t* positions;
+    int64_t* slots;
+    int32_t* granted;
+    int64_t num_tokens;
+    int32_t requests, table_width, num_pages, block_size;
+} fp_steps_args;
+size_t fp_steps_workspace_bytes(const fp_steps_args* a); /* 0: none needed, or invalid */
+int fp_build_step_tables(const fp_steps_args* a, void* workspace, void* stream);
+
 /* Copy the device status word to the host (synchronises `stream`). */
 int fp_read_status(const fp_problem* p, void* workspace, void* stream, uint32_t* status);
 
