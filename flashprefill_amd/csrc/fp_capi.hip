@@ -662,11 +662,11 @@ fp::KvCacheArgs cache_args(const fp_kv_cache_args* a) {
 // d = 128: 1, 32 and 128 sequences of 333 tokens 13.8, 18.5 and 37 us and 8.2, 10.5 and
 // 27; of 1,000 tokens 12.3, 23 and 71, and 12.0, 17 and 65; of 2,000 tokens 12.7, 39 and
 // 117, and 18, 32 and 114.
-// heads: KV heads of a segment.
+// heads: KV heads of a segment; most: workgroups that share the keys.
 int paged8_heads(const fp_paged_args* a) {
   return a->head_dim == 64 && a->num_kv_heads % 2 == 0 ? 2 : 1;
 }
-PagedSplit paged8_split(const fp_paged_args* a, int heads, int* unit) {
+PagedSplit paged8_split(const fp_paged_args* a, int heads, int most, int* unit) {
   constexpr int kWhole = 1024;
   PagedSplit r = paged_split(a);
   *unit = 128;
@@ -690,7 +690,7 @@ PagedSplit paged8_split(const fp_paged_args* a, int heads, int* unit) {
   if (longest <= kWhole) *unit = 1 << 30;
   while (*unit < 1 << 30 && units() >= int64_t(1) << 31) *unit *= 2;
   r.nc = static_cast<int>(longest <= kWhole ? segs
-                                            : std::min<int64_t>(fp::kPaged8Groups, units()));
+                                            : std::min<int64_t>(most, units()));
   if (longest > kWhole) r.bytes = static_cast<size_t>(r.nc) * 2 * 16 * heads * (a->head_dim + 2) * 4;
   return r;
 }
@@ -753,9 +753,9 @@ int scales_valid(const fp_kv_scales& s, const char* what) {
 }
 
 // The split and the argument block of a call over an 8- or 4-bit cache.
-int paged8_args(const fp_paged_args* a, int heads, const fp_kv_scales& ks, const fp_kv_scales& vs,
-                void* ws, fp::Paged8Args* r, PagedSplit* sp) {
-  *sp = paged8_split(a, heads, &r->unit);
+int paged8_args(const fp_paged_args* a, int heads, int most, const fp_kv_scales& ks,
+                const fp_kv_scales& vs, void* ws, fp::Paged8Args* r, PagedSplit* sp) {
+  *sp = paged8_split(a, heads, most, &r->unit);
   // (the merge's launch holds fewer than 2^32 threads, 1024 for each head of a segment)
   if (!sp->many && sp->tiles * a->num_kv_heads >= int64_t(1) << 22)
     return fail(FP_E_UNSUPPORTED, "paged: %lld tiles of query rows in one call",
@@ -953,9 +953,18 @@ int paged4_valid(const fp_paged_int4_args* a) {
   return fixed_valid(a->v_scale, "paged");
 }
 
+// Workgroups that share a 4-bit call's keys: what the card holds, three for each CU up to
+// head_dim 128 and two at 256 (32 sequences of 300 .. 15,000 tokens, 8 KV heads of 128: 63 us
+// with three, 69 with two, 71 with four in turn).
+int paged4_groups(int head_dim) { return head_dim == 256 ? 512 : 768; }
+
 // A 4-bit call is split as an 8-bit one, but that a segment of few rows serves as many KV
-// heads as make up a cache line of 128 bytes.
+// heads as make up a cache line of 128 bytes, unless segments are whole and too few to fill
+// the card even one by one (one sequence of 333 tokens, 8 KV heads of 128, two of them to a
+// segment: 15 us instead of 10).
 int paged4_heads(const fp_paged_args* a) {
+  const int64_t longest = static_cast<int64_t>(a->table_width) * a->block_size;
+  if (longest <= 1024 && paged_split(a).tiles * a->num_kv_heads <= 512) return 1;
   int heads = 1;
   while (heads < 256 / a->head_dim && a->num_kv_heads % (2 * heads) == 0) heads *= 2;
   return heads;
@@ -1175,7 +1184,7 @@ int fp_paged_attention(const fp_paged_args* a, void* ws, void* stream) {
 
 size_t fp_paged_fp8_workspace_bytes(const fp_paged_fp8_args* a) {
   int unit;
-  return paged8_valid(a) == FP_OK ? paged8_split(&a->base, paged8_heads(&a->base), &unit).bytes : 0;
+  return paged8_valid(a) == FP_OK ? paged8_split(&a->base, paged8_heads(&a->base), fp::kPaged8Groups, &unit).bytes : 0;
 }
 
 int fp_paged_attention_fp8(const fp_paged_fp8_args* a, void* ws, void* stream) {
@@ -1184,7 +1193,8 @@ int fp_paged_attention_fp8(const fp_paged_fp8_args* a, void* ws, void* stream) {
   if (a->base.num_tokens == 0) return FP_OK;
   fp::Paged8Args r;
   PagedSplit sp;
-  const int prc = paged8_args(&a->base, paged8_heads(&a->base), a->k_scale, a->v_scale, ws, &r, &sp);
+  const int prc = paged8_args(&a->base, paged8_heads(&a->base), fp::kPaged8Groups, a->k_scale, a->v_scale,
+                              ws, &r, &sp);
   if (prc != FP_OK) return prc;
   if (!r.vs.slot) {
     r.a.vscale = r.vs.p;
@@ -1274,7 +1284,7 @@ int fp_kv_cache_gather_int4(const fp_kv_gather_int4_args* a, void* stream) {
 
 size_t fp_paged_int4_workspace_bytes(const fp_paged_int4_args* a) {
   int unit;
-  return paged4_valid(a) == FP_OK ? paged8_split(&a->base, paged4_heads(&a->base), &unit).bytes : 0;
+  return paged4_valid(a) == FP_OK ? paged8_split(&a->base, paged4_heads(&a->base), paged4_groups(a->base.head_dim), &unit).bytes : 0;
 }
 
 int fp_paged_attention_int4(const fp_paged_int4_args* a, void* ws, void* stream) {
@@ -1283,7 +1293,7 @@ int fp_paged_attention_int4(const fp_paged_int4_args* a, void* ws, void* stream)
   const int heads = paged4_heads(&a->base);
   fp::Paged4Args r;
   PagedSplit sp;
-  if ((rc = paged8_args(&a->base, heads, a->k_scale, a->v_scale, ws, &r.p, &sp)) != FP_OK) return rc;
+  if ((rc = paged8_args(&a->base, heads, paged4_groups(a->base.head_dim), a->k_scale, a->v_scale, ws, &r.p, &sp)) != FP_OK) return rc;
   r.p.a.vscale = r.p.vs.p;
   r.p.a.vscale_head = r.p.vs.sh;
   r.kg = groups(a->k_groups);

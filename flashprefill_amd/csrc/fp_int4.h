@@ -58,41 +58,45 @@ __device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b) {
   return __builtin_amdgcn_perm(b, a, I ? 0x07060302u : 0x05040100u);
 }
 
+// Pointers of global memory, also where the compiler cannot see that they are (a load of
+// an unknown space waits with LDS)
+typedef const __attribute__((address_space(1))) uint8_t* gbytes;
+typedef const __attribute__((address_space(1))) uint16_t* gwords;
+__device__ __forceinline__ gbytes in_global(const uint8_t* p) { return (gbytes)(p); }
+__device__ __forceinline__ gwords in_global(const uint16_t* p) { return (gwords)(p); }
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+// N words of 32 bits (1, 2 or a multiple of 4) from P, in one load for each four
+template <int N, typename P>
+__device__ __forceinline__ void load32(P p, uint32_t (&w)[N]) {
+  if constexpr (N == 1) {
+    w[0] = *(const __attribute__((address_space(1))) uint32_t*)(p);
+  } else if constexpr (N == 2) {
+    const u32x2 x = *(const __attribute__((address_space(1))) u32x2*)(p);
+    w[0] = x[0]; w[1] = x[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const u32x4 x = *((const __attribute__((address_space(1))) u32x4*)(p) + i / 4);
+      w[i] = x[0]; w[i + 1] = x[1]; w[i + 2] = x[2]; w[i + 3] = x[3];
+    }
+  }
+}
 // A piece of a key, NB = d / 32 words: bytes 4 NB p .. 4 NB (p + 1) - 1, dims
 // 32 j + 8 p .. + 7 of every group j.
-template <int NB>
-__device__ __forceinline__ void load_piece(const uint8_t* p, uint32_t (&w)[NB]) {
-  if constexpr (NB == 2) {
-    const uint2 x = *reinterpret_cast<const uint2*>(p);
-    w[0] = x.x; w[1] = x.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < NB / 4; ++i) {
-      const uint4 x = ld16(p + 16 * i);
-      w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
-    }
-  }
+template <int NB, typename P>
+__device__ __forceinline__ void load_piece(P p, uint32_t (&w)[NB]) {
+  load32<NB>(p, w);
 }
 // N group words (a multiple of 2)
-template <int N>
-__device__ __forceinline__ void load_words(const uint16_t* p, uint32_t (&w)[N / 2]) {
-  if constexpr (N == 2) {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  } else if constexpr (N == 4) {
-    const uint2 x = *reinterpret_cast<const uint2*>(p);
-    w[0] = x.x; w[1] = x.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N / 8; ++i) {
-      const uint4 x = ld16(p + 8 * i);
-      w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
-    }
-  }
+template <int N, typename P>
+__device__ __forceinline__ void load_words(P p, uint32_t (&w)[N / 2]) {
+  load32<N / 2>(p, w);
 }
-// Group j of a piece as 8 fp16 numbers, dims 32 j + 8 p + {0, 2, 1, 3, 4, 6, 5, 7}
+// Group j of a piece as 8 fp16 numbers, dims 32 j + 8 p + {0, 2, 1, 3, 4, 6, 5, 7}, by the
+// group's step (in both halves)
 template <int NB>
-__device__ __forceinline__ uint4 piece_group(const uint32_t (&w)[NB], const uint32_t (&g)[NB / 2],
-                                             int j, const Int4Consts& k) {
+__device__ __forceinline__ uint4 piece_group(const uint32_t (&w)[NB], const Step2& s, int j,
+                                             const Int4Consts& k) {
   uint32_t h[2];  // groups j & ~1 and j | 1 of dim pairs 0, 1 and of 2, 3
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -103,11 +107,17 @@ __device__ __forceinline__ uint4 piece_group(const uint32_t (&w)[NB], const uint
       h[i] = j & 2 ? halves<1>(a, b) : halves<0>(a, b);
     }
   }
-  const Step2 s = steps(j & 1 ? halves<1>(g[j >> 1], g[j >> 1]) : halves<0>(g[j >> 1], g[j >> 1]), k);
   return j & 1 ? make_uint4(values2<2>(h[0], s, k), values2<3>(h[0], s, k), values2<2>(h[1], s, k),
                             values2<3>(h[1], s, k))
                : make_uint4(values2<0>(h[0], s, k), values2<1>(h[0], s, k), values2<0>(h[1], s, k),
                             values2<1>(h[1], s, k));
+}
+// the same from all of the key's group words
+template <int NB>
+__device__ __forceinline__ uint4 piece_group(const uint32_t (&w)[NB], const uint32_t (&g)[NB / 2],
+                                             int j, const Int4Consts& k) {
+  return piece_group<NB>(
+      w, steps(j & 1 ? halves<1>(g[j >> 1], g[j >> 1]) : halves<0>(g[j >> 1], g[j >> 1]), k), j, k);
 }
 
 }  // namespace fp

@@ -7,8 +7,11 @@
 // No cached value is rounded on the way: u enters v_mfma_f32_*_f16 as it is, whatever the
 // type of q. bf16 queries become fp16 ones times a power of two f that takes their row's
 // largest finite element to 2^13 .. 2^14: exactly, but for elements below 2^-39 of it,
-// whose last bits fp16's subnormals lose. P enters as P 2^15 (few rows: two fp16 parts, the
-// second of what the first lost), of which fp16 holds all above 2^-39 of m's exponent.
+// whose last bits fp16's subnormals lose. P enters as P 2^15 (many rows: up to P 2^15),
+// rounded to fp16 once: 2^-11 of each product, as much as rounding the output to fp16 may
+// lose (to bf16 2^-8) and less than a fiftieth of what rounding to 4 bits lost of the
+// cached value; a second part, of what the first lost, would cost few rows 20 of 290
+// vector instructions and many rows half as many MFMAs as P.V takes. l sums the rounded P.
 #include "fp_int4.h"
 #include "fp_paged_segments.h"
 
@@ -34,25 +37,22 @@ __device__ __forceinline__ uint4 query8(uint4 x, bool bf, float f) {
   return make_uint4(pack2<F16>(y[0], y[2]), pack2<F16>(y[1], y[3]), pack2<F16>(y[4], y[6]),
                     pack2<F16>(y[5], y[7]));
 }
-// largest finite magnitude of 8 bf16 elements and m
-__device__ __forceinline__ float most8(uint4 x, float m) {
+// Exponent fields of 8 bf16 elements, in both halves: one more than the largest that is not
+// infinite or NaN (those wrap to the smallest 16-bit integer), and than m's
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ i16x2 exponents8(uint4 x, i16x2 m) {
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float a = fabsf(__uint_as_float(w[e] << 16));
-    const float b = fabsf(__uint_as_float(w[e] & 0xffff0000u));
-    m = fmaxf(m, a < INFINITY ? a : 0.0f);
-    m = fmaxf(m, b < INFINITY ? b : 0.0f);
+    const i16x2 f = __builtin_bit_cast(i16x2, w[e] & 0x7f807f80u) + i16x2{0x80, 0x80};
+    m = __builtin_elementwise_max(m, f);
   }
   return m;
 }
-// log2 of a bf16 row's factor; rows below 2^-106 keep that of 2^-106
-__device__ __forceinline__ int row_exponent(float most) {
-  return 13 - max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -106);
-}
-__device__ __forceinline__ uint16_t round16(float x, bool bf) {
-  return bf ? BF16::from_f32(x) : F16::from_f32(x);
-}
+// log2 of a bf16 row's factor, from its lanes' exponents; rows below 2^-106 keep that of
+// 2^-106
+__device__ __forceinline__ int row_exponent(i16x2 m) { return (max(m.x, m.y) >> 7) - 1; }
+__device__ __forceinline__ int factor_exponent(int biased) { return 13 - max(biased - 127, -106); }
 __device__ __forceinline__ uint32_t round2(float a, float b, bool bf) {
   return bf ? pack2<BF16>(a, b) : pack2<F16>(a, b);
 }
@@ -75,6 +75,21 @@ __device__ __forceinline__ float piece_dot(const uint32_t (&w)[NB], const uint32
 // ---------------------------------------------------------------------------
 // Few rows
 // ---------------------------------------------------------------------------
+// What a wave's lanes pass each other through LDS: its LDS operations are carried out in
+// their order, so that only the compiler has to keep it.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+__device__ __forceinline__ void put(uint2* p, const Step2& s) {
+  *p = make_uint2(__builtin_bit_cast(uint32_t, s.s), __builtin_bit_cast(uint32_t, s.off));
+}
+__device__ __forceinline__ void get2(const uint2* p, Step2& a, Step2& b) {
+  const uint4 x = *reinterpret_cast<const uint4*>(p);
+  a = Step2{__builtin_bit_cast(f16x2, x.x), __builtin_bit_cast(f16x2, x.y)};
+  b = Step2{__builtin_bit_cast(f16x2, x.z), __builtin_bit_cast(f16x2, x.w)};
+}
+
 // As k_paged8: four waves take 32 keys in turn, a round ahead of their use, straight from
 // the pages into registers.
 //
@@ -91,16 +106,24 @@ __device__ __forceinline__ float piece_dot(const uint32_t (&w)[NB], const uint32
 // up 64 of them at a time, one per lane, and reads a tile's place from its lane. Other
 // pages look up every key's.
 template <int D, bool P16, int HP>
-__global__ __launch_bounds__(256, 2) void k_paged4(Paged4Args pa4) {
+__global__ __launch_bounds__(256, D == 256 ? 2 : 3) void k_paged4(Paged4Args pa4) {
   constexpr int NB = D / 32;  // groups, MFMA k-steps over the head dim
   constexpr int GW = NB / 2;  // words of 32 bits of a key's groups
+  constexpr int KG = NB == 8 ? 2 : 1;  // groups of a key that a lane makes steps of
+  constexpr int TR = 2;                // 16-key tiles of a wave's round
+  constexpr int VG = TR * NB >= 8 ? TR * NB / 8 : 1;  // groups of a pair of keys that a lane makes steps of
+  constexpr int VL = NB / VG;          // lanes for a pair
   constexpr int E = D / 16;
   constexpr int VW = NB < 4 ? 1 : NB / 4;  // words of 32 bits of V's bytes per lane and key
   constexpr int OS = D + 4;   // padded row of the merge buffer (floats)
   constexpr int NW = 4 / HP;  // waves of a head
-  constexpr int RK = 32 * NW;  // keys of a round, all waves of a head
+  constexpr int RK = 16 * TR * NW;  // keys of a round, all waves of a head
   __shared__ float sm[4][16][OS];
   __shared__ float sml[4][16][2];
+  // a round's steps: of key r of tile j, of the keys 2 i, 2 i + 1 that a row of 16 lanes
+  // multiplies (s of both, (z - 16) s of both)
+  __shared__ __align__(16) uint2 ksteps[4][TR][16][NB];
+  __shared__ __align__(16) uint2 vsteps[4][4][2 * TR][NB];
   const Paged8Args& pa = pa4.p;
   const PagedArgs& a = pa.a;
   const Work work = find_work(pa, static_cast<int>(blockIdx.x), -1);
@@ -132,27 +155,40 @@ __global__ __launch_bounds__(256, 2) void k_paged4(Paged4Args pa4) {
     const bool rvalid = rr < nq * a.G;
     const int qi = rvalid ? rr / a.G : 0;
     const int lim = rvalid ? nk - nq + qi : nk - 1;
-    f16x8 qb[NB];
-    float scale = a.scale_log2 * fixed_scale(pa.ks, h);
+    uint4 qx[NB];  // (made fp16 numbers once the first keys are on their way)
     {
       const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (sq.q0 + qi) * a.qst +
                            static_cast<int64_t>(h * a.G + (rvalid ? rr % a.G : 0)) * a.qhs + 8 * g;
-      uint4 x[NB];
-      float most = 0.0f;
 #pragma unroll
-      for (int j = 0; j < NB; ++j) x[j] = rvalid ? ld16(qp + 32 * j) : zero4();
-      float f = 1.0f;
-      if (bf) {
-#pragma unroll
-        for (int j = 0; j < NB; ++j) most = most8(x[j], most);
-        const int e = row_exponent(row4_max(most));
-        f = __builtin_amdgcn_ldexpf(1.0f, e);
-        scale *= __builtin_amdgcn_ldexpf(1.0f, -e);
-      }
-#pragma unroll
-      for (int j = 0; j < NB; ++j) qb[j] = as_vec8<F16>(query8(x[j], bf, f));
+      for (int j = 0; j < NB; ++j) qx[j] = ld16(qp + 32 * j);
     }
 
+    f16x8 qb[NB];
+    float scale = a.scale_log2 * fixed_scale(pa.ks, h);
+    auto make_q = [&]() {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) qx[j] = rvalid ? qx[j] : zero4();
+      float f = 1.0f;
+      if (scale < 0.0f) {  // (the sign goes into q, so that the largest score is the largest S)
+        f = -1.0f;
+        scale = -scale;
+      }
+      if (bf) {
+        i16x2 most{};
+#pragma unroll
+        for (int j = 0; j < NB; ++j) most = exponents8(qx[j], most);
+        // (as floats: small integers)
+        const int e = factor_exponent(
+            static_cast<int>(row4_max(static_cast<float>(row_exponent(most)))));
+        f = __builtin_amdgcn_ldexpf(f, e);
+        scale *= __builtin_amdgcn_ldexpf(1.0f, -e);
+      }
+      // (not 0, by which a masked score would be NaN: by 2^-149 no score reaches 2^-100)
+      if (scale == 0.0f) scale = 0x1p-149f;
+#pragma unroll
+      for (int j = 0; j < NB; ++j) qb[j] = as_vec8<F16>(query8(qx[j], bf, f));
+    };
+    if constexpr (D == 256) make_q();  // (no registers to hold them in)
     f32x4 acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = f32x4{};
@@ -164,11 +200,17 @@ __global__ __launch_bounds__(256, 2) void k_paged4(Paged4Args pa4) {
     const uint16_t* kg = pa4.kg.p + h * pa4.kg.sh;
     const uint16_t* vg = pa4.vg.p + h * pa4.vg.sh;
 
-    // what a round loads: 32 keys, lanes as above
+    // what a round loads: 32 keys, lanes as above. A lane takes the words of its share of
+    // the groups only (kj .. of key r, vj .. of the pair of keys vi of its row of 16 lanes)
+    // and passes their steps to the others through LDS: each for itself needs five
+    // instructions for every group of every key, a quarter of the loop's.
     struct {
-      uint32_t k[2][NB], kg[2][GW];
-      uint32_t v[2][4][VW], vg[2][4 * GW];
+      uint32_t k[TR][NB], kg[TR];
+      uint32_t v[TR][4][VW], vg[2];  // (vg: of a key and the next, combined when they are used)
     } r;
+    const int kj = KG * g & (NB - 1);
+    const int vi = r16 / VL % (2 * TR), vj = VG * (r16 % VL);
+    const int vkey = 16 * (vi >> 1) + 4 * g + 2 * (vi & 1);  // of the round
     // places of the 64 16-key tiles from key `win`, one per lane (P16; tiles past the
     // sequence repeat the last one, their scores are masked)
     int win = k0;
@@ -190,95 +232,143 @@ __global__ __launch_bounds__(256, 2) void k_paged4(Paged4Args pa4) {
               __builtin_amdgcn_readlane(static_cast<int>(x >> 32), tile))) << 32 |
           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), tile)));
     };
+    // A scalar base that the compiler does not take apart: with it a load takes a 32-bit offset
+    // of the lane's; else the loop holds 64-bit sums of the heads' bases and the offsets, and
+    // adds tiles' places to them (11 instructions and 20 registers).
+    auto at_tile = [&](const auto* head, int64_t x, int tile) {
+      auto p = in_global(head + place(x, tile));
+      asm volatile("" : "+s"(p));
+      return p;
+    };
     // a lane's offsets in a tile
     const uint32_t koff = static_cast<uint32_t>(r16 * static_cast<int>(a.kcs) + 4 * NB * g);
+    const uint32_t kgoff = static_cast<uint32_t>(r16 * NB + kj);
     uint32_t voff[4];
 #pragma unroll
     for (int v = 0; v < 4; ++v)
       voff[v] = static_cast<uint32_t>((4 * g + v) * static_cast<int>(a.vcs) + NB * r16);
+    auto load_group = [&](auto p, uint32_t& x, auto n) {
+      if constexpr (decltype(n)::value == 2) {
+        uint32_t y[1];
+        load32<1>(p, y);
+        x = y[0];
+      } else {
+        x = *(gwords)(p);
+      }
+    };
     auto load_k = [&](int base) {
       if constexpr (P16) {
         if (base >= win + 1024) look(k0 + ((base - k0) & ~1023));
       }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < TR; ++j) {
         if constexpr (P16) {
           const int tile = ((base - win) >> 4) + j;
-          load_piece<NB>(kc + place(kat, tile) + koff, r.k[j]);
-          load_words<NB>(kg + place(kgat, tile) + r16 * NB, r.kg[j]);
+          load_piece<NB>(at_tile(kc, kat, tile) + koff, r.k[j]);
+          load_group(at_tile(kg, kgat, tile) + kgoff, r.kg[j], IntC<KG>{});
         } else {
           const int key = min(base + 16 * j + r16, nk - 1);
           const int64_t pg = paged_page<false>(a, row, key, bad);
           const int in = key % a.bs;
           load_piece<NB>(kc + pg * a.kcb + static_cast<int64_t>(in) * a.kcs + 4 * NB * g, r.k[j]);
-          load_words<NB>(kg + pg * pa4.kg.sb + static_cast<int64_t>(in) * NB, r.kg[j]);
+          load_group(kg + pg * pa4.kg.sb + static_cast<int64_t>(in) * NB + kj, r.kg[j], IntC<KG>{});
         }
       }
     };
     auto load_v = [&](int base) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < TR; ++j) {
         const int tile = ((base - win) >> 4) + j;
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const uint8_t* p;
+          gbytes p;
           if constexpr (P16) {
-            p = vc + place(vat, tile) + voff[v];
+            p = at_tile(vc, vat, tile) + voff[v];
           } else {
             const int key = min(base + 16 * j + 4 * g + v, nk - 1);
             const int64_t pg = paged_page<false>(a, row, key, bad);
             const int in = key % a.bs;
-            p = vc + pg * a.vcb + static_cast<int64_t>(in) * a.vcs + NB * r16;
-            uint32_t x[GW];
-            load_words<NB>(vg + pg * pa4.vg.sb + static_cast<int64_t>(in) * NB, x);
-#pragma unroll
-            for (int q = 0; q < GW; ++q) r.vg[j][GW * v + q] = x[q];
+            p = in_global(vc + pg * a.vcb + static_cast<int64_t>(in) * a.vcs + NB * r16);
           }
-          if constexpr (NB == 2) {
-            r.v[j][v][0] = *reinterpret_cast<const uint16_t*>(p);
-          } else if constexpr (NB == 4) {
-            r.v[j][v][0] = *reinterpret_cast<const uint32_t*>(p);
-          } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(p);
-            r.v[j][v][0] = x.x; r.v[j][v][1] = x.y;
-          }
+          if constexpr (NB == 2) r.v[j][v][0] = *(gwords)(p);
+          else load32<VW>(p, r.v[j][v]);
         }
-        if constexpr (P16) load_words<4 * NB>(vg + place(vgat, tile) + 4 * g * NB, r.vg[j]);
       }
+      // (two keys, vkey and the next, in the halves of a word for each group)
+      const uint16_t* w0;
+      const uint16_t* w1;
+      if constexpr (P16) {
+        const int64_t at = shfl64(vgat, ((base - win) >> 4) + (vi >> 1));
+        w0 = vg + at + ((vkey & 15) * NB + vj);
+        w1 = w0 + NB;
+      } else {
+        const int key0 = min(base + vkey, nk - 1), key1 = min(base + vkey + 1, nk - 1);
+        w0 = vg + paged_page<false>(a, row, key0, bad) * pa4.vg.sb +
+             static_cast<int64_t>(key0 % a.bs) * NB + vj;
+        w1 = vg + paged_page<false>(a, row, key1, bad) * pa4.vg.sb +
+             static_cast<int64_t>(key1 % a.bs) * NB + vj;
+      }
+      load_group(w0, r.vg[0], IntC<VG>{});
+      load_group(w1, r.vg[1], IntC<VG>{});
     };
-    f32x4 s[2];
+    int base = k0 + 16 * TR * kw;
+    if (base < k1) {
+      if constexpr (P16) look(k0);
+      load_k(base);
+      load_v(base);
+    }
+    // what comes behind this sequence, on its way too
+    const bool on = left > take, last_seg = seg + 1 == tiles * pa.groups;
+    PagedSeq next = sq;
+    if constexpr (D < 256) {
+      if (on && last_seg) next = paged_seq(a, b + 1);
+    }
+    if constexpr (D < 256) make_q();
+    f32x4 s[TR];
     auto scores = [&]() {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < TR; ++j) {
+        put(&ksteps[w][j][r16][kj], steps(halves<0>(r.kg[j], r.kg[j]), k4));
+        if constexpr (KG == 2)
+          put(&ksteps[w][j][r16][kj + 1], steps(halves<1>(r.kg[j], r.kg[j]), k4));
+      }
+      wave_fence();
+#pragma unroll
+      for (int j = 0; j < TR; ++j) {
+        Step2 st[NB];
+#pragma unroll
+        for (int i = 0; i < NB; i += 2) get2(&ksteps[w][j][r16][i], st[i], st[i + 1]);
         s[j] = f32x4{};
 #pragma unroll
         for (int i = 0; i < NB; ++i)
-          s[j] = mfma16(as_vec8<F16>(piece_group<NB>(r.k[j], r.kg[j], i, k4)), qb[i], s[j]);
-#pragma unroll
-        for (int v = 0; v < 4; ++v) s[j][v] *= scale;
+          s[j] = mfma16(as_vec8<F16>(piece_group<NB>(r.k[j], st[i], i, k4)), qb[i], s[j]);
       }
+      wave_fence();
     };
     auto softmax_pv = [&](int base) {
-      if (base + 31 > nk - nq) {  // some row's causal limit or the end lies in this round
+      if (base + 16 * TR - 1 > nk - nq) {  // some row's causal limit or the end lies in this round
         asm volatile("");  // (a branch: as selects they would be in every round)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < TR; ++j)
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             const int key = base + 16 * j + 4 * g + v;
             if (key > lim) s[j][v] = -INFINITY;
-            if (key >= nk) {  // slots past the end may hold anything: a step of 0
-#pragma unroll
-              for (int q = 0; q < GW; ++q) r.vg[j][GW * v + q] = 0u;
-            }
           }
+        // slots past the end may hold anything: a step of 0
+        if (base + vkey >= nk) r.vg[0] = 0u;
+        if (base + vkey + 1 >= nk) r.vg[1] = 0u;
       }
+      put(&vsteps[w][g][vi][vj], steps(halves<0>(r.vg[0], r.vg[1]), k4));
+      if constexpr (VG == 2)
+        put(&vsteps[w][g][vi][vj + 1], steps(halves<1>(r.vg[0], r.vg[1]), k4));
+      wave_fence();
       float mx = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < TR; ++j)
 #pragma unroll
         for (int v = 0; v < 4; ++v) mx = fmaxf(mx, s[j][v]);
-      const float m_new = fmaxf(m_run, row4_max(mx));
+      const float m_new = fmaxf(m_run, row4_max(mx) * scale);
       if (__ballot(m_new > m_run) != 0) {
         // rows with no visible key yet keep m = -inf: their factors are 0
         const float ms = m_new == -INFINITY ? 0.0f : m_new;
@@ -292,59 +382,52 @@ __global__ __launch_bounds__(256, 2) void k_paged4(Paged4Args pa4) {
       }
       const float ms = m_run == -INFINITY ? 0.0f : m_run - kPScale;
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < TR; ++j)
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          s[j][v] = __builtin_amdgcn_exp2f(s[j][v] - ms);
-          l_part += s[j][v];
+          s[j][v] = __builtin_amdgcn_exp2f(fmaf(s[j][v], scale, -ms));
         }
-      uint32_t hi[4], lo[4];  // keys 2 i, 2 i + 1 of this lane
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x0 = s[i >> 1][2 * (i & 1)], x1 = s[i >> 1][2 * (i & 1) + 1];
-        hi[i] = pack2<F16>(x0, x1);
-        lo[i] = pack2<F16>(x0 - F16::to_f32(static_cast<uint16_t>(hi[i])),
-                           x1 - F16::to_f32(static_cast<uint16_t>(hi[i] >> 16)));
-      }
-      const f16x8 ph = as_vec8<F16>(make_uint4(hi[0], hi[1], hi[2], hi[3]));
-      const f16x8 pl = as_vec8<F16>(make_uint4(lo[0], lo[1], lo[2], lo[3]));
+      for (int jj = 0; jj < TR; jj += 2) {  // 32 keys
+        uint32_t pw[4];  // keys 2 i, 2 i + 1 of this lane
 #pragma unroll
-      for (int q = 0; q < GW; ++q) {  // groups 2 q and 2 q + 1
-        uint32_t hv[4];
-        Step2 st[2][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {  // a pair of keys
-          const int jt = i >> 1, va = 2 * (i & 1);
-          const uint32_t xa = r.v[jt][va][q >> 1], xb = r.v[jt][va + 1][q >> 1];
-          hv[i] = q & 1 ? halves<1>(xa, xb) : halves<0>(xa, xb);
-          const uint32_t ga = r.vg[jt][GW * va + q], gb = r.vg[jt][GW * (va + 1) + q];
-          st[0][i] = steps(halves<0>(ga, gb), k4);
-          st[1][i] = steps(halves<1>(ga, gb), k4);
+        for (int i = 0; i < 4; ++i) {
+          pw[i] = pack2<F16>(s[jj + (i >> 1)][2 * (i & 1)], s[jj + (i >> 1)][2 * (i & 1) + 1]);
+          l_part = add_pair<F16>(pw[i], l_part);
         }
-        auto pv = [&](auto nc) {
-          constexpr int N = decltype(nc)::value;
-          uint32_t x[4];
+        const f16x8 pb = as_vec8<F16>(make_uint4(pw[0], pw[1], pw[2], pw[3]));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = values2<N>(hv[i], st[N >> 1][i], k4);
-          const f16x8 va = as_vec8<F16>(make_uint4(x[0], x[1], x[2], x[3]));
-          acc[4 * q + N] = mfma16(va, pl, acc[4 * q + N]);
-          acc[4 * q + N] = mfma16(va, ph, acc[4 * q + N]);
-        };
-        pv(IntC<0>{});
-        pv(IntC<1>{});
-        pv(IntC<2>{});
-        pv(IntC<3>{});
+        for (int q = 0; q < GW; ++q) {  // groups 2 q and 2 q + 1
+          uint32_t hv[4];
+          Step2 st[2][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {  // a pair of keys
+            const int jt = jj + (i >> 1), va = 2 * (i & 1);
+            const uint32_t xa = r.v[jt][va][q >> 1], xb = r.v[jt][va + 1][q >> 1];
+            hv[i] = q & 1 ? halves<1>(xa, xb) : halves<0>(xa, xb);
+            get2(&vsteps[w][g][2 * jj + i][2 * q], st[0][i], st[1][i]);
+          }
+          auto pv = [&](auto nc) {
+            constexpr int N = decltype(nc)::value;
+            uint32_t x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = values2<N>(hv[i], st[N >> 1][i], k4);
+            const f16x8 va = as_vec8<F16>(make_uint4(x[0], x[1], x[2], x[3]));
+            acc[4 * q + N] = mfma16(va, pb, acc[4 * q + N]);
+          };
+          pv(IntC<0>{});
+          pv(IntC<1>{});
+          pv(IntC<2>{});
+          pv(IntC<3>{});
+        }
       }
+      wave_fence();
     };
 
     // A round's keys are loaded while the one before is used, its values after that: the
     // last round, which loads nothing, stands apart, since with the loads under a branch
     // the compiler waits for all of them at the next use. The steps are kept in order.
-    int base = k0 + 32 * kw;
     if (base < k1) {
-      if constexpr (P16) look(k0);
-      load_k(base);
-      load_v(base);
       for (; base + RK < k1; base += RK) {
         scores();
         __builtin_amdgcn_sched_barrier(0);
@@ -376,8 +459,8 @@ __global__ __launch_bounds__(256, 2) void k_paged4(Paged4Args pa4) {
         asm volatile("" : "+v"(lane2));
         const int g2 = (lane2 >> 4) & 3;
 #pragma unroll 1
-        for (int i = 0; i < 32 * ((k1 - k0 + RK - 1) / RK); ++i) {
-          const int key = k0 + 32 * kw + RK * (i >> 5) + (i & 31);
+        for (int i = 0; i < 16 * TR * ((k1 - k0 + RK - 1) / RK); ++i) {
+          const int key = k0 + 16 * TR * kw + RK * (i / (16 * TR)) + i % (16 * TR);
           if (key >= k1) break;
           const int64_t pg = paged_page<true>(a, row, key, bad);
           const int64_t in = key % a.bs;
@@ -471,13 +554,16 @@ __global__ __launch_bounds__(256, 2) void k_paged4(Paged4Args pa4) {
         }
       }
     }
+    if (!on) return;
     left -= take;
-    if (left <= 0) return;
     u = 0;
-    if (++seg == tiles * pa.groups) {  // the next sequence with rows (there are units left)
+    ++seg;
+    if (last_seg) {  // the next sequence with rows (there are units left)
       seg = 0;
-      do sq = uniform_seq(paged_seq(a, ++b));
-      while (sq.nq == 0);
+      ++b;
+      if constexpr (D == 256) next = paged_seq(a, b);
+      sq = uniform_seq(next);
+      while (sq.nq == 0) sq = uniform_seq(paged_seq(a, ++b));
       tiles = seq_tiles(a, sq);
       units = seq_units(pa.unit, sq);
     }
@@ -487,17 +573,14 @@ __global__ __launch_bounds__(256, 2) void k_paged4(Paged4Args pa4) {
 
 template <typename T, int D, int HP>
 __global__ __launch_bounds__(1024) void k_paged4_merge(Paged8Args pa) {
-  merge_segments<T, D, HP>(pa);
+  merge_segments<T, D, HP, true>(pa);
 }
 
 // Many rows (prefill over a cached prefix): 128-row tiles as in k_paged8_rows. The 64 keys
 // of a tile are loaded into registers (16 keys by each wave, four lanes to a key, a tile
 // ahead), made fp16 numbers once per workgroup and written to LDS, in which the dims of
 // every eight lie in the order of a piece ({0, 2, 1, 3, 4, 6, 5, 7}); so do the queries',
-// and O's come out in it. P 2^7 (at most 2^15, see kStep) is rounded to fp16 once: 2^-11 of
-// each product, as much as rounding the output to fp16 may lose (to bf16 2^-8) and less than
-// a fiftieth of what rounding to 4 bits lost of the cached value; a second part would add
-// half as many MFMAs to P.V again.
+// and O's come out in it. P enters as P 2^7, at most 2^15 (see kStep).
 template <int D, bool P16>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged4_rows(Paged4Args pa4) {
   constexpr int KT = 64, TT = KT / 32;
@@ -557,10 +640,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged4_rows(Paged4Arg
 #pragma unroll
     for (int s = 0; s < KS; ++s) y[s] = rvalid ? ld16(qp + 16 * s) : zero4();
     if (bf) {
-      float most = 0.0f;
+      i16x2 most{};
 #pragma unroll
-      for (int s = 0; s < KS; ++s) most = most8(y[s], most);
-      const int e = row_exponent(pair32_max(most));
+      for (int s = 0; s < KS; ++s) most = exponents8(y[s], most);
+      const int e = factor_exponent(
+          static_cast<int>(pair32_max(static_cast<float>(row_exponent(most)))));
       f = __builtin_amdgcn_ldexpf(f, e);
       scale *= __builtin_amdgcn_ldexpf(1.0f, -e);
     }
@@ -677,14 +761,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged4_rows(Paged4Arg
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           s[t4][v] = __builtin_amdgcn_exp2f(fmaf(s[t4][v], scale, -ms));
-          l_part += s[t4][v];
         }
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           uint32_t u[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < 4; ++e) {
             u[e] = pack2<F16>(s[t4][8 * hh + 2 * e], s[t4][8 * hh + 2 * e + 1]);
+            l_part = add_pair<F16>(u[e], l_part);
+          }
           const f16x8 pb = as_vec8<F16>(make_uint4(u[0], u[1], u[2], u[3]));
           const uint16_t* sv16 = reinterpret_cast<const uint16_t*>(sv[buf]);
           const int r = 32 * t4 + 16 * hh + tr_row;
@@ -799,7 +884,11 @@ hipError_t launch_few4(const Paged4Args& p, hipStream_t s) {
   if (a.bs % 16 != 0) hipLaunchKernelGGL((k_paged4<D, false, HP>), grid, b, 0, s, p);
   else hipLaunchKernelGGL((k_paged4<D, true, HP>), grid, b, 0, s, p);
   if (a.part != nullptr) {
-    const dim3 mg(static_cast<unsigned>(p.p.segs * HP)), mb(1024);
+    // few heads and rows: as many workgroups for each as make up 256 (one sequence of 131,000,
+    // 16 rows of 2 KV heads of 64: 65 us with one workgroup for each head)
+    unsigned split = 16;
+    while (split > 1 && p.p.segs * HP * split > 256) split /= 2;
+    const dim3 mg(static_cast<unsigned>(p.p.segs * HP), split), mb(1024);
     if (p.dtype == FP_DTYPE_BF16)
       hipLaunchKernelGGL((k_paged4_merge<BF16, D, HP>), mg, mb, 0, s, p.p);
     else

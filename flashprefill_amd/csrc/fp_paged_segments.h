@@ -114,7 +114,9 @@ __device__ __forceinline__ Work find_work(const Paged8Args& pa, int wg, int64_t 
 // One head of a segment per workgroup of 16 waves: its rows' partials, weighted by
 // exp2(m - max m) and divided by their l. They are the first of workgroups w0 + 1 .. w1
 // and the first or last of w0. As many waves as there are share a row's partials.
-template <typename T, int D, int HP>
+// SPLIT: a segment's rows are shared by the gridDim.y workgroups (a power of two) of its
+// head, each of which takes every gridDim.y-th.
+template <typename T, int D, int HP, bool SPLIT = false>
 __device__ __forceinline__ void merge_segments(const Paged8Args& pa) {
   constexpr int XD = D / 64;  // dims per lane
   typedef float vec __attribute__((ext_vector_type(XD)));
@@ -129,14 +131,19 @@ __device__ __forceinline__ void merge_segments(const Paged8Args& pa) {
   const int n = __builtin_amdgcn_readfirstlane((x0 + units - 1) / work.share) - w0 + 1;
   if (n == 1) return;  // written already
   const int h = seg / tiles * HP + hh, tl = seg % tiles;
-  const int rows = min(work.s.nq * a.G - 16 * tl, 16);
+  const int first_row = SPLIT ? static_cast<int>(blockIdx.y) : 0;
+  const int row_step = SPLIT ? static_cast<int>(gridDim.y) : 1;
+  int rows = min(work.s.nq * a.G - 16 * tl, 16);
+  if constexpr (SPLIT) rows = (rows - first_row + row_step - 1) / row_step;
+  if (SPLIT && rows <= 0) return;
   const int lgr = rows > 1 ? 32 - __clz(rows - 1) : 0;  // rows as a power of two
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int row = w & ((1 << lgr) - 1), share = 16 >> lgr;
   if (row < rows) {
     const int first = 2 * w0 + (x0 != w0 * work.share);
     const auto part = [&](int j) {
-      return static_cast<int64_t>(((j == 0 ? first : 2 * (w0 + j)) * HP + hh) * 16 + row);
+      return static_cast<int64_t>(((j == 0 ? first : 2 * (w0 + j)) * HP + hh) * 16 +
+                                  first_row + row * row_step);
     };
     float M = -INFINITY;
     for (int j = lane; j < n; j += 64) M = fmaxf(M, a.ml[2 * part(j)]);
@@ -148,7 +155,7 @@ __device__ __forceinline__ void merge_segments(const Paged8Args& pa) {
       const int64_t p = part(j);
       const vec x = *reinterpret_cast<const vec*>(a.part + p * D + XD * lane);
       const float m = a.ml[2 * p], l = a.ml[2 * p + 1];
-      // (2^-10: the sum over the partials, at most 512, stays finite)
+      // (2^-10: the sum over the partials, at most 768, stays finite)
       static_assert(kPaged8Groups <= 1024, "weights");
       const float f = m == -INFINITY ? 0.0f : 0x1p-10f * __builtin_amdgcn_exp2f(m - M);
       L += m == -INFINITY ? l : f * l;
@@ -168,7 +175,7 @@ __device__ __forceinline__ void merge_segments(const Paged8Args& pa) {
       o += so[k][d];
       L += sl[k];
     }
-    const int rr = 16 * tl + r;
+    const int rr = 16 * tl + first_row + r * row_step;
     static_cast<uint16_t*>(a.o)[(work.s.q0 + rr / a.G) * a.ost +
                                 static_cast<int64_t>(h * a.G + rr % a.G) * a.ohs + d] =
         T::from_f32(o / L * vs);

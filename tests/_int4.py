@@ -104,9 +104,7 @@ def attention(q, kc, vc, kg, vg, cu, used, table, ks, vs, scale):
         pos = torch.arange(n - (q1 - q0), n).view(1, -1, 1)
         hidden = torch.arange(n).view(1, 1, -1) > pos
         p = torch.softmax(s.masked_fill(hidden, float("-inf")), -1)
-        # (a hidden key's NaN reaches nothing)
-        far = hidden.expand_as(p).transpose(1, 2)  # (1 | heads, keys, queries)
-        if v.isnan().any():
+        if v.isnan().any():  # (a hidden key's reaches nothing)
             for i in range(q1 - q0):
                 see = n - (q1 - q0) + i + 1
                 out[q0 + i] = torch.einsum("hk,khd->hd", p[:, i, :see], v[:see])
@@ -117,15 +115,15 @@ def attention(q, kc, vc, kg, vg, cu, used, table, ks, vs, scale):
     return out, size, most
 
 
-def bound(want, size, most, dtype, many):
+def bound(want, size, most, dtype):
     """What a row may differ by. The output is rounded once, half a spacing: 2^-8 of the
     value in bf16, 2^-11 in fp16 (2^-25 below fp16's normal range). Scores are fp32 sums of
     exact products: of d <= 256 terms in chains of at most 16 MFMAs, off by less than
-    2^-19 `most`, and so is P, relatively. P is held to 2^-22, by many rows to 2^-11 (fp16),
-    and sums over the keys and factors to 2^-18: all of it of sum P |v|."""
+    2^-19 `most`, and so is P, relatively. P is held to 2^-11 (fp16), and sums over the keys
+    and factors to 2^-17: all of it of sum P |v|."""
     eps = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
     least = 0.0 if dtype == torch.bfloat16 else 2.0 ** -25
-    inner = most * 2.0 ** -19 + 2.0 ** -17 + (2.0 ** -11 if many else 0.0)
+    inner = most * 2.0 ** -19 + 2.0 ** -17 + 2.0 ** -11
     return want.abs() * eps * 1.01 + size * inner + least
 
 
