@@ -255,6 +255,7 @@ struct Cache4Args {
   const int64_t* slot_mapping;
   int64_t num_slots;
   int32_t num_tokens, block_size, num_kv_heads, head_dim;
+  int32_t heads_shift, block_shift;  // log2, -1 for no power of two; set by the write's launch
 };
 
 constexpr int kRopeMaxBatch = 64;  // sequences whose offsets k_rope takes
@@ -342,7 +343,7 @@ hipError_t launch_paged8(const Paged8Args& a, int dtype, int format, int head_di
 hipError_t launch_kv_cache_write8(const Cache8Args& a, int dtype, int format, hipStream_t s);
 hipError_t launch_kv_cache_gather(const GatherArgs& a, int dtype, int format, hipStream_t s);
 hipError_t launch_kv_cache_write(const KvCacheArgs& a, hipStream_t s);
-hipError_t launch_kv_cache_write4(const Cache4Args& a, int dtype, hipStream_t s);
+hipError_t launch_kv_cache_write4(Cache4Args a, int dtype, hipStream_t s);
 // (find: the call's sequences and pages)
 hipError_t launch_kv_cache_gather4(const Cache4Args& a, const GatherArgs& find, int dtype,
                                    hipStream_t s);

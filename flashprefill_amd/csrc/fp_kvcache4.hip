@@ -6,10 +6,11 @@
 // and bases are scalars.
 //
 // The write finds each group's smallest and largest element over the four lanes and
-// quantises by the rule of fp_kv_cache_write_int4. Its quotients are rounded as a division
-// rounds them: y = x r, r about 1 / s, then y - r (y s - x), whose error before its own
-// rounding is below 2^-43 of it, and x / s (s has 4 significant bits) is either an fp32
-// number or at least 2^-29 of itself away from a midpoint of two.
+// quantises by the rule of fp_kv_cache_write_int4. A group's step is one lane's work, passed
+// to the other three. Its quotients are rounded as a division rounds them: y = x r, r about
+// 1 / s, then y - r (y s - x), whose error before its own rounding is below 2^-43 of it, and
+// x / s (s has 4 significant bits) is either an fp32 number or at least 2^-29 of itself
+// away from a midpoint of two.
 #include "fp_int4.h"
 #include "fp_kvcache_common.h"
 
@@ -21,77 +22,63 @@ __device__ __forceinline__ float quotient(float x, float y, float r) {
   return fmaf(-fmaf(q, y, -x), r, q);
 }
 
+// The larger of two numbers, as the median of them and infinity: fmaxf would first quiet
+// each, since they might be signalling NaN.
+__device__ __forceinline__ float larger(float a, float b) {
+  return __builtin_amdgcn_fmed3f(a, b, INFINITY);
+}
 // max over the four lanes of a row
 __device__ __forceinline__ float quad_max(float x) {
   const auto other = [](float v, auto ctrl) {
     return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
         0, static_cast<int>(__float_as_uint(v)), decltype(ctrl)::value, 0xf, 0xf, true)));
   };
-  x = fmaxf(x, other(x, IntC<0xb1>{}));  // lanes 1 0 3 2
-  return fmaxf(x, other(x, IntC<0x4e>{}));  // lanes 2 3 0 1
+  x = larger(x, other(x, IntC<0xb1>{}));  // lanes 1 0 3 2
+  return larger(x, other(x, IntC<0x4e>{}));  // lanes 2 3 0 1
 }
 
-// x / t rounded once, clamped to the largest magnitude that a group holds. t from 2^-60 to
-// 2^60: as above, with a second step, since t may have any bits (Markstein, Computation of
-// elementary functions on the IBM RISC System/6000, 1990); others divide.
-constexpr float kInt4Most = 16384.0f;
-struct FixedScale {
-  float t, r, most;
-  bool easy;
-  __device__ __forceinline__ explicit FixedScale(float t_) : t(t_) {
-    easy = t >= 0x1p-60f && t <= 0x1p60f;
-    r = 1.0f / t;
-    most = t * (kInt4Most * 1.001f);  // (the infinite ones, whose remainder is NaN, among them)
-  }
-  __device__ __forceinline__ float divide(float x) const {
-    if (!easy) return x / t;
-    float y = x * r;
-    y = fmaf(-fmaf(y, t, -x), r, y);
-    y = fmaf(-fmaf(y, t, -x), r, y);
-    return fabsf(x) > most ? copysignf(kInt4Most, x) : y;
-  }
-};
+// lane L of the four, in all of them
+template <int L>
+__device__ __forceinline__ float quad_from(float x) {
+  return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
+      0, static_cast<int>(__float_as_uint(x)), 0x55 * L, 0xf, 0xf, true)));
+}
 
-// One group's eight elements of a lane: codes as small floats, and the group's word
-__device__ __forceinline__ uint16_t quantise_group(float (&x)[8]) {
-  float hi = -INFINITY, low = -INFINITY, nan = 0.0f;  // low: the largest -x
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    nan = x[e] != x[e] ? 1.0f : nan;
-    x[e] = __builtin_amdgcn_fmed3f(x[e], -kInt4Most, kInt4Most);
-    hi = fmaxf(hi, x[e]);
-    low = fmaxf(low, -x[e]);
-  }
-  hi = quad_max(hi);
-  low = quad_max(low);
-  nan = quad_max(nan);
-  const float want = fmaxf(quotient(hi + low, 15.0f, 1.0f / 15.0f),
-                           quotient(fmaxf(hi, low), 56.0f, 1.0f / 56.0f));
+constexpr float kInt4Most = 16384.0f;  // the largest magnitude that a group holds
+
+// A group's step: x becomes the code rint(x / s) - z, within 0 .. 15. Where all codes are 0
+// (s = 0, or NaN), r, s and z are 0.
+struct GroupStep {
+  float s, r, z;
+  uint16_t word;
+};
+// from its largest and smallest element (the largest infinite: some element is NaN)
+__device__ __forceinline__ GroupStep group_step(float hi, float lo) {
+  const bool nan = hi == INFINITY;
+  const float want = larger(quotient(hi - lo, 15.0f, 1.0f / 15.0f),
+                            quotient(larger(hi, -lo), 56.0f, 1.0f / 56.0f));
   uint32_t m = __float_as_uint(want);  // (-0 for a group of -0: s takes the magnitude)
   m = (m + 0x7ffffu + ((m >> 20) & 1u)) & ~0xfffffu;
   const float s = fabsf(want < 0x1p-14f ? rintf(want * 0x1p17f) * 0x1p-17f : __uint_as_float(m));
-  const float some = s == 0.0f ? 1.0f : s;
-  const float r = __builtin_amdgcn_rcpf(some);
-  const float z = s == 0.0f ? 0.0f
-                            : fminf(fmaxf(rintf(quotient(-low, some, r)), -64.0f), 63.0f);
-  const bool none = s == 0.0f || nan != 0.0f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float c = __builtin_amdgcn_fmed3f(rintf(quotient(x[e], some, r)) - z, 0.0f, 15.0f);
-    x[e] = none ? 0.0f : c;
-  }
-  if (nan != 0.0f) return 0x7f80u;
-  const uint16_t bits = __builtin_bit_cast(uint16_t, static_cast<_Float16>(s));
-  return static_cast<uint16_t>(bits | static_cast<uint32_t>(static_cast<int>(z) + 64));
+  const bool none = s == 0.0f || nan;
+  const float r = __builtin_amdgcn_rcpf(s);
+  const float z = none ? 0.0f : __builtin_amdgcn_fmed3f(rintf(quotient(lo, s, r)), -64.0f, 63.0f);
+  const uint32_t bits = __builtin_bit_cast(uint16_t, static_cast<_Float16>(s));
+  return GroupStep{none ? 0.0f : s, none ? 0.0f : r, z,
+                   static_cast<uint16_t>(nan ? 0x7f80u
+                                             : bits | static_cast<uint32_t>(static_cast<int>(z) + 64))};
 }
 
+// 131,072 tokens of 8 heads of 128 with scales, 688 MB: 167 us, 4.1 TB/s (a copy's rate
+// 5.15); without the group words' 8 bytes a row, scattered over the heads' pages, 157.
 template <typename T, int NB>
 __global__ __launch_bounds__(256) void k_cache_write4(Cache4Args a) {
+  constexpr int K = NB == 8 ? 2 : 1;  // groups whose steps a lane makes: K p .. (p modulo NB)
   const Cache4Side& sd = a.side[blockIdx.y];
   const int p = threadIdx.x & 3;
   const uint32_t row = blockIdx.x * 64u + (threadIdx.x >> 2);
   const uint32_t H = static_cast<uint32_t>(a.num_kv_heads);
-  const uint32_t tok = row / H, h = row - tok * H;
+  const uint32_t tok = a.heads_shift >= 0 ? row >> a.heads_shift : row / H, h = row - tok * H;
   if (tok >= static_cast<uint32_t>(a.num_tokens)) return;  // (all four lanes of a row)
   const int64_t slot = a.slot_mapping[tok];
   const uint16_t* src = sd.rows + tok * sd.row_tok + h * sd.row_head + 8 * p;
@@ -100,34 +87,83 @@ __global__ __launch_bounds__(256) void k_cache_write4(Cache4Args a) {
   for (int j = 0; j < NB; ++j) u[j] = ld16_once(src + 32 * j);
   if (slot < 0 || slot >= a.num_slots) return;
   int64_t blk, off;
-  split_slot(slot, a.block_size, blk, off);
-  const FixedScale fixed(sd.t ? sd.t[h * sd.t_head] : 1.0f);
-  uint32_t word[NB];
-  uint32_t b[4][NB];  // bytes (dim pair, group)
+  if (a.block_shift >= 0) {
+    blk = slot >> a.block_shift;
+    off = slot & (a.block_size - 1);
+  } else {
+    split_slot(slot, a.block_size, blk, off);
+  }
+  const float rt = sd.t ? 1.0f / sd.t[h * sd.t_head] : 1.0f;
+  float x[NB][8], hi[NB], lo[NB], most = 0.0f;
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     const uint32_t uw[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
-    float x[8];
+    bool nan = false;
+    hi[j] = -INFINITY;
+    lo[j] = INFINITY;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      x[2 * e] = T::to_f32(static_cast<uint16_t>(uw[e]));
-      x[2 * e + 1] = T::to_f32(static_cast<uint16_t>(uw[e] >> 16));
+      float* y = &x[j][2 * e];
+      y[0] = T::to_f32(static_cast<uint16_t>(uw[e])) * rt;
+      y[1] = T::to_f32(static_cast<uint16_t>(uw[e] >> 16)) * rt;
+      nan = nan || __builtin_isunordered(y[0], y[1]);
+      hi[j] = fmaxf(hi[j], fmaxf(y[0], y[1]));
+      lo[j] = fminf(lo[j], fminf(y[0], y[1]));
     }
-    if (sd.t) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = fixed.divide(x[e]);
-    }
-    word[j] = quantise_group(x);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      b[e][j] = static_cast<uint32_t>(fmaf(16.0f, x[2 * e + 1], x[2 * e]));
+    most = larger(most, larger(hi[j], -lo[j]));
+    hi[j] = __builtin_amdgcn_fmed3f(hi[j], -kInt4Most, kInt4Most);
+    lo[j] = __builtin_amdgcn_fmed3f(lo[j], -kInt4Most, kInt4Most);
+    hi[j] = quad_max(nan ? INFINITY : hi[j]);
+    lo[j] = -quad_max(-lo[j]);
   }
-  uint32_t w[NB];
+  // (seldom: elements past what a group holds, whose quotients may be infinite)
+  if (__ballot(most > kInt4Most) != 0) {
+    asm volatile("");
 #pragma unroll
-  for (int i = 0; i < NB; ++i) {
-    const int at = 4 * i;  // the piece's bytes at .. at + 3
-    w[i] = b[at / NB][at % NB] | b[(at + 1) / NB][(at + 1) % NB] << 8 |
-           b[(at + 2) / NB][(at + 2) % NB] << 16 | b[(at + 3) / NB][(at + 3) % NB] << 24;
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[j][e] = __builtin_amdgcn_fmed3f(x[j][e], -kInt4Most, kInt4Most);
+  }
+  GroupStep mine[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    float gh = hi[k], gl = lo[k];
+#pragma unroll
+    for (int j = 1; j < NB / K; ++j) {
+      const bool is = (p & (NB / K - 1)) == j;
+      gh = is ? hi[K * j + k] : gh;
+      gl = is ? lo[K * j + k] : gl;
+    }
+    mine[k] = group_step(gh, gl);
+  }
+  uint32_t w[NB] = {};  // the piece's bytes: dim pair e of group j at e NB + j
+  const auto codes = [&](auto jc) {
+    constexpr int j = decltype(jc)::value;
+    const GroupStep& m = mine[j % K];
+    const float s = quad_from<j / K>(m.s), r = quad_from<j / K>(m.r), z = quad_from<j / K>(m.z);
+    const float z15 = z + 15.0f, z17 = 17.0f * z;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float n[2];  // codes + z
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        n[i] = rintf(__builtin_amdgcn_fmed3f(quotient(x[j][2 * e + i], s, r), z, z15));
+      const int at = e * NB + j;
+      w[at >> 2] = __builtin_amdgcn_cvt_pk_u8_f32(fmaf(16.0f, n[1], n[0] - z17), at & 3, w[at >> 2]);
+    }
+  };
+  codes(IntC<0>{});
+  codes(IntC<1>{});
+  if constexpr (NB >= 4) {
+    codes(IntC<2>{});
+    codes(IntC<3>{});
+  }
+  if constexpr (NB == 8) {
+    codes(IntC<4>{});
+    codes(IntC<5>{});
+    codes(IntC<6>{});
+    codes(IntC<7>{});
   }
   uint8_t* dst = sd.cache + blk * sd.block + off * sd.slot + h * sd.head + 4 * NB * p;
   if constexpr (NB == 2) {
@@ -137,22 +173,19 @@ __global__ __launch_bounds__(256) void k_cache_write4(Cache4Args a) {
     for (int i = 0; i < NB / 4; ++i)
       st16_once(dst + 16 * i, make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
   }
-  // lane p stores the words of groups p (NB / 4) ..; with two groups lanes 0 and 1 one each
-  uint16_t* g = sd.g.p + blk * sd.g.sb + h * sd.g.sh + off * NB;
-  if constexpr (NB == 8) {
-    const uint32_t x01 = word[0] | word[1] << 16, x23 = word[2] | word[3] << 16;
-    const uint32_t x45 = word[4] | word[5] << 16, x67 = word[6] | word[7] << 16;
-    *reinterpret_cast<uint32_t*>(g + 2 * p) = p < 2 ? (p ? x23 : x01) : p == 2 ? x45 : x67;
-  } else if constexpr (NB == 4) {
-    g[p] = static_cast<uint16_t>(p < 2 ? (p ? word[1] : word[0]) : p == 2 ? word[2] : word[3]);
-  } else if (p < 2) {
-    g[p] = static_cast<uint16_t>(p ? word[1] : word[0]);
-  }
+  uint16_t* g = sd.g.p + blk * sd.g.sb + h * sd.g.sh + off * NB + K * p;
+  if constexpr (K == 2)
+    *reinterpret_cast<uint32_t*>(g) = mine[0].word | static_cast<uint32_t>(mine[1].word) << 16;
+  else if (p < NB)
+    *g = mine[0].word;
 }
 
-hipError_t launch_kv_cache_write4(const Cache4Args& a, int dtype, hipStream_t s) {
+hipError_t launch_kv_cache_write4(Cache4Args a, int dtype, hipStream_t s) {
   const int64_t rows = static_cast<int64_t>(a.num_tokens) * a.num_kv_heads;
   if (rows <= 0) return hipSuccess;
+  const auto shift = [](int n) { return (n & (n - 1)) == 0 ? 31 - __builtin_clz(n) : -1; };
+  a.heads_shift = shift(a.num_kv_heads);
+  a.block_shift = shift(a.block_size);
   const dim3 g(static_cast<unsigned>((rows + 63) / 64), 2), b(256);
   with_head_dim(a.head_dim, [&](auto d) {
     constexpr int NB = decltype(d)::value / 32;
@@ -163,12 +196,16 @@ hipError_t launch_kv_cache_write4(const Cache4Args& a, int dtype, hipStream_t s)
   return hipGetLastError();
 }
 
-// tokens: of a workgroup; di, dh: tokens and heads from a thread's row to its next one,
-// 64 rows on
+// A workgroup takes the tokens that make up a pass of its 64 rows (131,072 tokens of 8 heads
+// of 128: 141 us; with two passes, the second's rows loaded before the first's are used, 154,
+// with four 177), and stores through L2, since a store covers half a cache line of each of 16
+// rows (past it: 169 us). 688 MB in 141 us are 4.9 TB/s, a copy's rate 5.15.
+// di, dh: tokens and heads from a thread's row to its next one, 64 rows on.
+constexpr int kGatherTokens = 64;
 template <typename T, int NB>
 __global__ __launch_bounds__(256) void k_cache_gather4(Cache4Args a, GatherArgs find, int tokens,
                                                        int di, int dh) {
-  __shared__ CachedToken s_at[kRowTokens];
+  __shared__ CachedToken s_at[kGatherTokens];
   const Cache4Side& sd = a.side[blockIdx.y];
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * tokens;
   const int n = static_cast<int>(min(static_cast<int64_t>(tokens), a.num_tokens - t0));
@@ -179,15 +216,13 @@ __global__ __launch_bounds__(256) void k_cache_gather4(Cache4Args a, GatherArgs 
   __syncthreads();
   const int p = threadIdx.x & 3, H = a.num_kv_heads;
   int i = static_cast<int>(threadIdx.x >> 2) / H, h = static_cast<int>(threadIdx.x >> 2) % H;
-  for (; i < n; i += di) {
+  while (i < n) {
     const CachedToken f = s_at[i];
     if (f.page != kSkip) {
       uint16_t* dst = sd.rows + (t0 + i) * sd.row_tok + h * sd.row_head + 8 * p;
-      const int64_t page = max(f.page, int64_t(0));
-      const int64_t in = f.page < 0 ? 0 : f.in;
-      const uint8_t* src = sd.cache + page * sd.block + in * sd.slot + h * sd.head + 4 * NB * p;
+      const int64_t page = max(f.page, int64_t(0)), in = f.page < 0 ? 0 : f.in;
       uint32_t w[NB], g[NB / 2];
-      load_piece<NB>(src, w);
+      load_piece<NB>(sd.cache + page * sd.block + in * sd.slot + h * sd.head + 4 * NB * p, w);
       load_words<NB>(sd.g.p + page * sd.g.sb + h * sd.g.sh + in * NB, g);
       const float t = sd.t ? sd.t[h * sd.t_head] : 1.0f;
 #pragma unroll
@@ -195,7 +230,7 @@ __global__ __launch_bounds__(256) void k_cache_gather4(Cache4Args a, GatherArgs 
         const uint32_t word = g[j >> 1] >> (16 * (j & 1));
         float s = static_cast<float>(
             __builtin_bit_cast(_Float16, static_cast<uint16_t>(word & 0x7f80u)));
-        if (f.page < 0) s = __uint_as_float(0x7fc00000u);
+        if (f.page == kNaN) s = __uint_as_float(0x7fc00000u);
         const float off = static_cast<float>(static_cast<int>(word & 0x7fu) - 64) * s;
         uint32_t y[4];
 #pragma unroll
@@ -205,9 +240,10 @@ __global__ __launch_bounds__(256) void k_cache_gather4(Cache4Args a, GatherArgs 
           const float lo = static_cast<float>(b & 15u), hi = static_cast<float>((b >> 4) & 15u);
           y[e] = pack2<T>(fmaf(lo, s, off) * t, fmaf(hi, s, off) * t);
         }
-        st16_once(dst + 32 * j, make_uint4(y[0], y[1], y[2], y[3]));
+        st16(dst + 32 * j, make_uint4(y[0], y[1], y[2], y[3]));
       }
     }
+    i += di;
     h += dh;
     if (h >= H) {
       h -= H;
@@ -219,8 +255,7 @@ __global__ __launch_bounds__(256) void k_cache_gather4(Cache4Args a, GatherArgs 
 hipError_t launch_kv_cache_gather4(const Cache4Args& a, const GatherArgs& find, int dtype,
                                    hipStream_t s) {
   if (a.num_tokens <= 0) return hipSuccess;
-  int tokens = kRowTokens;  // (as row_walk has them)
-  while (tokens > 1 && a.num_tokens / tokens < 1024) tokens /= 2;
+  const int tokens = a.num_kv_heads < kGatherTokens ? kGatherTokens / a.num_kv_heads : 1;
   const dim3 g(static_cast<unsigned>((a.num_tokens + tokens - 1) / tokens), 2), b(256);
   const int di = 64 / a.num_kv_heads, dh = 64 % a.num_kv_heads;
   with_head_dim(a.head_dim, [&](auto d) {
