@@ -752,10 +752,11 @@ int scales_valid(const fp_kv_scales& s, const char* what) {
   return FP_OK;
 }
 
-// The split and the argument block of a call over an 8- or 4-bit cache.
-int paged8_args(const fp_paged_args* a, int heads, int most, const fp_kv_scales& ks,
-                const fp_kv_scales& vs, void* ws, fp::Paged8Args* r, PagedSplit* sp) {
-  *sp = paged8_split(a, heads, most, &r->unit);
+// The argument block of a call over an 8- or 4-bit cache, split into units of `unit` keys.
+int paged8_args(const fp_paged_args* a, int heads, const PagedSplit& split, int unit,
+                const fp_kv_scales& ks, const fp_kv_scales& vs, void* ws, fp::Paged8Args* r) {
+  const PagedSplit* sp = &split;
+  r->unit = unit;
   // (the merge's launch holds fewer than 2^32 threads, 1024 for each head of a segment)
   if (!sp->many && sp->tiles * a->num_kv_heads >= int64_t(1) << 22)
     return fail(FP_E_UNSUPPORTED, "paged: %lld tiles of query rows in one call",
@@ -1035,6 +1036,26 @@ int steps_valid(const fp_steps_args* a) {
   return FP_OK;
 }
 
+// Many rows, 2,048 per sequence and more, up to head_dim 128: tiles of 256 rows, whose keys a
+// workgroup of eight waves converts once, one workgroup per CU; chunks for about 256 of them.
+// With tiles of 128 and of 256 rows: 2,048 new tokens of each of 4 sequences of 4,096 ..
+// 6,144, 32 q / 8 kv heads of 128, 645 and 609 us; 512 of 8,192 111 and 101; 500 of 6,144,
+// 2,500 and 1,111, 28 / 4, 137 and 126; 300 of 5,500 and 1,200 80 and 89.
+PagedSplit paged4_split(const fp_paged_args* a, int heads, int* unit, int* row_tile) {
+  PagedSplit r = paged8_split(a, heads, paged4_groups(a->head_dim), unit);
+  *row_tile = 128;
+  const int64_t rows = a->num_tokens * (a->num_q_heads / a->num_kv_heads);
+  if (!r.many || a->head_dim > 128 || rows < int64_t(2048) * a->batch) return r;
+  *row_tile = 256;
+  r.tiles = row_tiles(a, 256);
+  const int64_t longest = static_cast<int64_t>(a->table_width) * a->block_size;
+  const int64_t wgs = std::max<int64_t>(1, r.tiles * a->num_kv_heads);
+  const int64_t nc = std::min<int64_t>((256 + wgs - 1) / wgs, (longest + 255) / 256);
+  r.nc = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(nc, fp::kPagedMaxChunks)));
+  r.bytes = partial_bytes(a, r.nc);
+  return r;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1192,9 +1213,10 @@ int fp_paged_attention_fp8(const fp_paged_fp8_args* a, void* ws, void* stream) {
   if (rc != FP_OK) return rc;
   if (a->base.num_tokens == 0) return FP_OK;
   fp::Paged8Args r;
-  PagedSplit sp;
-  const int prc = paged8_args(&a->base, paged8_heads(&a->base), fp::kPaged8Groups, a->k_scale, a->v_scale,
-                              ws, &r, &sp);
+  int unit;
+  const int heads = paged8_heads(&a->base);
+  const PagedSplit sp = paged8_split(&a->base, heads, fp::kPaged8Groups, &unit);
+  const int prc = paged8_args(&a->base, heads, sp, unit, a->k_scale, a->v_scale, ws, &r);
   if (prc != FP_OK) return prc;
   if (!r.vs.slot) {
     r.a.vscale = r.vs.p;
@@ -1283,8 +1305,9 @@ int fp_kv_cache_gather_int4(const fp_kv_gather_int4_args* a, void* stream) {
 }
 
 size_t fp_paged_int4_workspace_bytes(const fp_paged_int4_args* a) {
-  int unit;
-  return paged4_valid(a) == FP_OK ? paged8_split(&a->base, paged4_heads(&a->base), paged4_groups(a->base.head_dim), &unit).bytes : 0;
+  int unit, row_tile;
+  return paged4_valid(a) == FP_OK
+             ? paged4_split(&a->base, paged4_heads(&a->base), &unit, &row_tile).bytes : 0;
 }
 
 int fp_paged_attention_int4(const fp_paged_int4_args* a, void* ws, void* stream) {
@@ -1292,8 +1315,10 @@ int fp_paged_attention_int4(const fp_paged_int4_args* a, void* ws, void* stream)
   if (rc != FP_OK || a->base.num_tokens == 0) return rc;
   const int heads = paged4_heads(&a->base);
   fp::Paged4Args r;
-  PagedSplit sp;
-  if ((rc = paged8_args(&a->base, heads, paged4_groups(a->base.head_dim), a->k_scale, a->v_scale, ws, &r.p, &sp)) != FP_OK) return rc;
+  int unit;
+  const PagedSplit sp = paged4_split(&a->base, heads, &unit, &r.row_tile);
+  rc = paged8_args(&a->base, heads, sp, unit, a->k_scale, a->v_scale, ws, &r.p);
+  if (rc != FP_OK) return rc;
   r.p.a.vscale = r.p.vs.p;
   r.p.a.vscale_head = r.p.vs.sh;
   r.kg = groups(a->k_groups);

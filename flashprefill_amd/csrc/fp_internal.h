@@ -238,6 +238,7 @@ struct Paged4Args {
   Paged8Args p;  // (ks, vs: fixed)
   CacheGroups kg, vg;
   int32_t dtype;
+  int32_t row_tile;  // rows of a tile of many rows, 128 or 256
 };
 
 // Write of a 4-bit cache and its read-back (fp_kvcache4.hip), K in side[0], V in side[1].

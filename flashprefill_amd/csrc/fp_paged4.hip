@@ -576,16 +576,17 @@ __global__ __launch_bounds__(1024) void k_paged4_merge(Paged8Args pa) {
   merge_segments<T, D, HP, true>(pa);
 }
 
-// Many rows (prefill over a cached prefix): 128-row tiles as in k_paged8_rows. The 64 keys
-// of a tile are loaded into registers (16 keys by each wave, four lanes to a key, a tile
+// Many rows (prefill over a cached prefix): tiles of 32 rows of each of W waves as in
+// k_paged8_rows. The 64 keys of a tile are loaded into registers (four lanes to a key, a tile
 // ahead), made fp16 numbers once per workgroup and written to LDS, in which the dims of
 // every eight lie in the order of a piece ({0, 2, 1, 3, 4, 6, 5, 7}); so do the queries',
 // and O's come out in it. P enters as P 2^7, at most 2^15 (see kStep).
-template <int D, bool P16>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged4_rows(Paged4Args pa4) {
+template <int D, bool P16, int W>
+__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void k_paged4_rows(Paged4Args pa4) {
   constexpr int KT = 64, TT = KT / 32;
   constexpr int KS = D / 16, DT = D / 32, CH = D / 8;
   constexpr int NB = D / 32, GW = NB / 2;
+  constexpr int RT = 32 * W;  // rows of a tile
   constexpr float kStep = 8.0f, kPScaleRows = 7.0f;
   __shared__ uint4 sk[2][KT * CH];
   __shared__ uint4 sv[2][KT * CH];
@@ -595,7 +596,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged4_rows(Paged4Arg
   const int h = static_cast<int>(blockIdx.x % a.Hkv);
   const int64_t x = blockIdx.x / a.Hkv;
   const int c = static_cast<int>(blockIdx.y);
-  const PagedTile tile = paged_find(a, 128, x, -1);
+  const PagedTile tile = paged_find(a, RT, x, -1);
   if (tile.b < 0) return;
   const PagedSeq& sq = tile.s;
   const int nk = static_cast<int>(sq.nk), nq = sq.nq;
@@ -609,22 +610,22 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged4_rows(Paged4Arg
   const int half = lane >> 5, l32 = lane & 31;
   const int rows = nq * a.G;
   // (a sequence's last rows see most keys and start first)
-  const int tl = (rows + 127) / 128 - 1 - tile.tl;
+  const int tl = (rows + RT - 1) / RT - 1 - tile.tl;
 
   // this lane's query row and its last visible key
-  const int rr = tl * 128 + 32 * w + l32;
+  const int rr = tl * RT + 32 * w + l32;
   const bool rvalid = rr < rows;
   const int qi = (rvalid ? rr : rows - 1) / a.G;
   const int64_t tok = sq.q0 + qi;
   const int hq = h * a.G + (rvalid ? rr : rows - 1) % a.G;
   const int lim = nk - nq + qi;
   // the wave's first and last visible keys' bounds (wave-uniform)
-  const int r0 = min(tl * 128 + 32 * w, rows - 1);
-  const int r1 = min(tl * 128 + 32 * w + 31, rows - 1);
+  const int r0 = min(tl * RT + 32 * w, rows - 1);
+  const int r1 = min(tl * RT + 32 * w + 31, rows - 1);
   const int lim_lo = __builtin_amdgcn_readfirstlane(nk - nq + r0 / a.G);
   const int lim_hi = __builtin_amdgcn_readfirstlane(nk - nq + r1 / a.G);
   // keys past the last row of the tile are visible to none of its rows
-  const int last_row = min(tl * 128 + 127, rows - 1);
+  const int last_row = min(tl * RT + RT - 1, rows - 1);
   const int k1 = __builtin_amdgcn_readfirstlane(
       min(min(k0 + tile.chunk, nk), max(nk - nq + last_row / a.G + 1, 0)));
 
@@ -665,40 +666,48 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged4_rows(Paged4Arg
   const uint16_t* kg = pa4.kg.p + h * pa4.kg.sh;
   const uint16_t* vg = pa4.vg.p + h * pa4.vg.sh;
 
-  const int lkey = lane >> 2, lp = lane & 3;  // the lane's key of a load, and its piece
-  uint32_t kr[NB], vr[NB], kgr[GW], vgr[GW];
+  // the lane's key of a load, and its piece: of K and V, or of eight waves the first four of
+  // K and the others of V
+  const int lkey = 16 * (w & 3) + (lane >> 2), lp = lane & 3;
+  const bool takes_k = W == 4 || w < 4, takes_v = W == 4 || w >= 4;
+  constexpr int SIDES = W == 4 ? 2 : 1;
+  uint32_t cr[SIDES][NB], gr[SIDES][GW];
   const int last16 = (nk - 1) & ~15;
   // tile of keys base .. base + 63; keys past the sequence read its last 16-key
   // group (P16) or its last key
   auto load = [&](int base) {
     int64_t pg, in;
     if constexpr (P16) {
-      const int tb = min(base + 16 * w, last16);
+      const int tb = min(base + 16 * (w & 3), last16);
       pg = paged_page<true>(a, row, tb, bad);
-      in = (a.bs_shift >= 0 ? tb & (a.bs - 1) : tb % a.bs) + lkey;
+      in = (a.bs_shift >= 0 ? tb & (a.bs - 1) : tb % a.bs) + (lane >> 2);
     } else {
-      const int key = min(base + 16 * w + lkey, nk - 1);
+      const int key = min(base + lkey, nk - 1);
       pg = paged_page<false>(a, row, key, bad);
       in = key % a.bs;
     }
-    load_piece<NB>(kc + pg * a.kcb + in * a.kcs + 4 * NB * lp, kr);
-    load_piece<NB>(vc + pg * a.vcb + in * a.vcs + 4 * NB * lp, vr);
-    load_words<NB>(kg + pg * pa4.kg.sb + in * NB, kgr);
-    load_words<NB>(vg + pg * pa4.vg.sb + in * NB, vgr);
+    if (takes_k) {
+      load_piece<NB>(kc + pg * a.kcb + in * a.kcs + 4 * NB * lp, cr[0]);
+      load_words<NB>(kg + pg * pa4.kg.sb + in * NB, gr[0]);
+    }
+    if (takes_v) {
+      load_piece<NB>(vc + pg * a.vcb + in * a.vcs + 4 * NB * lp, cr[SIDES - 1]);
+      load_words<NB>(vg + pg * pa4.vg.sb + in * NB, gr[SIDES - 1]);
+    }
   };
   // as fp16 numbers into buffer `buf`; V of slots past the sequence is 0 (they may hold
   // anything)
   auto store = [&](int base, int buf) {
-    const int r = 16 * w + lkey;
-    if (base + r >= nk) {
+    if (takes_v && base + lkey >= nk) {
 #pragma unroll
-      for (int q = 0; q < GW; ++q) vgr[q] = 0u;
+      for (int q = 0; q < GW; ++q) gr[SIDES - 1][q] = 0u;
     }
+    uint4* to = takes_k ? sk[buf] : sv[buf];
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      const int at = r * CH + ((4 * j + lp) ^ swz<D>(r));
-      sk[buf][at] = piece_group<NB>(kr, kgr, j, k4);
-      sv[buf][at] = piece_group<NB>(vr, vgr, j, k4);
+      const int at = lkey * CH + ((4 * j + lp) ^ swz<D>(lkey));
+      to[at] = piece_group<NB>(cr[0], gr[0], j, k4);
+      if constexpr (SIDES == 2) sv[buf][at] = piece_group<NB>(cr[1], gr[1], j, k4);
     }
   };
   const int g16 = lane >> 4, i16 = lane & 15;
@@ -911,9 +920,20 @@ hipError_t launch_paged4(const Paged4Args& p, int head_dim, int hp, bool rows, i
       }
       return launch_few4<D, 1>(p, s);
     }
-    const dim3 grid(static_cast<unsigned>(tiles * a.Hkv), static_cast<unsigned>(a.nc)), b(256);
-    if (a.bs % 16 != 0) hipLaunchKernelGGL((k_paged4_rows<D, false>), grid, b, 0, s, p);
-    else hipLaunchKernelGGL((k_paged4_rows<D, true>), grid, b, 0, s, p);
+    const dim3 grid(static_cast<unsigned>(tiles * a.Hkv), static_cast<unsigned>(a.nc));
+    const auto run = [&](auto wc) {
+      constexpr int W = decltype(wc)::value;
+      if (a.bs % 16 != 0)
+        hipLaunchKernelGGL((k_paged4_rows<D, false, W>), grid, dim3(64 * W), 0, s, p);
+      else
+        hipLaunchKernelGGL((k_paged4_rows<D, true, W>), grid, dim3(64 * W), 0, s, p);
+    };
+    if constexpr (D < 256) {
+      if (p.row_tile == 256) run(IntC<8>{});
+      else run(IntC<4>{});
+    } else {
+      run(IntC<4>{});
+    }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nc <= 1) return e;
     return launch_paged_merge8(a, p.dtype, D, s);
