@@ -32,7 +32,7 @@ from . import _lib
 from . import vllm_backend as vb
 
 _SCALINGS = ("none", "linear", "ntk", "yarn", "bands")
-_ON_DEVICE: Dict[Tuple["Rotary", str], torch.Tensor] = {}
+_ON_DEVICE: Dict[Tuple["Rotary", torch.device], torch.Tensor] = {}
 
 
 @dataclass(frozen=True)
@@ -97,11 +97,19 @@ class Rotary:
         return f
 
     def on(self, device) -> torch.Tensor:
-        """``frequencies()`` on a device, made once."""
-        key = self, str(torch.device(device))
-        hit = _ON_DEVICE.get(key)
+        """``frequencies()`` on a device, made once: before a captured graph reads them.
+        (A trace or a dispatch mode gets its own, which nothing after it could use.)"""
+        if vb._torch_only():
+            return self.frequencies().to(device)
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        hit = _ON_DEVICE.get((self, device))
         if hit is None:
-            hit = _ON_DEVICE[key] = self.frequencies().to(device)
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"{self} is not on {device} yet: call on() before the capture")
+            with torch.inference_mode(False):
+                hit = _ON_DEVICE[self, device] = self.frequencies().to(device)
         return hit
 
 
@@ -161,13 +169,18 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
             raise ValueError("q, k, positions and frequencies must be on one GPU")
     outs = [out for _, _, out in pairs]
     vb._check_written(*outs)
+    torch_only = vb._torch_only()
+    if k is not None and q_out.numel() and k_out.numel() and \
+            vb._place(q_out, torch_only) == vb._place(k_out, torch_only):
+        raise ValueError("the outputs of q and k must be memory of their own")
     for _, x, out in pairs:  # its own input, or no input's memory
-        if out is x or (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()):
+        if out is x or (vb._place(out, torch_only) == vb._place(x, torch_only) and
+                        out.stride() == x.stride()):
             continue
         store = out.untyped_storage()._cdata
         if any(store == y.untyped_storage()._cdata for _, y, _ in pairs):
             raise ValueError("outputs must be the inputs themselves or memory of their own")
-    if vb._torch_only():
+    if torch_only:
         apply_rotary_reference(q, k, positions, frequencies, interleaved=interleaved,
                                amplitude=amplitude, inverse=inverse, q_out=q_out, k_out=k_out)
         return

@@ -95,7 +95,26 @@ def test_outputs_that_lie_in_an_input():
         apply_rotary(x[:3], None, pos[:3], f, q_out=x[1:])
     with pytest.raises(RuntimeError):
         apply_rotary(x, None, pos, f, q_out=x[:, :1].expand(4, 4, 64))
+    with pytest.raises(ValueError, match="own"):
+        apply_rotary(x, x, pos, f)
+    out = torch.empty_like(x)
+    with pytest.raises(ValueError, match="own"):
+        apply_rotary(x[:, :2], x[:, 2:], pos, f, q_out=out[:, :2], k_out=out[:, :2])
     apply_rotary(x[:0], None, pos[:0], f)
+
+
+def test_frequencies_on_the_current_device():
+    spec = Rotary(64, theta=54321.0)
+    graph, x = torch.cuda.CUDAGraph(), torch.zeros(1, device="cuda")
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="before the capture"):
+            spec.on("cuda")
+        x += 1
+    f = spec.on("cuda")
+    assert spec.on(f.device) is f and f.device.index == torch.cuda.current_device()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert x.item() == 1
 
 
 def test_capture_and_replay():

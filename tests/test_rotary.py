@@ -140,3 +140,31 @@ def _args(**kw):
 def test_the_c_entry_refuses(kw, code):
     assert _lib.load().fp_rotary(ctypes.byref(_args(**kw)), None) == code
     assert _lib.load().fp_rotary(None, None) == _lib.FP_E_INVALID_ARG
+
+
+def test_frequencies_made_in_a_dispatch_or_inference_mode():
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+    spec = Rotary(64, theta=12345.0)
+    with FakeTensorMode():
+        assert isinstance(spec.on("cpu"), FakeTensor)
+    with torch.inference_mode():
+        got = spec.on("cpu")
+    assert not isinstance(got, FakeTensor) and not got.is_inference()
+    assert torch.equal(got, spec.frequencies()) and spec.on(torch.device("cpu")) is got
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_a_trace_sees_torch_operations(own):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def step(q, k, pos, f):
+        out = dict(q_out=torch.empty_like(q), k_out=torch.empty_like(k)) if own else {}
+        apply_rotary(q, k, pos, f, **out)
+        return out.get("q_out", q)
+
+    with FakeTensorMode():
+        q, k = (torch.empty(4, h, 64, dtype=torch.bfloat16, device="cuda") for h in (4, 2))
+        pos, f = torch.arange(4, device="cuda"), torch.ones(32, dtype=torch.float64, device="cuda")
+        ops = [str(n.target) for n in make_fx(step)(q, k, pos, f).graph.nodes]
+    assert any("cos" in op for op in ops) and any("copy_" in op for op in ops)
