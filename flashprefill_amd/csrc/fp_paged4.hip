@@ -103,7 +103,7 @@ __device__ __forceinline__ void get2(const uint2* p, Step2& a, Step2& b) {
 // one segment's.
 //
 // Latency and bytes in flight bound it: 32 sequences of 300 .. 15,000 tokens, 8 KV heads of 128
-// (252 MB), take 63 us, 4.0 TB/s, and the merge 7. 16 of the 63 pass without any keys (the
+// (252 MB), take 62 us, 4.1 TB/s, and the merge 6. 16 of the 62 pass without any keys (the
 // search, the first page and key, the partials), the loads alone take 43 .. 50 beyond them
 // and the arithmetic alone 33 .. 36.
 //

@@ -15,13 +15,14 @@ __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
 }
 
 // entry x of a 32- or 64-bit (is64 1) integer array. Loads under no branch: several of
-// them are in flight together, where a branch makes the compiler wait for each.
+// them are in flight together, where a branch makes the compiler wait for each. (It makes one
+// of a choice between loaded values, so both go through a mask.)
 __device__ __forceinline__ int64_t ld_int(const void* p, int is64, int64_t x) {
   const int32_t* q = static_cast<const int32_t*>(p) + (x << is64);
   const int32_t lo = q[0], hi = q[is64];
-  return is64 ? static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 |
-                                     static_cast<uint32_t>(lo))
-              : static_cast<int64_t>(lo);
+  return static_cast<int64_t>(
+      static_cast<uint64_t>(static_cast<uint32_t>((hi & -is64) | (lo >> 31 & (is64 - 1)))) << 32 |
+      static_cast<uint32_t>(lo));
 }
 
 // One sequence as the workgroups see it. `bad`: more tokens than the block

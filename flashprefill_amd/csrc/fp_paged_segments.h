@@ -114,8 +114,8 @@ __device__ __forceinline__ Work find_work(const Paged8Args& pa, int wg, int64_t 
 // One head of a segment per workgroup of 16 waves: its rows' partials, weighted by
 // exp2(m - max m) and divided by their l. They are the first of workgroups w0 + 1 .. w1
 // and the first or last of w0. As many waves as there are share a row's partials.
-// SPLIT: a segment's rows are shared by the gridDim.y workgroups (a power of two) of its
-// head, each of which takes every gridDim.y-th.
+// SPLIT (the 4-bit form): a segment's rows are shared by the gridDim.y workgroups (a power of
+// two) of its head, each of which takes every gridDim.y-th.
 template <typename T, int D, int HP, bool SPLIT = false>
 __device__ __forceinline__ void merge_segments(const Paged8Args& pa) {
   constexpr int XD = D / 64;  // dims per lane
@@ -139,35 +139,110 @@ __device__ __forceinline__ void merge_segments(const Paged8Args& pa) {
   const int lgr = rows > 1 ? 32 - __clz(rows - 1) : 0;  // rows as a power of two
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int row = w & ((1 << lgr) - 1), share = 16 >> lgr;
+  const float vs = fixed_scale(pa.vs, h);
   if (row < rows) {
     const int first = 2 * w0 + (x0 != w0 * work.share);
     const auto part = [&](int j) {
       return static_cast<int64_t>(((j == 0 ? first : 2 * (w0 + j)) * HP + hh) * 16 +
                                   first_row + row * row_step);
     };
-    float M = -INFINITY;
-    for (int j = lane; j < n; j += 64) M = fmaxf(M, a.ml[2 * part(j)]);
-    M = wave_max(M);
+    float M = -INFINITY, L = 0.0f;
     vec acc{};
-    float L = 0.0f;
-#pragma unroll 4
-    for (int j = w >> lgr; j < n; j += share) {
-      const int64_t p = part(j);
-      const vec x = *reinterpret_cast<const vec*>(a.part + p * D + XD * lane);
-      const float m = a.ml[2 * p], l = a.ml[2 * p + 1];
-      // (2^-10: the sum over the partials, at most 768, stays finite)
-      static_assert(kPaged8Groups <= 1024, "weights");
-      const float f = m == -INFINITY ? 0.0f : 0x1p-10f * __builtin_amdgcn_exp2f(m - M);
-      L += m == -INFINITY ? l : f * l;
+    if constexpr (SPLIT) {
+      // What a row needs is on its way at once, since each trip is 1 to 2 us (other XCDs have
+      // just written it): a wave's lanes hold the weights of up to 64 of its partials, U
+      // of which are loaded at a time (past the last one, that again: its weight is 0 there).
+      // 256 rows of up to 14 partials: 6.0 us, loaded in three trips 7.0; 32 rows of 512
+      // partials 11.2 and 11.6 (one CU's loads of each, 128 KB).
+      constexpr int MM = 12;
+      static_assert(64 * MM >= 768, "partials");
+      const int j0 = w >> lgr, mine = j0 < n ? (n - 1 - j0) / share + 1 : 0;
+      // a row's partials lie `step` rows apart, but for the first, a workgroup's last, `odd`
+      // behind its place (fewer than 2 x 768 x 4 x 16 rows in all)
+      constexpr uint32_t step = 2 * HP * 16;
+      const uint32_t row0 = (2 * w0 * HP + hh) * 16 + first_row + row * row_step;
+      const uint32_t odd = (first & 1) * HP * 16;
+      const auto at = [&](int j) {
+        return row0 + static_cast<uint32_t>(j) * step + (j == 0 ? odd : 0u);
+      };
+      const auto run = [&](auto uc) {
+        constexpr int U = decltype(uc)::value, MU = U <= 4 ? 1 : MM;
+        vec x[U];
+        float m[MU], ml, l, f;
+        const uint32_t gap = share * step, last = at(j0 + share * (mine - 1));
+        const auto weights = [&](int k0) {
+          const uint32_t p = at(j0 + share * min(k0 + lane, mine - 1));
+          ml = a.ml[2 * p];
+          l = a.ml[2 * p + 1];
+        };
+        const auto load = [&](int k) {
+          uint32_t p = row0 + (j0 + share * k) * step;
 #pragma unroll
-      for (int q = 0; q < XD; ++q) acc[q] = fmaf(f, x[q], acc[q]);
+          for (int i = 0; i < U; ++i) {
+            const uint32_t r = i == 0 && k == 0 ? at(j0) : min(p, last);
+            x[i] = *reinterpret_cast<const vec*>(a.part + (r * D + XD * lane));
+            p += gap;
+          }
+        };
+        const auto weigh = [&](int k0) {
+          const bool in = k0 + lane < mine;
+          // (2^-10: the sum over the partials, at most 768, stays finite)
+          f = ml == -INFINITY || !in ? 0.0f : 0x1p-10f * __builtin_amdgcn_exp2f(ml - M);
+          L += !in ? 0.0f : ml == -INFINITY ? l : f * l;
+        };
+        const auto add = [&](int k) {
+#pragma unroll
+          for (int i = 0; i < U; ++i) {
+            const float fi =
+                __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (k + i) & 63));
+            // (partials are finite, or the row is NaN)
+#pragma unroll
+            for (int q = 0; q < XD; ++q) acc[q] = fmaf(fi, x[i][q], acc[q]);
+          }
+        };
+#pragma unroll
+        for (int i = 0; i < MU; ++i) m[i] = a.ml[2 * at(min(lane + 64 * i, n - 1))];
+        weights(0);
+        load(0);
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < MU; ++i) M = fmaxf(M, m[i]);
+        M = wave_max(M);
+        weigh(0);
+        add(0);
+        for (int k = U; k < mine; k += U) {
+          if (k % 64 == 0) weights(k);
+          load(k);
+          if (k % 64 == 0) weigh(k);
+          add(k);
+        }
+      };
+      if (mine > 0) {
+        if (n <= 64 && mine <= 4) run(IntC<4>{});
+        else run(IntC<XD == 1 ? 16 : 8>{});
+      }
+      L = static_cast<float>(wave_sum_d(L));
+    } else {
+      for (int j = lane; j < n; j += 64) M = fmaxf(M, a.ml[2 * part(j)]);
+      M = wave_max(M);
+#pragma unroll 4
+      for (int j = w >> lgr; j < n; j += share) {
+        const int64_t p = part(j);
+        const vec x = *reinterpret_cast<const vec*>(a.part + p * D + XD * lane);
+        const float m = a.ml[2 * p], l = a.ml[2 * p + 1];
+        // (2^-10: the sum over the partials, at most 768, stays finite)
+        static_assert(kPaged8Groups <= 1024, "weights");
+        const float f = m == -INFINITY ? 0.0f : 0x1p-10f * __builtin_amdgcn_exp2f(m - M);
+        L += m == -INFINITY ? l : f * l;
+#pragma unroll
+        for (int q = 0; q < XD; ++q) acc[q] = fmaf(f, x[q], acc[q]);
+      }
     }
 #pragma unroll
     for (int q = 0; q < XD; ++q) so[w][XD * lane + q] = acc[q];
     if (lane == 0) sl[w] = L;
   }
   __syncthreads();
-  const float vs = fixed_scale(pa.vs, h);
   for (int i = t; i < rows * D; i += 1024) {
     const int r = i / D, d = i % D;
     float o = 0.0f, L = 0.0f;
