@@ -12,9 +12,9 @@
 // ten dependent steps. Larger ones share the moves over the card: the sums in a
 // workspace, then a launch that returns pages, if any request can be finished, and one that
 // takes pages and writes tokens: 16 bytes for each, to be written at the memory's rate.
-// 256 requests with a token each: 8.8 us. 1,000 requests with 400,000 tokens, of which half can
-// be granted: 7.0 us for the sums (the requests' loads and two passes of prefix sums, one
-// after the other), 4.0 for the pages that return, 7.4 for those taken and the tokens.
+// 256 requests with a token each: 6.5 us. 1,000 requests with 400,000 tokens, of which half can
+// be granted: 4.8 us for the sums (the requests' loads and two passes of prefix sums, one
+// after the other), 4.0 for the pages that return, 7.0 for those taken and the tokens.
 #include "fp_internal.h"
 
 namespace fp {
@@ -22,28 +22,53 @@ namespace fp {
 constexpr int kStepThreads = 1024;
 constexpr int kStepWaves = kStepThreads / 64;
 
+// x of another lane, by DPP control C; 0 in the rows that mask M leaves out and where there is
+// no such lane
+template <int C, int M>
+__device__ __forceinline__ int32_t lane_of(int32_t x) {
+  return __builtin_amdgcn_update_dpp(0, x, C, M, 0xf, false);
+}
+template <int C, int M>
+__device__ __forceinline__ int64_t lane_of(int64_t x) {
+  return static_cast<int64_t>(
+      static_cast<uint64_t>(static_cast<uint32_t>(lane_of<C, M>(static_cast<int32_t>(x >> 32))))
+          << 32 |
+      static_cast<uint32_t>(lane_of<C, M>(static_cast<int32_t>(x))));
+}
+// sums over the lanes up to this one within rows of 16 lanes
+template <typename X>
+__device__ __forceinline__ X row_prefix(X x) {
+  x += lane_of<0x111, 0xf>(x);
+  x += lane_of<0x112, 0xf>(x);
+  x += lane_of<0x114, 0xf>(x);
+  return x + lane_of<0x118, 0xf>(x);
+}
+__device__ __forceinline__ int32_t at_lane(int32_t x, int l) {
+  return __builtin_amdgcn_readlane(x, l);
+}
+__device__ __forceinline__ int64_t at_lane(int64_t x, int l) {
+  return static_cast<int64_t>(
+      static_cast<uint64_t>(static_cast<uint32_t>(at_lane(static_cast<int32_t>(x >> 32), l)))
+          << 32 |
+      static_cast<uint32_t>(at_lane(static_cast<int32_t>(x), l)));
+}
 // Inclusive sums over the workgroup's threads; `total` is that of all of them. Every thread
-// calls it; s is its own buffer until the next barrier.
+// calls it; s is its own buffer until the next barrier. A step's sums are three of these and two
+// block_max, one after the other: with the exchanges through LDS, 7.0 us instead of 4.8.
 template <typename X>
 __device__ __forceinline__ X block_prefix(X x, int64_t* s, X& total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const X y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  x = row_prefix(x);
+  x += lane_of<0x142, 0xa>(x);  // (lane 15 of the row below, then lane 31 of the lower half)
+  x += lane_of<0x143, 0xc>(x);
   if (lane == 63) s[w] = x;
   __syncthreads();
-  X before = 0;
-  total = 0;
-#pragma unroll 4
-  for (int i = 0; i < kStepWaves; ++i) {
-    const X y = static_cast<X>(s[i]);
-    if (i < w) before += y;
-    total += y;
-  }
+  static_assert(kStepWaves == 16, "a row of lanes");
+  const X y = row_prefix(static_cast<X>(s[lane & 15]));
+  total = at_lane(y, 15);
   __syncthreads();
-  return x + before;
+  return x + (w > 0 ? at_lane(y, max(w - 1, 0)) : X(0));
 }
 __device__ __forceinline__ int32_t block_max(int32_t x, int64_t* s) {
   const int lane = threadIdx.x & 63;
@@ -51,8 +76,9 @@ __device__ __forceinline__ int32_t block_max(int32_t x, int64_t* s) {
   for (int o = 32; o > 0; o >>= 1) x = max(x, __shfl_xor(x, o));
   if (lane == 0) s[threadIdx.x >> 6] = x;
   __syncthreads();
-#pragma unroll 4
-  for (int i = 0; i < kStepWaves; ++i) x = max(x, static_cast<int32_t>(s[i]));
+  x = static_cast<int32_t>(s[lane & 15]);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) x = max(x, __shfl_xor(x, o));
   __syncthreads();
   return x;
 }
@@ -258,7 +284,7 @@ __global__ __launch_bounds__(256) void k_step_return(StepArgs a) {
            [&](int x, int lo, int hi) { return_page(a, m, k, x, lo, hi); });
 }
 // The first kStepMovers workgroups take pages, the others place tokens, kStepTokens each: one
-// for each thread (7.4 us for 400,000; with two 7.5, with four, one after the other, 9.9).
+// for each thread (400,000: with two, one after the other, 0.1 us more, with four 2.5).
 constexpr int kStepTokens = 256;
 __global__ __launch_bounds__(256) void k_step_place(StepArgs a) {
   const StepSums m = ws_sums(a);
