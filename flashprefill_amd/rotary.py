@@ -161,24 +161,26 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     tensors = [t for _, x, out in pairs for t in (x, out)]
     if forward_ad._current_level >= 0:
         vb._check_no_tangents(*tensors)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if not vb._none_requires_grad(*tensors):
         raise RuntimeError("q or k requires a gradient, which apply_rotary does not record: use "
                            "torch.no_grad()")
     for t in (*tensors, positions, frequencies):
-        if not t.is_cuda or t.device != dev:
+        if t.device != dev or dev.type != "cuda":
             raise ValueError("q, k, positions and frequencies must be on one GPU")
-    outs = [out for _, _, out in pairs]
+    outs = tensors[1::2]
     vb._check_written(*outs)
     torch_only = vb._torch_only()
     if k is not None and q_out.numel() and k_out.numel() and \
             vb._place(q_out, torch_only) == vb._place(k_out, torch_only):
         raise ValueError("the outputs of q and k must be memory of their own")
+    stores = None
     for _, x, out in pairs:  # its own input, or no input's memory
         if out is x or (vb._place(out, torch_only) == vb._place(x, torch_only) and
                         out.stride() == x.stride()):
             continue
-        store = out.untyped_storage()._cdata
-        if any(store == y.untyped_storage()._cdata for _, y, _ in pairs):
+        if stores is None:
+            stores = [y.untyped_storage()._cdata for y in tensors[::2]]
+        if out.untyped_storage()._cdata in stores:
             raise ValueError("outputs must be the inputs themselves or memory of their own")
     if torch_only:
         apply_rotary_reference(q, k, positions, frequencies, interleaved=interleaved,

@@ -77,11 +77,20 @@ def build_step_tables(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
         raise ValueError(f"block_size must be positive, got {block_size}")
     written = [block_table, free_pages, cu_seqlens, positions, slots, granted, seq_lens_out,
                num_free_out]
-    vb._check_written(*written)
+    vb._check_written(block_table)
+    for t in written:  # (the others are contiguous, and of integers)
+        if t.is_inference():
+            vb._check_written(t)
     torch_only = vb._torch_only()
-    others = [t for t in (seq_lens, num_free) if t is not seq_lens_out and t is not num_free_out]
-    named = [t for t in (*written, *others, new_lens, finished) if t is not None and t.numel()]
-    if len({vb._place(t, torch_only) for t in named}) < len(named):
+    named = [new_lens, *written]
+    if finished is not None:
+        named.append(finished)
+    if seq_lens is not seq_lens_out:
+        named.append(seq_lens)
+    if num_free is not num_free_out:
+        named.append(num_free)
+    places = [vb._place(t, True) if torch_only else t.data_ptr() for t in named if t.numel()]
+    if len(set(places)) < len(places):
         raise ValueError("the tensors must be memory of their own (but seq_lens_out and "
                          "num_free_out may be seq_lens and num_free)")
     if torch_only:
