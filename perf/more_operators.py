@@ -37,7 +37,7 @@ own = False
 
 DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 GROUP = 32  # elements that share a step and a zero point
-MOST = 16384.0  # the largest magnitude that a group holds
+MOST = 57344.0  # the largest magnitude that a group holds
 WIDEST = 56.0  # steps from zero to a group's largest magnitude, about
 
 
