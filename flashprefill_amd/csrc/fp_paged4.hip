@@ -7,11 +7,10 @@
 // No cached value is rounded on the way: u enters v_mfma_f32_*_f16 as it is, whatever the
 // type of q. bf16 queries become fp16 ones times a power of two f that takes their row's
 // largest finite element to 2^13 .. 2^14: exactly, but for elements below 2^-39 of it,
-// whose last bits fp16's subnormals lose. P enters as P 2^15 (many rows: up to P 2^15),
-// rounded to fp16 once: 2^-11 of each product, as much as rounding the output to fp16 may
-// lose (to bf16 2^-8) and less than a fiftieth of what rounding to 4 bits lost of the
-// cached value; a second part, of what the first lost, would cost few rows 20 of 290
-// vector instructions and many rows half as many MFMAs as P.V takes. l sums the rounded P.
+// whose last bits fp16's subnormals lose. P enters as P 2^15 (many rows: up to P 2^15) in two
+// fp16 parts, the second of what the first lost: all but 2^-22 of it, and 2^-25 of the
+// factored P where the parts are subnormal. (One part would be off by up to 2^-11, as much as
+// an fp16 output's rounding.)
 #include "fp_int4.h"
 #include "fp_paged_segments.h"
 
@@ -55,6 +54,22 @@ __device__ __forceinline__ int row_exponent(i16x2 m) { return (max(m.x, m.y) >> 
 __device__ __forceinline__ int factor_exponent(int biased) { return 13 - max(biased - 127, -106); }
 __device__ __forceinline__ uint32_t round2(float a, float b, bool bf) {
   return bf ? pack2<BF16>(a, b) : pack2<F16>(a, b);
+}
+
+// Two numbers as fp16 ones, hi, and what those lost, lo. minus_one: -1 that the compiler does
+// not see, so that x - hi is one instruction that converts.
+struct F16Parts {
+  uint32_t hi, lo;
+};
+__device__ __forceinline__ F16Parts f16_parts(float x0, float x1, float minus_one) {
+  const uint32_t hi = pack2<F16>(x0, x1);
+  const f16x2 h = __builtin_bit_cast(f16x2, hi);
+  return F16Parts{hi, pack2<F16>(fmaf(static_cast<float>(h[0]), minus_one, x0),
+                                 fmaf(static_cast<float>(h[1]), minus_one, x1))};
+}
+__device__ __forceinline__ float opaque(float x) {
+  asm volatile("" : "+s"(x));
+  return x;
 }
 
 // a key's dot product with a lane's share of a query row: groups of a piece, in fp32
@@ -103,7 +118,7 @@ __device__ __forceinline__ void get2(const uint2* p, Step2& a, Step2& b) {
 // one segment's.
 //
 // Latency and bytes in flight bound it: 32 sequences of 300 .. 15,000 tokens, 8 KV heads of 128
-// (252 MB), take 62 us, 4.1 TB/s, and the merge 6. 16 of the 62 pass without any keys (the
+// (252 MB), take 63 us, 4.0 TB/s, and the merge 6. 16 of the 62 pass without any keys (the
 // search, the first page and key, the partials), the loads alone take 43 .. 50 beyond them
 // and the arithmetic alone 33 .. 36.
 //
@@ -134,6 +149,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void k_paged4(Paged4Args pa4
   const Work work = find_work(pa, static_cast<int>(blockIdx.x), -1);
   if (work.b < 0) return;
   const Int4Consts k4;
+  const float minus_one = opaque(-1.0f);
   const bool bf = pa4.dtype == FP_DTYPE_BF16;
   const int t = threadIdx.x, lane = t & 63;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -391,16 +407,17 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void k_paged4(Paged4Args pa4
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
           s[j][v] = __builtin_amdgcn_exp2f(fmaf(s[j][v], scale, -ms));
+          l_part += s[j][v];
         }
 #pragma unroll
       for (int jj = 0; jj < TR; jj += 2) {  // 32 keys
-        uint32_t pw[4];  // keys 2 i, 2 i + 1 of this lane
+        F16Parts pw[4];  // keys 2 i, 2 i + 1 of this lane
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          pw[i] = pack2<F16>(s[jj + (i >> 1)][2 * (i & 1)], s[jj + (i >> 1)][2 * (i & 1) + 1]);
-          l_part = add_pair<F16>(pw[i], l_part);
-        }
-        const f16x8 pb = as_vec8<F16>(make_uint4(pw[0], pw[1], pw[2], pw[3]));
+        for (int i = 0; i < 4; ++i)
+          pw[i] = f16_parts(s[jj + (i >> 1)][2 * (i & 1)], s[jj + (i >> 1)][2 * (i & 1) + 1],
+                            minus_one);
+        const f16x8 ph = as_vec8<F16>(make_uint4(pw[0].hi, pw[1].hi, pw[2].hi, pw[3].hi));
+        const f16x8 pl = as_vec8<F16>(make_uint4(pw[0].lo, pw[1].lo, pw[2].lo, pw[3].lo));
 #pragma unroll
         for (int q = 0; q < GW; ++q) {  // groups 2 q and 2 q + 1
           uint32_t hv[4];
@@ -418,7 +435,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void k_paged4(Paged4Args pa4
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = values2<N>(hv[i], st[N >> 1][i], k4);
             const f16x8 va = as_vec8<F16>(make_uint4(x[0], x[1], x[2], x[3]));
-            acc[4 * q + N] = mfma16(va, pb, acc[4 * q + N]);
+            acc[4 * q + N] = mfma16(va, pl, acc[4 * q + N]);
+            acc[4 * q + N] = mfma16(va, ph, acc[4 * q + N]);
           };
           pv(IntC<0>{});
           pv(IntC<1>{});
@@ -506,7 +524,9 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void k_paged4(Paged4Args pa4
       sml[w][r16][1] = l;
     }
     __syncthreads();
-    const int orow = t >> 4, od = E * (t & 15);
+    int t2 = t;  // (places formed here, not kept across the loop)
+    asm volatile("" : "+v"(t2));
+    const int orow = t2 >> 4, od = E * (t2 & 15);
     const int orr = tl * 16 + orow;
     if (orr < nq * a.G) {
 #pragma unroll
@@ -552,7 +572,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void k_paged4(Paged4Args pa4
 #pragma unroll
           for (int e = 0; e < E; e += 4)
             *reinterpret_cast<float4*>(pp + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          if ((t & 15) == 0) {
+          if (od == 0) {
             a.ml[2 * part] = M;
             a.ml[2 * part + 1] = L;
           }
@@ -587,9 +607,11 @@ __global__ __launch_bounds__(1024) void k_paged4_merge(Paged8Args pa) {
 // every eight lie in the order of a piece ({0, 2, 1, 3, 4, 6, 5, 7}); so do the queries',
 // and O's come out in it. P enters as P 2^7, at most 2^15 (see kStep).
 //
-// The matrix instructions and the softmax between them bound it: 2,048 new tokens of each of 4
-// sequences of 4,096 .. 6,144, 32 q / 8 kv heads of 128, take 609 us, 852 TFLOP/s (an 8192^3
-// fp16 product reaches 1,159).
+// The matrix instructions bound it, of which P's second part is a third: 2,048 new tokens of
+// each of 4 sequences of 4,096 .. 6,144, 32 q / 8 kv heads of 128, take 737 us, 704 TFLOP/s,
+// 1,056 counting both parts (an 8192^3 fp16 product reaches 1,159). Without the second part
+// 604 us. The softmax of the next 16 keys between the products of these, in the compiler's
+// order or alternating with them: no gain (742).
 template <int D, bool P16, int W>
 __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void k_paged4_rows(Paged4Args pa4) {
   constexpr int KT = 64, TT = KT / 32;
@@ -612,6 +634,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void k_paged4_rows(Paged4
   const int k0 = c * tile.chunk;
   if (k0 >= nk && c > 0) return;
   const Int4Consts k4;
+  const float minus_one = opaque(-1.0f);
   const bool bf = pa4.dtype == FP_DTYPE_BF16;
   const bool single = nk <= tile.chunk;
   const int t = threadIdx.x, lane = t & 63;
@@ -779,16 +802,16 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void k_paged4_rows(Paged4
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           s[t4][v] = __builtin_amdgcn_exp2f(fmaf(s[t4][v], scale, -ms));
+          l_part += s[t4][v];
         }
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
-          uint32_t u[4];
+          F16Parts u[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            u[e] = pack2<F16>(s[t4][8 * hh + 2 * e], s[t4][8 * hh + 2 * e + 1]);
-            l_part = add_pair<F16>(u[e], l_part);
-          }
-          const f16x8 pb = as_vec8<F16>(make_uint4(u[0], u[1], u[2], u[3]));
+          for (int e = 0; e < 4; ++e)
+            u[e] = f16_parts(s[t4][8 * hh + 2 * e], s[t4][8 * hh + 2 * e + 1], minus_one);
+          const f16x8 ph = as_vec8<F16>(make_uint4(u[0].hi, u[1].hi, u[2].hi, u[3].hi));
+          const f16x8 pl = as_vec8<F16>(make_uint4(u[0].lo, u[1].lo, u[2].lo, u[3].lo));
           const uint16_t* sv16 = reinterpret_cast<const uint16_t*>(sv[buf]);
           const int r = 32 * t4 + 16 * hh + tr_row;
           __builtin_amdgcn_sched_barrier(0);
@@ -796,7 +819,10 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void k_paged4_rows(Paged4
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) va[dt] = read_vt<F16, D>(sv16, r, 32 * dt + tr_col);
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt) o[dt] = F16::mfma32(va[dt], pb, o[dt]);
+          for (int dt = 0; dt < DT; ++dt) o[dt] = F16::mfma32(va[dt], pl, o[dt]);
+          // (a dim tile's two products apart: the second would wait for the first)
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[dt] = F16::mfma32(va[dt], ph, o[dt]);
         }
       }
     }
