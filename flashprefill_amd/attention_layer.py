@@ -25,7 +25,7 @@ import torch
 
 from . import _lib
 from .flashprefill_varlen_func import flash_prefill_varlen_func
-from .rotary import Rotary, apply_rotary, apply_rotary_reference
+from .rotary import Rotary, apply_rotary, rotated
 
 
 def positions_from_cu_seqlens(cu_seqlens: torch.Tensor, total: int) -> torch.Tensor:
@@ -177,15 +177,18 @@ class PrefillAttention(torch.nn.Module):
 
     def project_qkv_rotary(self, q, k, v, pos):
         """The norms, where there are any, in torch, then ``self.rotary``: one kernel, in
-        place on the projection or its norms, on the GPU."""
+        place on the projection or its norms, on the GPU (no derivative: inputs that require
+        one are refused there); for other types, and on the CPU, torch operations that
+        autograd differentiates."""
         if self.qk_norm:
             q = rms_norm_heads(q, self.q_norm, self.rms_eps)
             k = rms_norm_heads(k, self.k_norm, self.rms_eps)
-        on_gpu = q.is_cuda and q.dtype in (torch.bfloat16, torch.float16)
-        rotate = apply_rotary if on_gpu else apply_rotary_reference
-        rotate(q, k, pos.to(q.device), self.rotary.on(q.device),
-               interleaved=self.rotary.interleaved, amplitude=self.rotary.amplitude)
-        return q, k, v
+        how = dict(interleaved=self.rotary.interleaved, amplitude=self.rotary.amplitude)
+        pos, f = pos.to(q.device), self.rotary.on(q.device)
+        if q.is_cuda and q.dtype in (torch.bfloat16, torch.float16):
+            apply_rotary(q, k, pos, f, **how)
+            return q, k, v
+        return rotated(q, pos, f, **how), rotated(k, pos, f, **how), v
 
     def project_qkv_reference(self, q, k, v, pos):
         """The torch composition of the same steps (the fused kernel's

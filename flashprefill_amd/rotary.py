@@ -197,23 +197,31 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     torch.autograd.graph.increment_version(outs)
 
 
-@torch.no_grad()
-def apply_rotary_reference(q, k, positions, frequencies, *, interleaved=False, amplitude=1.0,
-                           inverse=False, q_out=None, k_out=None) -> None:
-    """The torch composition of ``apply_rotary``: angles in 64 bits, cosines and sines and
-    the rotation in 32, rounded once."""
+def rotated(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, *,
+            interleaved: bool = False, amplitude: float = 1.0, inverse: bool = False
+            ) -> torch.Tensor:
+    """Rows x (tokens, heads, d) as ``apply_rotary`` turns them, in a tensor of its own, of
+    torch operations that record a derivative: angles in 64 bits, cosines and sines and the
+    rotation in 32, rounded once."""
     angle = positions.double().view(-1, 1) * frequencies.to(positions.device)
     cos, sin = ((f(angle) * amplitude).float().unsqueeze(1) for f in (torch.cos, torch.sin))
     if inverse:
         sin = -sin
     n = frequencies.numel()
+    z = x.float()
+    part = z[..., :2 * n]
+    a, b = (part[..., 0::2], part[..., 1::2]) if interleaved else (part[..., :n], part[..., n:])
+    u, v = a * cos - b * sin, b * cos + a * sin
+    part = torch.stack([u, v], -1).flatten(-2) if interleaved else torch.cat([u, v], -1)
+    return torch.cat([part, z[..., 2 * n:]], -1).to(x.dtype)
+
+
+@torch.no_grad()
+def apply_rotary_reference(q, k, positions, frequencies, *, interleaved=False, amplitude=1.0,
+                           inverse=False, q_out=None, k_out=None) -> None:
+    """The torch composition of ``apply_rotary``, in place or into the outputs as there."""
     for x, out in ((q, q_out), (k, k_out)):
-        if x is None:
-            continue
-        y = x if out is None else out
-        z = x.float()
-        part = z[..., :2 * n]
-        a, b = (part[..., 0::2], part[..., 1::2]) if interleaved else (part[..., :n], part[..., n:])
-        u, v = a * cos - b * sin, b * cos + a * sin
-        part = torch.stack([u, v], -1).flatten(-2) if interleaved else torch.cat([u, v], -1)
-        y.copy_(torch.cat([part, z[..., 2 * n:]], -1))
+        if x is not None:
+            (x if out is None else out).copy_(
+                rotated(x, positions, frequencies, interleaved=interleaved, amplitude=amplitude,
+                        inverse=inverse))
