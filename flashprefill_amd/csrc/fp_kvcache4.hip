@@ -22,6 +22,29 @@ __device__ __forceinline__ float quotient(float x, float y, float r) {
   return fmaf(-fmaf(q, y, -x), r, q);
 }
 
+// x / t, rounded as a division rounds it, up to magnitudes of 2^15 (larger ones stay that): two
+// steps of the above make it so where no product comes near the ends of fp32's range (Markstein,
+// Computation of elementary functions on the IBM RISC System/6000, 1990; of an |x| below 2^-102
+// the quotient, below 2^-42, is nothing beside any step), other scales divide.
+__device__ __forceinline__ void divide8(float (&x)[8], float t, float r) {
+  if (fabsf(t) >= 0x1p-60f && fabsf(t) <= 0x1p60f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float y = x[e] * r;
+      const float q = fmaf(-fmaf(y, t, -x[e]), r, y);
+      x[e] = fabsf(y) < 0x1p15f ? fmaf(-fmaf(q, t, -x[e]), r, q) : y;  // (a NaN stays)
+    }
+  } else {
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) {
+      const float y = x[0] / t;
+#pragma unroll
+      for (int i = 0; i < 7; ++i) x[i] = x[i + 1];
+      x[7] = y;
+    }
+  }
+}
+
 // The larger of two numbers, as the median of them and infinity: fmaxf would first quiet
 // each, since they might be signalling NaN.
 __device__ __forceinline__ float larger(float a, float b) {
@@ -93,7 +116,7 @@ __global__ __launch_bounds__(256) void k_cache_write4(Cache4Args a) {
   } else {
     split_slot(slot, a.block_size, blk, off);
   }
-  const float rt = sd.t ? 1.0f / sd.t[h * sd.t_head] : 1.0f;
+  const float t = sd.t ? sd.t[h * sd.t_head] : 1.0f, rt = 1.0f / t;
   float x[NB][8], hi[NB], lo[NB], most = 0.0f;
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
@@ -103,9 +126,13 @@ __global__ __launch_bounds__(256) void k_cache_write4(Cache4Args a) {
     lo[j] = INFINITY;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      float* y = &x[j][2 * e];
-      y[0] = T::to_f32(static_cast<uint16_t>(uw[e])) * rt;
-      y[1] = T::to_f32(static_cast<uint16_t>(uw[e] >> 16)) * rt;
+      x[j][2 * e] = T::to_f32(static_cast<uint16_t>(uw[e]));
+      x[j][2 * e + 1] = T::to_f32(static_cast<uint16_t>(uw[e] >> 16));
+    }
+    if (sd.t) divide8(x[j], t, rt);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float* y = &x[j][2 * e];
       nan = nan || __builtin_isunordered(y[0], y[1]);
       hi[j] = fmaxf(hi[j], fmaxf(y[0], y[1]));
       lo[j] = fminf(lo[j], fminf(y[0], y[1]));

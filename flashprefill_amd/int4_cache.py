@@ -133,8 +133,7 @@ def reshape_and_cache_int4(key: torch.Tensor, value: torch.Tensor, key_cache: to
     mapping's length is the number of tokens written, negative slots (and those past the
     cache) are skipped.
 
-    With x' = x (1 / t) (t: the fixed scale, its reciprocal rounded to fp32) within +-16384,
-    infinities too, and lo and hi a group's smallest and largest x', every rounding to
+    With x' = x / t (t: the fixed scale) within +-16384, infinities too, and lo and hi a group's smallest and largest x', every rounding to
     nearest even:
 
     * s = max((hi - lo) / 15, hi / 56, -lo / 56) to 4 significant bits (below 2^-14 to a
@@ -176,7 +175,7 @@ def quantise_int4(x: torch.Tensor, scale: Optional[torch.Tensor] = None
     n, h, d = x.shape
     x = x.float()
     if scale is not None:
-        x = x * (1 / scale.to(x.device)).view(1, -1, 1)
+        x = x / scale.to(x.device).view(1, -1, 1)
     x = x.view(n, h, d // GROUP, GROUP).clamp(-_MOST, _MOST)
     lo, hi = x.amin(-1), x.amax(-1)  # (NaN where there is one)
     # (tensors, by which torch divides: by numbers it multiplies with their reciprocals)

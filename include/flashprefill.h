@@ -322,7 +322,7 @@ typedef struct fp_kv_groups {
 
 /* fp_kv_cache_write into a 4-bit cache. The cache strides count bytes (multiples of 16;
  * bases 16-byte aligned); the groups are aligned to head_dim / 16 bytes, with strides of
- * whole slots; scales are fixed. With x' = x (1 / t), the reciprocal rounded to fp32, clamped to
+ * whole slots; scales are fixed. With x' = x / t clamped to
  * +-16384, lo and hi the group's smallest and largest x', rounding to nearest even throughout:
  *   s = max((hi - lo) / 15, hi / 56, -lo / 56) rounded to 4 significant bits (to a multiple
  *   of 2^-17 below 2^-14),  z = lo / s rounded, within -64 .. 63,
