@@ -8,8 +8,8 @@
 // heads: it finds their n cosines and sines once, in LDS, then rotates the heads' rows, a
 // thread V pairs at a time. An angle of position 131,071 needs 17 bits before the point:
 // p f is a 64-bit product, reduced in 64 bits to |r| <= pi / 4 (two parts of pi / 2, so that
-// the second product's rounding is below 2^-50 for angles to 2^30), and only r is rounded to
-// fp32, off by at most 2^-25. 65,536 tokens of 32 heads of 128, the pairs of half of each
+// the second product's rounding is below 2^-50 for angles to 2^30), and cosine and sine of r, of
+// the series of Taylor in 64 bits, times A are rounded to fp32 once. 65,536 tokens of 32 heads of 128, the pairs of half of each
 // rotated: 220 us, 4.9 TB/s (a copy reaches 5.15).
 #include <algorithm>
 
@@ -24,13 +24,24 @@ __device__ __forceinline__ float2 turn(int64_t p, double f, float amplitude, boo
   const double k = rint(t * 0x1.45f306dc9c883p-1);      // 2 / pi
   double r = fma(-k, 0x1.921fb54442d18p+0, t);          // pi / 2, its first 53 bits
   r = fma(-k, 0x1.1a62633145c07p-54, r);                // and the next
-  float s, c;
-  sincosf(static_cast<float>(r), &s, &c);
+  // (the terms left out are below 2^-54 of the sine and 2^-49 of the cosine)
+  const double z = r * r;
+  double s = -1.0 / 1307674368000.0, c = 1.0 / 20922789888000.0;  // 15!, 16!
+  constexpr double kSin[6] = {1.0 / 6227020800.0, -1.0 / 39916800.0, 1.0 / 362880.0,
+                              -1.0 / 5040.0,      1.0 / 120.0,       -1.0 / 6.0};
+  constexpr double kCos[7] = {-1.0 / 87178291200.0, 1.0 / 479001600.0, -1.0 / 3628800.0,
+                              1.0 / 40320.0,        -1.0 / 720.0,      1.0 / 24.0, -0.5};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) s = fma(s, z, kSin[i]);
+#pragma unroll
+  for (int i = 0; i < 7; ++i) c = fma(c, z, kCos[i]);
+  s = fma(s * z, r, r);
+  c = fma(c, z, 1.0);
   const int q = static_cast<int>(static_cast<int64_t>(k) & 3);
-  const float sn = q & 1 ? c : s, cs = q & 1 ? s : c;
-  const float sign_s = (q & 2) != 0 ? -amplitude : amplitude;
-  const float sign_c = q == 1 || q == 2 ? -amplitude : amplitude;
-  return make_float2(sign_c * cs, (inverse ? -sign_s : sign_s) * sn);
+  const double sn = q & 1 ? c : s, cs = q & 1 ? s : c, a = amplitude;
+  const double sign_s = (q & 2) != 0 ? -a : a, sign_c = q == 1 || q == 2 ? -a : a;
+  return make_float2(static_cast<float>(sign_c * cs),
+                     static_cast<float>((inverse ? -sign_s : sign_s) * sn));
 }
 
 // x / d for x, d < 2^16 and m = ceil(2^32 / d): m d is less than d above 2^32, so that the
