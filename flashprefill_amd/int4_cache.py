@@ -54,7 +54,8 @@ def int4_cache_views(cache: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     if d not in _HEAD_DIMS or int4_row_bytes(d) != row:
         raise ValueError(f"rows of {row} bytes: int4_row_bytes(head_dim) are "
                          f"{[int4_row_bytes(x) for x in _HEAD_DIMS]}")
-    if cache.stride()[1:] != (hkv * row, row, 1):
+    if any(size > 1 and stride != want for size, stride, want in
+           zip(cache.shape[1:], cache.stride()[1:], (hkv * row, row, 1))):
         raise ValueError("the pages of a 4-bit cache must be contiguous")
     n = bs * hkv * (d // 2)
     pages = cache.view(nb, bs * hkv * row)
