@@ -14,7 +14,7 @@
 // takes pages and writes tokens: 16 bytes for each, to be written at the memory's rate.
 // 256 requests with a token each: 6.5 us. 1,000 requests with 400,000 tokens, of which half can
 // be granted: 4.8 us for the sums (the requests' loads and two passes of prefix sums, one
-// after the other), 4.0 for the pages that return, 7.0 for those taken and the tokens.
+// after the other), 4.4 for the pages that return, 7.0 for those taken and the tokens.
 #include "fp_internal.h"
 
 namespace fp {
@@ -201,6 +201,30 @@ __device__ __forceinline__ void return_page(const StepArgs& a, const StepSums& m
   const int j = x - (r > 0 ? m.back[r - 1] : 0);
   a.free_pages[k.free + x] = a.block_table[r * a.table_stride + j];
 }
+// The same for all n of them, by a workgroup whose waves take 1,024 neighbours at a time: the whole
+// wave searches for their rows, and of one row's a lane's sixteen loads are on their way together.
+__device__ __forceinline__ void return_pages(const StepArgs& a, const StepSums& m,
+                                             const StepTotals& k, int n) {
+  constexpr int U = 16;
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  for (int64_t x0 = w * 64 * U; x0 < n; x0 += kStepThreads * U) {
+    const int first = static_cast<int>(x0), last = static_cast<int>(min(x0 + 64 * U, int64_t(n))) - 1;
+    const int lo = find_row64(m.back, 0, a.R - 1, first);
+    const int hi = find_row64(m.back, lo, a.R - 1, last);
+    if (lo < hi) {
+      for (int x = first + lane; x <= last; x += 64) return_page(a, m, k, x, lo, hi);
+      continue;
+    }
+    const int32_t* row = a.block_table + lo * a.table_stride - (lo > 0 ? m.back[lo - 1] : 0);
+    int32_t page[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) page[u] = row[min(first + 64 * u + lane, last)];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (first + 64 * u + lane <= last) a.free_pages[k.free + first + 64 * u + lane] = page[u];
+  }
+}
 // page x of the step's, from the free ones' end
 __device__ __forceinline__ void take_page(const StepArgs& a, const StepSums& m,
                                           const StepTotals& k, int x, int lo, int hi) {
@@ -243,6 +267,12 @@ __device__ __forceinline__ void place_token(const StepArgs& a, const StepSums& m
   a.slots[x] = slot;
 }
 
+// Pages that come back up to here go by return_page, a thread each, past it by return_pages (256
+// requests, 4,000, 16,000, 24,576, 65,536 and 491,520 pages of rows of 250 .. 8,192: 9.0, 17, 23.5,
+// 53 and 356 us the first way, 17, 16, 9.5, 14.5 and 68 the second, whose waves move rows of few
+// pages no faster). How many come back the host cannot know, and three launches would cost
+// every step that ends none 3 us.
+constexpr int kStepFew = 16384;
 // A whole step by one workgroup, of at most kStepThreads requests
 __global__ __launch_bounds__(kStepThreads) void k_step_one(StepArgs a) {
   __shared__ int64_t s[kStepWaves];
@@ -252,7 +282,12 @@ __global__ __launch_bounds__(kStepThreads) void k_step_one(StepArgs a) {
   const StepTotals k = step_sums(a, m, cu, granted, s);
   __syncthreads();
   const int t = static_cast<int>(threadIdx.x);
-  for (int x = t; x < k.all - k.free; x += kStepThreads) return_page(a, m, k, x, 0, a.R - 1);
+  const int back_n = k.all - k.free;
+  if (back_n > kStepFew) {
+    return_pages(a, m, k, back_n);
+  } else {
+    for (int x = t; x < back_n; x += kStepThreads) return_page(a, m, k, x, 0, a.R - 1);
+  }
   __syncthreads();  // (pages taken may have just come back, rows that gave them be written)
   for (int x = t; x < k.taken; x += kStepThreads) take_page(a, m, k, x, 0, a.R - 1);
   for (int64_t x = t; x < a.N; x += kStepThreads) place_token(a, m, k, x, 0, a.R - 1);
