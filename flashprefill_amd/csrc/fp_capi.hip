@@ -959,7 +959,8 @@ int paged4_valid(const fp_paged_int4_args* a) {
 // Workgroups that share a 4-bit call's keys: what the card holds, three for each CU up to
 // head_dim 128 and two at 256 (32 sequences of 300 .. 15,000 tokens, 8 KV heads of 128: 63 us
 // with three, 69 with two, 71 with four in turn).
-int paged4_groups(int head_dim) { return head_dim == 256 ? 512 : 768; }
+int paged4_groups(int head_dim) { return head_dim == 256 ? 512 : fp::kPaged4Groups; }
+static_assert(512 <= fp::kPaged4Groups, "the merge takes partials of at most that many");
 
 // A 4-bit call is split as an 8-bit one, but that a segment of few rows serves as many KV
 // heads as make up a cache line of 128 bytes, unless segments are whole and too few to fill

@@ -177,6 +177,7 @@ struct CacheScales {
 // shares are whole units of `unit` keys, min_share at least; a.part and a.ml hold two
 // partials of 16 rows for each (null: a segment is one workgroup's).
 constexpr int kPaged8Groups = 512;  // workgroups where they share the keys, at most
+constexpr int kPaged4Groups = 768;  // the same over a 4-bit cache
 struct Paged8Args {
   PagedArgs a;
   CacheScales ks, vs;

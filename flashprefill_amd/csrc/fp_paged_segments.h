@@ -1,6 +1,7 @@
 // How few query rows over a paged cache of 8- or 4-bit values are shared out
 // (fp_paged8.hip, fp_paged4.hip): the segments of a call, the workgroups' shares of their
-// keys, and the merge of the segments that several workgroups served.
+// keys, and the merge of the segments that several workgroups served (k_paged8_merge,
+// k_paged4_merge).
 #pragma once
 
 #include "fp_float8.h"
@@ -17,7 +18,7 @@ namespace fp {
 // few leaves workgroups without any: 1,620 units are four for each of 405 workgroups of 512,
 // 2,152 five for each of 431, 13,728 twenty-seven for each of 509. A segment that is one workgroup's is written out,
 // the others as partials (O, m, l), the first and the last of a workgroup at most, which
-// k_paged8_merge combines. Where the table has room for few keys, a unit is a whole
+// merge_segments combines. Where the table has room for few keys, a unit is a whole
 // sequence and a segment a workgroup's: no merge.
 struct Work {
   int total, share;  // units of the call, and of a workgroup
@@ -154,11 +155,10 @@ __device__ __forceinline__ void merge_segments(const Paged8Args& pa) {
       // of which are loaded at a time (past the last one, that again: its weight is 0 there).
       // 256 rows of up to 14 partials: 6.0 us, loaded in three trips 7.0; 32 rows of 512
       // partials 11.2 and 11.6 (one CU's loads of each, 128 KB).
-      constexpr int MM = 12;
-      static_assert(64 * MM >= 768, "partials");
+      constexpr int MM = (kPaged4Groups + 63) / 64;
       const int j0 = w >> lgr, mine = j0 < n ? (n - 1 - j0) / share + 1 : 0;
       // a row's partials lie `step` rows apart, but for the first, a workgroup's last, `odd`
-      // behind its place (fewer than 2 x 768 x 4 x 16 rows in all)
+      // behind its place (fewer than 2 kPaged4Groups x 4 x 16 rows in all)
       constexpr uint32_t step = 2 * HP * 16;
       const uint32_t row0 = (2 * w0 * HP + hh) * 16 + first_row + row * row_step;
       const uint32_t odd = (first & 1) * HP * 16;
@@ -187,6 +187,7 @@ __device__ __forceinline__ void merge_segments(const Paged8Args& pa) {
         const auto weigh = [&](int k0) {
           const bool in = k0 + lane < mine;
           // (2^-10: the sum over the partials, at most 768, stays finite)
+          static_assert(kPaged4Groups <= 1024, "weights");
           f = ml == -INFINITY || !in ? 0.0f : 0x1p-10f * __builtin_amdgcn_exp2f(ml - M);
           L += !in ? 0.0f : ml == -INFINITY ? l : f * l;
         };
@@ -230,7 +231,7 @@ __device__ __forceinline__ void merge_segments(const Paged8Args& pa) {
         const int64_t p = part(j);
         const vec x = *reinterpret_cast<const vec*>(a.part + p * D + XD * lane);
         const float m = a.ml[2 * p], l = a.ml[2 * p + 1];
-        // (2^-10: the sum over the partials, at most 768, stays finite)
+        // (2^-10: the sum over the partials, at most 512, stays finite)
         static_assert(kPaged8Groups <= 1024, "weights");
         const float f = m == -INFINITY ? 0.0f : 0x1p-10f * __builtin_amdgcn_exp2f(m - M);
         L += m == -INFINITY ? l : f * l;
