@@ -7,7 +7,7 @@
 // numbers whose other bits are those of 16 read as 16 + c (one shift, one and-or), and
 //   s (c + z) = (16 + c) s + (z - 16) s
 // is one packed fma, in which nothing is rounded: (z - 16) s has 7 + 4 bits, and magnitudes
-// up to 16384 with steps up to 2176 keep it below 52,288.
+// up to 16384 with steps up to 2304 (a 15th of 32768, rounded) keep it to 52,992.
 //
 // Byte m (d / 32) + j of a row holds dims 32 j + 2 m and 32 j + 2 m + 1: what a lane of 16
 // loads (d / 32 bytes of each key) are two dims of every group, so that a matrix
