@@ -85,10 +85,13 @@ def build_step_tables(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
     named = [new_lens, *written]
     if finished is not None:
         named.append(finished)
-    places = [vb._place(t, torch_only) for t in named if t.numel()]
-    for t, out in ((seq_lens, seq_lens_out), (num_free, num_free_out)):
-        if t is not out and t.numel() and vb._place(t, torch_only) != vb._place(out, torch_only):
-            places.append(vb._place(t, torch_only))
+    if seq_lens is not seq_lens_out and \
+            vb._place(seq_lens, torch_only) != vb._place(seq_lens_out, torch_only):
+        named.append(seq_lens)
+    if num_free is not num_free_out and \
+            vb._place(num_free, torch_only) != vb._place(num_free_out, torch_only):
+        named.append(num_free)
+    places = [vb._place(t, True) if torch_only else t.data_ptr() for t in named if t.numel()]
     if len(set(places)) < len(places):
         raise ValueError("the tensors must be memory of their own (but seq_lens_out and "
                          "num_free_out may be seq_lens and num_free)")
