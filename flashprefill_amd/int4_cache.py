@@ -318,8 +318,10 @@ def _kernel_takes(query, key_cache, value_cache, key_groups, value_groups, out, 
     nb, bs, hkv, _ = key_cache.shape
     if not vb._call_fits(query, out, (nb, bs, hkv, d), cu, used, table):
         return False
+    if key_cache.device != query.device or value_cache.device != query.device:
+        return False
     for t in (query, key_cache, value_cache, out):
-        if t.device != query.device or not vb._rows_ok(t, True):
+        if not vb._rows_ok(t, True):
             return False
     words = 8 if bs % 16 == 0 else d // GROUP
     for g in (key_groups, value_groups):

@@ -114,6 +114,13 @@ def _scale_args(scale: Optional[torch.Tensor], device) -> tuple:
     return _lib.FpKvScales(scale.data_ptr(), 0, 1 if scale.numel() > 1 else 0, 0), scale
 
 
+def _on_device(t: torch.Tensor, device) -> torch.Tensor:
+    """t there and contiguous; itself, without torch's calls, where it is that already."""
+    if t.device != device:
+        t = t.to(device)
+    return t if t.is_contiguous() else t.contiguous()
+
+
 def _launch(device: torch.device, fn, *args) -> None:
     """``fn(*args, stream)`` with ``device`` current, on torch's current stream there."""
     if torch.cuda.current_device() == device.index:
@@ -288,9 +295,11 @@ def _check_sequences(cu_seqlens, block_table, starts, rows: int) -> int:
     if B < 0 or block_table.shape[0] < B or (starts is not None and starts.numel() < B):
         raise ValueError(f"block_table {tuple(block_table.shape)} or starts do not match "
                          f"{B} sequences")
-    for name, t in (("cu_seqlens", cu_seqlens), ("block_table", block_table), ("starts", starts)):
-        if t is not None and t.dtype not in _INDEX:
-            raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
+    if cu_seqlens.dtype not in _INDEX or block_table.dtype not in _INDEX or \
+            (starts is not None and starts.dtype not in _INDEX):
+        raise ValueError(f"cu_seqlens, block_table and starts must be int32 or int64, got "
+                         f"{cu_seqlens.dtype}, {block_table.dtype} and "
+                         f"{None if starts is None else starts.dtype}")
     if not cu_seqlens.is_cuda:  # known without a synchronisation
         at = cu_seqlens.tolist()
         if at[0] < 0 or at[-1] > rows or any(x > y for x, y in zip(at, at[1:])):
@@ -300,11 +309,13 @@ def _check_sequences(cu_seqlens, block_table, starts, rows: int) -> int:
 
 def _sequence_args(cu_seqlens, block_table, starts, device):
     """The trailing fields of the read-backs' arguments, and the tensors they name."""
-    cu, table = cu_seqlens.to(device).contiguous(), block_table.to(device)
+    cu, table = _on_device(cu_seqlens, device), block_table
+    if table.device != device:
+        table = table.to(device)
     if table.stride(1) != 1:
         table = table.contiguous()
     if starts is not None:
-        starts = starts.to(device).contiguous()
+        starts = _on_device(starts, device)
     return (cu.numel() - 1, table.shape[1], cu.dtype == torch.int64, table.dtype == torch.int64,
             starts is not None and starts.dtype == torch.int64, cu.data_ptr(), table.data_ptr(),
             None if starts is None else starts.data_ptr(), table.stride(0)), (cu, table, starts)
@@ -517,10 +528,11 @@ def _paged_kernel_takes(query, key_cache, value_cache, out, cu, used, table, k_s
             not _call_fits(query, out, key_cache.shape, cu, used, table):
         return False
     dev, dt, cdt = query.device, query.dtype, key_cache.dtype
-    if cdt != dt and cdt not in _FORMATS:
+    if (cdt != dt and cdt not in _FORMATS) or value_cache.dtype != cdt or \
+            key_cache.device != dev or value_cache.device != dev:
         return False
-    for t, want in ((query, dt), (key_cache, cdt), (value_cache, cdt), (out, dt)):
-        if t.dtype != want or t.device != dev or not _rows_ok(t, cdt != dt):
+    for t in (query, key_cache, value_cache, out):
+        if not _rows_ok(t, cdt != dt):
             return False
     bs = key_cache.shape[1]
     for s in (k_scale, v_scale):
@@ -537,8 +549,9 @@ def _paged_args(query, key_cache, value_cache, out, cu, used, table, scale, d):
     dev = query.device
     nb, bs, hkv, _ = key_cache.shape
     T, hq = query.shape[:2]
-    cu, used = cu.to(dev).contiguous(), used.to(dev).contiguous()
-    table = table.to(dev)
+    cu, used = _on_device(cu, dev), _on_device(used, dev)
+    if table.device != dev:
+        table = table.to(dev)
     if table.stride(1) != 1:
         table = table.contiguous()
     return _lib.FpPagedArgs(
