@@ -957,8 +957,8 @@ int paged4_valid(const fp_paged_int4_args* a) {
 }
 
 // Workgroups that share a 4-bit call's keys: what the card holds, three for each CU up to
-// head_dim 128 and two at 256 (32 sequences of 300 .. 15,000 tokens, 8 KV heads of 128: 63 us
-// with three, 69 with two, 71 with four in turn).
+// head_dim 128 and two at 256 (32 sequences of 300 .. 15,000 tokens, 8 KV heads of 128, in
+// replayed graphs: 75 us with three, 83 with two).
 int paged4_groups(int head_dim) { return head_dim == 256 ? 512 : fp::kPaged4Groups; }
 static_assert(512 <= fp::kPaged4Groups, "the merge takes partials of at most that many");
 
@@ -1045,8 +1045,9 @@ int steps_valid(const fp_steps_args* a) {
 // Many rows, 2,048 per sequence and more, up to head_dim 128: tiles of 256 rows, whose keys a
 // workgroup of eight waves converts once, one workgroup per CU; chunks for about 256 of them.
 // With tiles of 128 and of 256 rows: 2,048 new tokens of each of 4 sequences of 4,096 ..
-// 6,144, 32 q / 8 kv heads of 128, 645 and 609 us; 512 of 8,192 111 and 101; 500 of 6,144,
-// 2,500 and 1,111, 28 / 4, 137 and 126; 300 of 5,500 and 1,200 80 and 89.
+// 6,144, 32 q / 8 kv heads of 128, 780 and 737 us; 512 of 8,192 128 and 117; 500 of 6,144,
+// 2,500 and 1,111, 28 / 4, 157 and 142; 1,000 of 9,000 and 7,000, 16 / 4 of 64, 159 and 156;
+// 300 of 5,500 and 1,200 (fewer rows than that) 80 and 89 while P was in one part.
 PagedSplit paged4_split(const fp_paged_args* a, int heads, int* unit, int* row_tile) {
   PagedSplit r = paged8_split(a, heads, paged4_groups(a->head_dim), unit);
   *row_tile = 128;

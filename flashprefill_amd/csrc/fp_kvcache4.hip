@@ -92,7 +92,7 @@ __device__ __forceinline__ GroupStep group_step(float hi, float lo) {
                                              : bits | static_cast<uint32_t>(static_cast<int>(z) + 64))};
 }
 
-// 131,072 tokens of 8 heads of 128 with scales, 688 MB: 167 us, 4.1 TB/s (a copy's rate
+// 131,072 tokens of 8 heads of 128 with scales, 688 MB: 169 us, 4.1 TB/s (a copy's rate
 // 5.15); without the group words' 8 bytes a row, scattered over the heads' pages, 157.
 template <typename T, int NB>
 __global__ __launch_bounds__(256) void k_cache_write4(Cache4Args a) {

@@ -118,9 +118,10 @@ __device__ __forceinline__ void get2(const uint2* p, Step2& a, Step2& b) {
 // one segment's.
 //
 // Latency and bytes in flight bound it: 32 sequences of 300 .. 15,000 tokens, 8 KV heads of 128
-// (252 MB), take 63 us, 4.0 TB/s, and the merge 6. 16 of the 62 pass without any keys (the
+// (252 MB), take 63 us, 4.0 TB/s, and the merge 6. 16 of the 63 pass without any keys (the
 // search, the first page and key, the partials), the loads alone take 43 .. 50 beyond them
-// and the arithmetic alone 33 .. 36.
+// and the arithmetic alone 35 .. 40. P's second part is 1 to 2 us of it (5 in kernels that run
+// apart from each other, at lower clocks).
 //
 // P16: the page size is a multiple of 16, so a 16-key tile lies in one page: a wave looks
 // up 64 of them at a time, one per lane, and reads a tile's place from its lane. Other

@@ -14,7 +14,7 @@
 // takes pages and writes tokens: 16 bytes for each, to be written at the memory's rate.
 // 256 requests with a token each: 6.5 us. 1,000 requests with 400,000 tokens, of which half can
 // be granted: 4.8 us for the sums (the requests' loads and two passes of prefix sums, one
-// after the other), 4.4 for the pages that return, 7.0 for those taken and the tokens.
+// after the other), 4.2 to 4.4 for the pages that return, 7.0 for those taken and the tokens.
 #include "fp_internal.h"
 
 namespace fp {
