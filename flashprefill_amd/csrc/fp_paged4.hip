@@ -798,12 +798,15 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void k_paged4_rows(Paged4
       }
       // rows with no visible key yet keep m = -inf: their P is 0
       const float ms = m_run == -INFINITY ? 0.0f : m_run - kPScaleRows;
+      // (a tile's sum apart from l: in one chain over thousands of keys fp32's roundings would be
+      // most of what outputs are off by)
+      float l_tile[4] = {};
 #pragma unroll
       for (int t4 = 0; t4 < TT; ++t4) {
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           s[t4][v] = __builtin_amdgcn_exp2f(fmaf(s[t4][v], scale, -ms));
-          l_part += s[t4][v];
+          l_tile[v & 3] += s[t4][v];
         }
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
@@ -826,6 +829,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void k_paged4_rows(Paged4
           for (int dt = 0; dt < DT; ++dt) o[dt] = F16::mfma32(va[dt], ph, o[dt]);
         }
       }
+      l_part += (l_tile[0] + l_tile[1]) + (l_tile[2] + l_tile[3]);
     }
     if (more) store(base + KT, buf ^ 1);
   }

@@ -353,8 +353,8 @@ int fp_kv_cache_gather_int4(const fp_kv_gather_int4_args* a, void* stream);
  * aligned, with strides of multiples of 8 words. No cached value is rounded: keys and
  * values enter the products as fp16 numbers, t multiplies fp32 scores and rows. bf16
  * queries enter them as fp16 numbers times a power of two of their row: what lies below
- * 2^-39 of the row's largest element is lost. Probabilities are held to 2^-22
- * in fp16 parts. */
+ * 2^-39 of the row's largest element is lost. Probabilities are held to 2^-22,
+ * those below 2^-10 of a row's largest to 2^-32 of that, in fp16 parts. */
 typedef struct fp_paged_int4_args {
   fp_paged_args base;
   fp_kv_groups k_groups, v_groups;
