@@ -120,8 +120,8 @@ __device__ __forceinline__ void get2(const uint2* p, Step2& a, Step2& b) {
 // Latency and bytes in flight bound it: 32 sequences of 300 .. 15,000 tokens, 8 KV heads of 128
 // (252 MB), take 63 us, 4.0 TB/s, and the merge 6. 16 of the 63 pass without any keys (the
 // search, the first page and key, the partials), the loads alone take 43 .. 50 beyond them
-// and the arithmetic alone 35 .. 40. P's second part is 1 to 2 us of it (5 in kernels that run
-// apart from each other, at lower clocks).
+// and the arithmetic alone 33 .. 36 with P in one part; its second part is 1 to 2 us of the 63
+// (5 in kernels that run apart from each other, at lower clocks).
 //
 // P16: the page size is a multiple of 16, so a 16-key tile lies in one page: a wave looks
 // up 64 of them at a time, one per lane, and reads a tile's place from its lane. Other
@@ -608,10 +608,11 @@ __global__ __launch_bounds__(1024) void k_paged4_merge(Paged8Args pa) {
 // every eight lie in the order of a piece ({0, 2, 1, 3, 4, 6, 5, 7}); so do the queries',
 // and O's come out in it. P enters as P 2^7, at most 2^15 (see kStep).
 //
-// The matrix instructions bound it, of which P's second part is a third: 2,048 new tokens of
-// each of 4 sequences of 4,096 .. 6,144, 32 q / 8 kv heads of 128, take 737 us, 704 TFLOP/s,
-// 1,056 counting both parts (an 8192^3 fp16 product reaches 1,159). Without the second part
-// 604 us. The softmax of the next 16 keys between the products of these, in the compiler's
+// The matrix instructions (busy 45 % of the cycles, a third of it P's second part) and the vector
+// ones (issuing 48 %) bound it, one after the other in waves that a barrier keeps in step: 2,048
+// new tokens of each of 4 sequences of 4,096 .. 6,144, 32 q / 8 kv heads of 128, take 737 us, 704
+// TFLOP/s, 1,056 counting both parts (an 8192^3 fp16 product reaches 1,159). Without the second
+// part 604 us. The softmax of the next 16 keys between the products of these, in the compiler's
 // order or alternating with them: no gain (742).
 template <int D, bool P16, int W>
 __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void k_paged4_rows(Paged4Args pa4) {
